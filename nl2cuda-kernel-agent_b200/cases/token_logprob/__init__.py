@@ -1,0 +1,23 @@
+"""Token log-probability case: exposes ``CASE`` for the harness."""
+import os
+
+from framework.case import Case
+from cases.token_logprob import config
+from cases.token_logprob.reference import make_inputs, reference_forward
+
+
+def _description():
+    with open(os.path.join(os.path.dirname(os.path.abspath(__file__)), "description.md"),
+              encoding="utf-8") as f:
+        return f.read()
+
+
+CASE = Case(
+    name="token_logprob",
+    description=_description(),
+    params={"ignore_index": config.IGNORE_INDEX},
+    grad_inputs=["logits"],
+    dtype=config.DTYPE,
+    make_inputs=make_inputs,
+    reference_forward=reference_forward,
+)

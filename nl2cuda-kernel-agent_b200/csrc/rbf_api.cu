@@ -9,6 +9,7 @@
 #include <mutex>
 
 #include "../../include/cos_sm100.h"
+#include "lm_common.cuh"
 #include "rbf_common.cuh"
 #include "rbf_kernels.cuh"
 
@@ -45,11 +46,10 @@ WaitConfig wait_config_from_env() {
   return w;
 }
 
-namespace {
+static thread_local char g_detail[512] = "";
 
-thread_local char g_detail[512] = "";
-
-int set_detail(int status, const char* what, cudaError_t e = cudaSuccess) {
+// Shared with lm_api.cu (declared in lm_common.cuh): one detail string for every C entry.
+int set_detail(int status, const char* what, cudaError_t e) {
   if (e != cudaSuccess) {
     std::snprintf(g_detail, sizeof(g_detail), "%s: %s (%s)", what, cudaGetErrorName(e),
                   cudaGetErrorString(e));
@@ -58,6 +58,8 @@ int set_detail(int status, const char* what, cudaError_t e = cudaSuccess) {
   }
   return status;
 }
+
+namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -89,6 +91,8 @@ int check_shape(int64_t N, int64_t M, int64_t D, float gamma, bool is_eps = fals
   return RBF_OK;
 }
 
+}  // namespace
+
 // The current device must be an sm_100 part (B200).  Cached per device ordinal.
 int check_device() {
   int dev = -1;
@@ -114,12 +118,14 @@ int check_device() {
   return st;
 }
 
-size_t backward_extra_bytes(int64_t N, int64_t M, int64_t D) {
-  return backward_scratch_bytes(N, M, D);
-}
-
 int cuda_status(cudaError_t e, const char* what) {
   return e == cudaSuccess ? RBF_OK : set_detail(RBF_ERR_CUDA, what, e);
+}
+
+namespace {
+
+size_t backward_extra_bytes(int64_t N, int64_t M, int64_t D) {
+  return backward_scratch_bytes(N, M, D);
 }
 
 int forward_impl(const float* X, const float* Y, float* K, int64_t N, int64_t M, int64_t D,

@@ -27,5 +27,6 @@ PROTOCOL = Protocol()
 
 def dtype_of(name):
     import torch
-    table = {"float32": torch.float32, "float64": torch.float64, "float16": torch.float16}
+    table = {"float32": torch.float32, "float64": torch.float64, "float16": torch.float16,
+             "bfloat16": torch.bfloat16}
     return table[name]

@@ -1,0 +1,227 @@
+"""Layer norm on the GPU against a 64-bit implementation of its formulas."""
+import pytest
+import torch
+
+from lm_util import DTYPES, U32, assert_within, rounded
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-5
+
+
+def inputs(rows, D, dtype, wdtype, seed, offset=0.5):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def randn(*s):
+        return torch.randn(*s, device="cuda", generator=g)
+
+    x = (randn(rows, D) * 2 + offset).to(dtype)
+    return x, (1 + 0.3 * randn(D)).to(wdtype), (0.2 * randn(D)).to(wdtype), randn(rows, D).to(dtype)
+
+
+def formulas(x, w, b, dy, eps):
+    """(y, dx, dw, db, rstd) in fp64."""
+    x, dy = x.double(), dy.double()
+    D = x.size(1)
+    w = torch.ones(D, device=x.device).double() if w is None else w.double()
+    b = torch.zeros(D, device=x.device).double() if b is None else b.double()
+    mean = x.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + eps)
+    h = (x - mean) * rstd
+    g = dy * w
+    dx = rstd * (g - g.mean(1, keepdim=True) - h * (g * h).mean(1, keepdim=True))
+    return h * w + b, dx, (dy * h).sum(0), dy.sum(0), rstd
+
+
+def bounds(x, w, b, dy, want, dtype, wdtype):
+    """Errors of the fp32 arithmetic plus one rounding of each output.
+
+    A row's sums add at most 16 values in a lane and 10 levels of lanes and warps: 26 roundings,
+    each of at most U32 of the sum of absolute values.  So mean is off by 26 U32 mean|x| plus the
+    division, xh by that times rstd plus a few roundings of xh itself (the variance's relative
+    error halves in rstd): within e = 40 U32 (max|x| rstd + |xh|).  g's sums are off by 26 U32 of
+    mean|g| and of mean|g xh|, plus e times mean|g|.  Columns: every addend carries e, and the
+    sum of n rows at most (rows + 32) U32 of the absolute sum (a running sum, then a tree)."""
+    y, dx, dw, db, rstd = want
+    xd, dyd = x.double(), dy.double()
+    wd = torch.ones_like(xd[0]) if w is None else w.double()
+    bd = torch.zeros_like(wd) if b is None else b.double()
+    h = (xd - xd.mean(1, keepdim=True)) * rstd
+    e = 40 * U32 * (xd.abs().amax(1, keepdim=True) * rstd + h.abs())
+    g = dyd * wd
+    gm = g.abs().mean(1, keepdim=True)
+    gh = (g * h).abs().mean(1, keepdim=True)
+    em = e.mean(1, keepdim=True)
+    hm = (h * h).mean(1, keepdim=True).sqrt()
+    eg = 30 * U32 * (g.abs() + gm)
+    eh = e * gh + h.abs() * ((g.abs() * e).mean(1, keepdim=True) + 30 * U32 * (gh + gm * hm))
+    n = x.size(0)
+    return {
+        "y": e * wd.abs() + 3 * U32 * (h * wd).abs() + 2 * U32 * bd.abs() + rounded(y, dtype),
+        "dx": rstd * (eg + eh + em * gm * 0) + 30 * U32 * dx.abs() + rounded(dx, dtype),
+        "dw": (dyd.abs() * e).sum(0) + (n + 32) * U32 * (dyd * h).abs().sum(0) + rounded(dw, wdtype),
+        "db": (n + 32) * U32 * dyd.abs().sum(0) + rounded(db, wdtype),
+    }
+
+
+def check(x, w, b, dy, eps=EPS):
+    from cases.layernorm.op import layer_norm
+    wdtype = w.dtype if w is not None else b.dtype if b is not None else x.dtype
+    want = formulas(x, w, b, dy, eps)
+    bound = bounds(x, w, b, dy, want, x.dtype, wdtype)
+    leaves = [t.detach().requires_grad_(True) if t is not None else None for t in (x, w, b)]
+    y = layer_norm(*leaves, eps)
+    y.backward(dy)
+    assert y.dtype == x.dtype
+    assert_within("y", y, want[0], bound["y"])
+    assert_within("dx", leaves[0].grad, want[1], bound["dx"])
+    if w is not None:
+        assert_within("dw", leaves[1].grad, want[2], bound["dw"])
+    if b is not None:
+        assert_within("db", leaves[2].grad, want[3], bound["db"])
+    with torch.no_grad():
+        assert torch.equal(layer_norm(x, w, b, eps), y.detach())
+
+
+SHAPES = [(1, 1), (3, 2), (1, 48), (8, 64), (5, 127), (300, 128), (33, 255), (7, 256), (9, 257),
+          (40, 511), (40, 512), (600, 513), (3, 1000), (64, 1023), (65, 1024), (2, 2048),
+          (17, 4095), (513, 4096), (4, 6000), (3, 8192), (5, 8194), (2, 16383), (3, 16384),
+          (2, 16385), (5, 40000)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D", SHAPES)
+def test_against_formulas(rows, D, dtype, cuda_device):
+    check(*inputs(rows, D, dtype, dtype, rows * 31 + D))
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("rows,D", [(9, 130), (50, 1024), (3, 16384), (2, 20000)])
+def test_fp32_parameters(rows, D, dtype, cuda_device):
+    check(*inputs(rows, D, dtype, torch.float32, D))
+
+
+@pytest.mark.parametrize("has_w,has_b", [(True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("D", [96, 4096, 17000])
+def test_without_parameters(has_w, has_b, D, cuda_device):
+    x, w, b, dy = inputs(6, D, torch.bfloat16, torch.bfloat16, D)
+    check(x, w if has_w else None, b if has_b else None, dy)
+
+
+def test_large_offset_does_not_cancel(cuda_device):
+    """mean 1000 times the deviation: the two-pass variance keeps its digits (the bound scales
+    with max|x| rstd, a one-pass E[x^2] - mean^2 would be off by its square)."""
+    x, w, b, dy = inputs(20, 3000, torch.float32, torch.float32, 5, offset=2000.0)
+    check(x, w, b, dy)
+
+
+@pytest.mark.parametrize("rows,D", [(1000, 64), (40000, 136)])
+def test_many_rows(rows, D, cuda_device):
+    check(*inputs(rows, D, torch.float32, torch.float32, 77))
+
+
+def test_strided_and_broadcast_operands(cuda_device):
+    """Rows that lie apart, a transposed matrix, a misaligned slice, an expanded dy."""
+    from cases.layernorm.op import layer_norm
+    base, w, b, _ = inputs(60, 512, torch.bfloat16, torch.bfloat16, 3)
+    views = [base[:, :256], base[:, 3:259], base[::2, 8:264], base.t()[:256].t(),
+             base.view(12, 5, 512)[:, :, 100:356], base.view(12, 5, 512)[:, 2:4, :256]]
+    for v in views:
+        x = v.detach().requires_grad_(True)
+        ww, bb = (t[:256].detach().requires_grad_(True) for t in (w, b))
+        dy = torch.full((), 0.5, dtype=x.dtype, device="cuda").expand(x.shape)
+        y = layer_norm(x, ww, bb, EPS)
+        y.backward(dy)
+        flat = v.reshape(-1, 256).contiguous()
+        full = dy.reshape(-1, 256).contiguous()
+        want = formulas(flat, ww.detach(), bb.detach(), full, EPS)
+        bound = bounds(flat, ww.detach(), bb.detach(), full, want, x.dtype, x.dtype)
+        assert_within("y", y.reshape(-1, 256), want[0], bound["y"])
+        assert_within("dx", x.grad.reshape(-1, 256), want[1], bound["dx"])
+        assert_within("dw", ww.grad, want[2], bound["dw"])
+        assert_within("db", bb.grad, want[3], bound["db"])
+
+
+def test_empty_operands(cuda_device):
+    from cases.layernorm.op import layer_norm
+    x = torch.empty(0, 64, device="cuda", requires_grad=True)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    y = layer_norm(x, w, None, EPS)
+    y.sum().backward()
+    assert y.shape == (0, 64) and x.grad.shape == (0, 64)
+    assert torch.equal(w.grad, torch.zeros_like(w))
+    assert layer_norm(torch.empty(4, 0, device="cuda")).shape == (4, 0)
+
+
+def test_constant_rows_and_nan_stay_in_their_row(cuda_device):
+    from cases.layernorm.op import layer_norm
+    x, w, b, _ = inputs(8, 300, torch.float32, torch.float32, 9)
+    x[2] = 7.0
+    x[5, 10] = float("nan")
+    y = layer_norm(x, w, b, EPS)
+    assert torch.equal(y[2], b)
+    assert torch.isnan(y[5]).all()
+    assert torch.isfinite(y[[0, 1, 2, 3, 4, 6, 7]]).all()
+
+
+def test_equal_calls_give_equal_bits(cuda_device):
+    from cases.layernorm import native
+    x, w, b, dy = inputs(5000, 1000, torch.bfloat16, torch.float32, 1)
+    y, mean, rstd = native.ln_forward(x, w, b, EPS)
+    first = native.ln_backward(dy, x, w, mean, rstd)
+    for _ in range(3):
+        for a, c in zip(first, native.ln_backward(dy, x, w, mean, rstd)):
+            assert torch.equal(a, c)
+
+
+def test_gradient_against_differences(cuda_device):
+    """The directional derivative of sum(y * dy) by central differences of the fp64 formulas."""
+    from cases.layernorm.op import layer_norm
+    x, w, b, dy = inputs(6, 70, torch.float32, torch.float32, 21)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    layer_norm(*leaves, EPS).backward(dy)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for k in range(3):
+        v = torch.randn(leaves[k].shape, device="cuda", generator=g).double()
+        h = 1e-5
+        def f(s):
+            t = [u.detach().double() for u in leaves]
+            t[k] = t[k] + s * v
+            return float((formulas(*t, dy, EPS)[0] * dy.double()).sum())
+        want = (f(h) - f(-h)) / (2 * h)
+        got = float((leaves[k].grad.double() * v).sum())
+        # h^2 of the third derivative and fp64 cancellation (1e-16 / h) are below 1e-6 here.
+        assert abs(got - want) <= 1e-5 * (1 + float((leaves[k].grad.double().abs() * v.abs()).sum()))
+
+
+def test_other_stream_and_graph(cuda_device):
+    """On a side stream, and captured with its backward and replayed on new data."""
+    from cases.layernorm import native
+    x, w, b, dy = inputs(700, 768, torch.bfloat16, torch.bfloat16, 2)
+    want = native.ln_forward(x, w, b, EPS)
+    wantb = native.ln_backward(dy, x, w, want[1], want[2])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y, mean, rstd = native.ln_forward(x, w, b, EPS)
+        out = native.ln_backward(dy, x, w, mean, rstd)
+    s.synchronize()
+    assert torch.equal(y, want[0]) and all(torch.equal(p, q) for p, q in zip(out, wantb))
+    sx, sdy = torch.zeros_like(x), torch.zeros_like(dy)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, mean, rstd = native.ln_forward(sx, w, b, EPS)
+        out = native.ln_backward(sdy, sx, w, mean, rstd)
+    sx.copy_(x)
+    sdy.copy_(dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want[0]) and all(torch.equal(p, q) for p, q in zip(out, wantb))
+
+
+def test_verify_all_passes(cuda_device):
+    from cases.layernorm import CASE
+    from cases.layernorm.op import candidate
+    from framework.verify import verify_all
+    ok, report = verify_all(CASE, candidate, device="cuda")
+    assert ok, report
