@@ -97,6 +97,21 @@ RBF_API int policy_sm100_loss(const float* logprob, const float* old_logprob,
                               float kl_coef, int64_t ignore_index, void* workspace,
                               size_t workspace_bytes, rbf_stream_t stream);
 
+/* ---- orthogonalisation of an update ---------------------------------------------------------
+ * Newton-Schulz products on each of `batch` matrices G [rows, cols] (type dtype; rows contiguous,
+ * row_stride and matrix_stride elements apart):
+ *   X = G / (|G|_F + eps);  `steps` times:  A = X X^T,  X <- a X + (b A + c A^2) X
+ * (with X transposed where rows > cols; the result is the same), (a, b, c) = coefficients[step]
+ * (host memory, 3 * steps floats, read during the call).  out [batch, rows, cols] contiguous,
+ * type dtype; it must not overlap the update.  Products keep 22 bits of each operand and
+ * accumulate in fp32.  1 <= steps <= 32.  The workspace's first int is the device status word
+ * (rbf_sm100_read_status): 0, or 7 if a bounded device wait ran out and out is incomplete. */
+RBF_API size_t ortho_sm100_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int steps);
+RBF_API int ortho_sm100(const void* update, int64_t row_stride, int64_t matrix_stride, void* out,
+                        int64_t batch, int64_t rows, int64_t cols, const float* coefficients,
+                        int steps, float eps, int dtype, void* workspace, size_t workspace_bytes,
+                        rbf_stream_t stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

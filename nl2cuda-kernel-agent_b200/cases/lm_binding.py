@@ -33,6 +33,9 @@ _SIGNATURES = {
     "pref_sm100_loss": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _F, _F, _I64, _P, _SZ, _P]),
     "policy_sm100_loss": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I64, _I64, _F, _F, _F,
                                _I64, _P, _SZ, _P]),
+    "ortho_sm100_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I]),
+    "ortho_sm100": (_I, [_P, _I64, _I64, _P, _I64, _I64, _I64, ctypes.POINTER(_F), _I, _F, _I, _P,
+                         _SZ, _P]),
 }
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}

@@ -289,4 +289,48 @@ int policy_sm100_loss(const float* logprob, const float* old_logprob, const floa
   return cuda_status(launch_loss(a, false, as_stream(stream)), "policy loss launch");
 }
 
+size_t ortho_sm100_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int steps) {
+  if (batch < 0 || rows < 0 || cols < 0 || steps < 1 || steps > ortho_max_steps()) return 0;
+  return ortho_workspace_bytes(batch, rows, cols, steps);
+}
+
+int ortho_sm100(const void* update, int64_t row_stride, int64_t matrix_stride, void* out,
+                int64_t batch, int64_t rows, int64_t cols, const float* coefficients, int steps,
+                float eps, int dtype, void* workspace, size_t workspace_bytes,
+                rbf_stream_t stream) {
+  if (batch < 0 || rows < 0 || cols < 0) return refuse(RBF_ERR_INVALID_ARGUMENT, "negative size");
+  if (rows > (1 << 20) || cols > (1 << 20) || batch > 65535)
+    return refuse(RBF_ERR_UNSUPPORTED, "rows or cols > 2^20, or batch > 65535");
+  if (steps < 1 || steps > ortho_max_steps())
+    return refuse(RBF_ERR_INVALID_ARGUMENT, "steps must be in [1, 32]");
+  if (!dtype_ok(dtype)) return refuse(RBF_ERR_INVALID_ARGUMENT, "unknown element type");
+  if (!std::isfinite(eps) || eps < 0.f) return refuse(RBF_ERR_INVALID_ARGUMENT, "eps must be finite and >= 0");
+  if ((rows > 1 && row_stride < cols) || (batch > 1 && matrix_stride < 0))
+    return refuse(RBF_ERR_INVALID_ARGUMENT, "row stride smaller than cols, or negative matrix stride");
+  if (coefficients == nullptr) return refuse(RBF_ERR_INVALID_ARGUMENT, "coefficients is NULL");
+  for (int i = 0; i < 3 * steps; ++i)
+    if (!std::isfinite(coefficients[i])) return refuse(RBF_ERR_INVALID_ARGUMENT, "a coefficient is not finite");
+  int st;
+  const size_t e = elem_bytes(dtype);
+  const int64_t n = batch * rows * cols;
+  if ((st = need(update, n, e, "update"))) return st;
+  if ((st = need(out, n, e, "out"))) return st;
+  if ((st = check_workspace(workspace, workspace_bytes, ortho_workspace_bytes(batch, rows, cols, steps)))) return st;
+  if ((st = check_device())) return st;
+  OrthoArgs a{};
+  a.update = update;
+  a.out = out;
+  a.batch = batch;
+  a.rows = rows;
+  a.cols = cols;
+  a.row_stride = row_stride;
+  a.matrix_stride = matrix_stride;
+  a.dtype = dtype;
+  a.steps = steps;
+  a.coefficients = coefficients;
+  a.eps = eps;
+  a.workspace = workspace;
+  return cuda_status(launch_orthogonalize(a, wait_config_from_env(), as_stream(stream)), "orthogonalisation launch");
+}
+
 }  // extern "C"

@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "rbf_kernels.cuh"
+
 namespace rbf {
 namespace lm {
 
@@ -63,6 +65,20 @@ struct LossArgs {
 };
 size_t loss_workspace_bytes(int64_t B, int64_t T);
 cudaError_t launch_loss(const LossArgs& a, bool preference, cudaStream_t stream);
+
+// ortho.cu
+struct OrthoArgs {
+  const void* update;
+  void* out;
+  int64_t batch, rows, cols, row_stride, matrix_stride;
+  int dtype, steps;
+  const float* coefficients;  // host, [steps][3]
+  float eps;
+  void* workspace;
+};
+size_t ortho_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int steps);
+int ortho_max_steps();
+cudaError_t launch_orthogonalize(const OrthoArgs& a, const WaitConfig& wc, cudaStream_t stream);
 
 }  // namespace lm
 }  // namespace rbf

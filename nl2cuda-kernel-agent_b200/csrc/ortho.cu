@@ -1,0 +1,762 @@
+// ortho.cu -- orthogonalisation of an update by Newton-Schulz products, on the tensor cores.
+//
+//   X_0 = G / (|G|_F + eps)          (transposed where G has more rows than columns: X is r x c,
+//   A = X X^T,  B = b A + c A^2       r <= c)
+//   X <- a X + B X                    `steps` times, with (a, b, c) of each step
+//
+// All three products run as D = P Q^T with both operands K-major, on tcgen05.mma kind::f16: A takes
+// X twice, A^2 takes A twice (A is symmetric), and B X takes B and X^T, so every step keeps X in
+// both orders.  A and B are symmetric: only tiles that touch the lower triangle are computed, and
+// each value is stored at (i, j) and (j, i).  Flops of a step: r^2 c + r^3 + 2 r^2 c.
+//
+// Precision: 3 x fp16.  An operand v is kept as v * 2^k = hi + lo, hi = fp16(v 2^k) and
+// lo = fp16(v 2^k - hi), and P Q^T = hi hi^T + hi lo^T + lo hi^T in fp32: 22 bits of each operand,
+// which is what fp32 products of long sums deliver.  (Why not plain fp16 or bf16: the iteration
+// multiplies small singular values by 3.4 in each step, and the rounding of X with them; one
+// rounding to 8 or 11 bits in the first steps is a few percent of the result.)  fp16 has the range
+// for it because the spectrum is bounded: |X_0|_2 <= |X_0|_F <= 1, and |X_{k+1}|_2 <= the maximum of
+// |a s + b s^3 + c s^5| over [0, bound_k], a bound on every entry of X; those of A and B follow.
+// The scales 2^k put each matrix's bound just below 2^15; scale_table() works them out per matrix
+// on the device, so zero, tiny and diverging updates need no host round trip.  Powers of two, so
+// scaling adds no error.
+//
+// Kernel (persistent): warp 0 loads operand slices by TMA (64 deep, 128-byte swizzle, hi and lo of
+// both operands) into a ring of stages; one thread of warp 1 issues 3 x 4 MMAs per stage into one of
+// two TMEM accumulators; warps 2..9 read the other one, apply the epilogue and store.  Large
+// products run on CTA pairs (cta_group::2): a 256 x 256 tile reads 64 KiB of operands per CTA and
+// slice for 12 MMAs, two thirds of what a single CTA's 128 x 256 tile would.  No multicast.
+// Every mbarrier wait is bounded, as in rbf_fwd_tc.cu.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "lm_common.cuh"
+#include "lm_kernels.cuh"
+
+namespace rbf {
+namespace lm {
+namespace {
+
+constexpr int BK = 64;                         // operand depth of a stage: 128 bytes of fp16
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr size_t kSmemMax = 232448;
+
+// Scale factors of one step of one matrix (see scale_table).
+struct StepScale {
+  float gram;             // A      from the accumulator of X X^T
+  float square, linear;   // B      from the accumulator of A^2, and from A
+  float product, keep;    // X_next from the accumulator of B X, and from X
+};
+
+enum class Out { kSymmetric, kBoth, kFinal };
+
+struct GemmArgs {
+  int64_t M, N, K;          // D [M, N] per matrix
+  int tiles_m, tiles_n, batch;
+  int64_t tiles;            // of one matrix
+  int num_kc;
+  // D = alpha * accumulator + beta * (add_hi + add_lo), alpha and beta from the scale table
+  const StepScale* scale;   // of matrix 0
+  int scale_stride;         // StepScales between matrices
+  int kind;                 // 0 gram, 1 square, 2 product
+  const __half* add_hi;     // row-major [M, ld_d] (NULL: no addend)
+  const __half* add_lo;
+  __half* d_hi;             // row-major [M, ld_d]
+  __half* d_lo;
+  __half* t_hi;             // transposed [N, ld_t]
+  __half* t_lo;
+  int64_t ld_d, ld_t, d_matrix, t_matrix;  // strides of rows and of matrices, in elements
+  void* out;                // kFinal: out[col * ld_out + row], type out_dtype
+  int64_t ld_out, out_matrix;
+  int out_dtype;
+  int* status;
+  unsigned long long timeout_ns;
+  int debug_skip_first_load;
+};
+
+// Tile t of a matrix.  Symmetric products: only tiles with a row >= their first column, so
+// `per` = TM / TN more column tiles for each further row tile.
+template <int TM, int TN, bool SYM>
+__device__ __forceinline__ void tile_of(int64_t t, const GemmArgs& a, int& tm, int& tn) {
+  if (!SYM) {
+    // Bands of 8 row tiles, so that the tiles in flight share both operands in L2.
+    const int band = 8;
+    const int64_t per_band = (int64_t)band * a.tiles_n;
+    const int64_t bi = t / per_band;
+    const int64_t in = t - bi * per_band;
+    const int left = a.tiles_m - (int)bi * band;
+    const int rows = left < band ? left : band;
+    tm = (int)bi * band + (int)(in % rows);
+    tn = (int)(in / rows);
+    return;
+  }
+  constexpr int per = TM / TN;
+  int row = 0;
+  int64_t left = t;
+  while (true) {
+    const int64_t n = min((int64_t)per * (row + 1), (int64_t)a.tiles_n);
+    if (left < n) break;
+    left -= n;
+    ++row;
+  }
+  tm = row;
+  tn = (int)left;
+}
+
+__device__ __forceinline__ void split_f16(float x, __half& hi, __half& lo) {
+  hi = __float2half_rn(x);
+  lo = __float2half_rn(x - __half2float(hi));
+}
+
+template <bool PAIR, int BN, Out OUT>
+struct Plan {
+  static constexpr int TM = PAIR ? 256 : 128;          // rows of a tile
+  static constexpr int BROWS = PAIR ? BN / 2 : BN;     // rows of Q each CTA loads
+  static constexpr uint32_t A_BYTES = 128 * BK * 2;
+  static constexpr uint32_t B_BYTES = BROWS * BK * 2;
+  static constexpr uint32_t STAGE = 2 * (A_BYTES + B_BYTES);
+  static constexpr int STAGES = (int)((kSmemMax - 2048) / STAGE) > 6 ? 6 : (int)((kSmemMax - 2048) / STAGE);
+  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 256;
+  static constexpr uint32_t TCOLS = 2 * BN;
+  static_assert(STAGES >= 2 && SMEM <= kSmemMax, "stages");
+};
+
+template <bool PAIR, int BN, Out OUT>
+__global__ void __launch_bounds__(kThreads, 1)
+    ortho_gemm_kernel(const __grid_constant__ CUtensorMap tm_phi,
+                      const __grid_constant__ CUtensorMap tm_plo,
+                      const __grid_constant__ CUtensorMap tm_qhi,
+                      const __grid_constant__ CUtensorMap tm_qlo, const GemmArgs a) {
+  using P = Plan<PAIR, BN, OUT>;
+  constexpr bool SYM = OUT == Out::kSymmetric;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + P::STAGES * P::STAGE);  // [STAGES] TMA -> MMA
+  uint64_t* empty = full + P::STAGES;                                         // [STAGES] MMA -> TMA
+  uint64_t* acc_full = empty + P::STAGES;                                     // [2] MMA -> epilogue
+  uint64_t* acc_empty = acc_full + 2;                                         // [2] epilogue -> MMA
+  uint64_t* drain = acc_empty + 2;                                            // MMA teardown
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? ptx::cluster_ctarank() : 0;
+  const bool leader = rank == 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < P::STAGES; ++s) {
+      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(&acc_full[b], 1);
+      ptx::mbar_init(&acc_empty[b], PAIR ? 2 * kEpiWarps : kEpiWarps);
+    }
+    ptx::mbar_init(drain, 1);
+    ptx::fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    ptx::prefetch_tensormap(&tm_phi);
+    ptx::prefetch_tensormap(&tm_plo);
+    ptx::prefetch_tensormap(&tm_qhi);
+    ptx::prefetch_tensormap(&tm_qlo);
+  }
+  if (PAIR) ptx::cluster_sync();  // the peer's barriers exist before any remote arrive
+  if (warp == 1) {
+    if (PAIR) {
+      ptx::tmem_alloc_pair(tmem_slot, P::TCOLS);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(tmem_slot, P::TCOLS);
+      ptx::tmem_relinquish();
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  ptx::griddep_wait();  // the operands come from the previous kernel
+  const int64_t total = a.tiles * a.batch;
+  const int64_t unit = PAIR ? (blockIdx.x >> 1) : blockIdx.x;
+  const int64_t units = PAIR ? (gridDim.x >> 1) : gridDim.x;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, issued = 0, last = 0;
+      bool ok = true, skipped = false;
+      for (int64_t t = unit; t < total && ok; t += units) {
+        const int z = (int)(t / a.tiles);
+        int tm, tn;
+        tile_of<P::TM, BN, SYM>(t - z * a.tiles, a, tm, tn);
+        const int i0 = tm * P::TM + (int)rank * 128;
+        const int j0 = tn * BN + (int)rank * (PAIR ? P::BROWS : 0);
+        for (int kc = 0; kc < a.num_kc; ++kc) {
+          if (!ptx::mbar_wait_bounded(&empty[stage], phase ^ 1, a.status, a.timeout_ns)) { ok = false; break; }
+          if (a.debug_skip_first_load && !skipped && blockIdx.x == 0) {
+            skipped = true;  // test hook: this stage never fills, so its consumer times out
+          } else {
+            uint8_t* s = smem + stage * P::STAGE;
+            if (leader) ptx::mbar_arrive_expect_tx(&full[stage], (PAIR ? 2 : 1) * P::STAGE);
+            if (PAIR) {
+              const uint32_t fc = ptx::map_to_rank(&full[stage], 0);
+              ptx::tma_load_3d_pair(s, &tm_phi, kc * BK, i0, z, fc);
+              ptx::tma_load_3d_pair(s + P::A_BYTES, &tm_plo, kc * BK, i0, z, fc);
+              ptx::tma_load_3d_pair(s + 2 * P::A_BYTES, &tm_qhi, kc * BK, j0, z, fc);
+              ptx::tma_load_3d_pair(s + 2 * P::A_BYTES + P::B_BYTES, &tm_qlo, kc * BK, j0, z, fc);
+            } else {
+              ptx::tma_load_3d(s, &tm_phi, kc * BK, i0, z, &full[stage]);
+              ptx::tma_load_3d(s + P::A_BYTES, &tm_plo, kc * BK, i0, z, &full[stage]);
+              ptx::tma_load_3d(s + 2 * P::A_BYTES, &tm_qhi, kc * BK, j0, z, &full[stage]);
+              ptx::tma_load_3d(s + 2 * P::A_BYTES + P::B_BYTES, &tm_qlo, kc * BK, j0, z, &full[stage]);
+            }
+            if (leader) {
+              issued |= 1u << stage;
+              last = (last & ~(1u << stage)) | (phase << stage);
+            }
+          }
+          if (++stage == P::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // Error path: let every load issued land before the CTA exits (the leader's barriers count
+      // both CTAs' bytes, and the final cluster barrier holds the peer until then).
+      if (!ok)
+        for (int s = 0; s < P::STAGES; ++s)
+          if (issued >> s & 1u) ptx::mbar_wait_bounded(&full[s], (last >> s) & 1u, a.status, a.timeout_ns);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0 && leader) {
+      constexpr uint32_t idesc = ptx::idesc_f16(P::TM, BN);
+      auto commit = [](uint64_t* bar) {
+        if (PAIR) ptx::mma_commit_pair(bar);
+        else ptx::mma_commit(bar);
+      };
+      auto mma = [](uint32_t d, uint64_t x, uint64_t y, uint32_t acc) {
+        if (PAIR) ptx::mma_f16_ss_pair(d, x, y, idesc, acc);
+        else ptx::mma_f16_ss(d, x, y, idesc, acc);
+      };
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int64_t t = unit; t < total && ok; t += units) {
+        if (!ptx::mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1, a.status, a.timeout_ns)) break;
+        ptx::tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(acc * BN);
+        for (int kc = 0; kc < a.num_kc; ++kc) {
+          if (!ptx::mbar_wait_bounded(&full[stage], phase, a.status, a.timeout_ns)) { ok = false; break; }
+          ptx::tc_fence_after();
+          const uint32_t s = ptx::smem_u32(smem + stage * P::STAGE);
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) {
+            const uint32_t off = (uint32_t)k * 32;  // 16 fp16 along the swizzled row
+            const uint64_t phi = ptx::smem_desc(s + off, 16, 1024, 2);
+            const uint64_t plo = ptx::smem_desc(s + P::A_BYTES + off, 16, 1024, 2);
+            const uint64_t qhi = ptx::smem_desc(s + 2 * P::A_BYTES + off, 16, 1024, 2);
+            const uint64_t qlo = ptx::smem_desc(s + 2 * P::A_BYTES + P::B_BYTES + off, 16, 1024, 2);
+            mma(d, phi, qhi, (kc | k) != 0);
+            mma(d, phi, qlo, 1);
+            mma(d, plo, qhi, 1);
+          }
+          commit(&empty[stage]);
+          if (++stage == P::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        commit(&acc_full[acc]);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+      }
+      commit(drain);  // every MMA issued so far finishes before TMEM is freed
+      ptx::mbar_wait_bounded(drain, 0, a.status, a.timeout_ns);
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;           // TMEM lane quadrant this warp may access
+    const int h = (warp - 2) >> 2;    // half of the tile's columns
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int64_t t = unit; t < total; t += units) {
+      const int z = (int)(t / a.tiles);
+      int tm, tn;
+      tile_of<P::TM, BN, SYM>(t - z * a.tiles, a, tm, tn);
+      const int64_t i = (int64_t)tm * P::TM + rank * 128 + q * 32 + lane;
+      const StepScale sc = a.scale[(int64_t)z * a.scale_stride];
+      const float alpha = a.kind == 0 ? sc.gram : a.kind == 1 ? sc.square : sc.product;
+      const float beta = a.kind == 0 ? 0.f : a.kind == 1 ? sc.linear : sc.keep;
+      if (!ptx::mbar_wait_bounded(&acc_full[acc], acc_phase, a.status, a.timeout_ns)) break;
+      ptx::tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < BN / 64; ++c) {
+        const int col = h * (BN / 2) + c * 32;
+        const int64_t j0 = (int64_t)tn * BN + col;
+        uint32_t v[32];
+        __syncwarp();  // the TMEM load is a whole warp's
+        ptx::tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + col), v);
+        ptx::tmem_wait_ld();
+        if (c == BN / 64 - 1) {  // the accumulator goes back before the stores
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR) ptx::mbar_arrive_cluster(ptx::map_to_rank(&acc_empty[acc], 0));
+            else ptx::mbar_arrive(&acc_empty[acc]);
+          }
+        }
+        if (j0 >= a.N || i >= a.M) continue;
+        if (SYM && j0 > i) continue;
+        float f[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = alpha * __uint_as_float(v[e]);
+        if (a.add_hi != nullptr) {
+          // ld_d is a multiple of 32, so a chunk of 32 columns lies inside its row.
+          const int64_t at = z * a.d_matrix + i * a.ld_d + j0;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const Pack<__half, 8> hi = *reinterpret_cast<const Pack<__half, 8>*>(a.add_hi + at + 8 * g);
+            const Pack<__half, 8> lo = *reinterpret_cast<const Pack<__half, 8>*>(a.add_lo + at + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              f[8 * g + e] = fmaf(beta, __half2float(hi.v[e]) + __half2float(lo.v[e]), f[8 * g + e]);
+          }
+        }
+        if constexpr (OUT == Out::kFinal) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (j0 + e < a.N) store_as(a.out, z * a.out_matrix + (j0 + e) * a.ld_out + i, a.out_dtype, f[e]);
+        } else {
+          Pack<__half, 32> hi, lo;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) split_f16(f[e], hi.v[e], lo.v[e]);
+          __half* dh = a.d_hi + z * a.d_matrix + i * a.ld_d + j0;
+          __half* dl = a.d_lo + z * a.d_matrix + i * a.ld_d + j0;
+          if (!SYM || j0 + 31 <= i) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              *reinterpret_cast<uint4*>(dh + 8 * g) = reinterpret_cast<const uint4*>(&hi)[g];
+              *reinterpret_cast<uint4*>(dl + 8 * g) = reinterpret_cast<const uint4*>(&lo)[g];
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (j0 + e <= i) {
+                dh[e] = hi.v[e];
+                dl[e] = lo.v[e];
+              }
+          }
+          // The other order: the lanes of a warp write 32 consecutive values.
+          __half* th = (SYM ? a.d_hi : a.t_hi) + z * (SYM ? a.d_matrix : a.t_matrix) + i;
+          __half* tl = (SYM ? a.d_lo : a.t_lo) + z * (SYM ? a.d_matrix : a.t_matrix) + i;
+          const int64_t ld = SYM ? a.ld_d : a.ld_t;
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (j0 + e < (SYM ? i : a.N)) {
+              th[(j0 + e) * ld] = hi.v[e];
+              tl[(j0 + e) * ld] = lo.v[e];
+            }
+        }
+      }
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+  }
+  ptx::griddep_launch_dependents();
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (PAIR) ptx::cluster_sync();  // neither CTA leaves before both are done with each other's memory
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    if (PAIR) ptx::tmem_dealloc_pair(tmem, P::TCOLS);
+    else ptx::tmem_dealloc(tmem, P::TCOLS);
+  }
+}
+
+// ---- the norm, the scales and the first X ---------------------------------------------------
+
+constexpr int kMaxSteps = 32;
+constexpr int kNormThreads = 256;
+constexpr int kMaxNormParts = 256;
+
+struct PrepArgs {
+  const void* g;
+  int64_t rows, cols, row_stride, matrix_stride;  // of G; its rows are contiguous
+  int dtype, tall, parts, steps;
+  float eps;
+  float coef[kMaxSteps][3];
+  double* part;            // [batch][parts] sums of squares
+  StepScale* scale;        // [batch][steps]
+  __half* g_hi;            // G's order: [rows, ld_g]
+  __half* g_lo;
+  __half* t_hi;            // the other order: [cols, ld_t]
+  __half* t_lo;
+  int64_t ld_g, ld_t, g_matrix, t_matrix;
+  int* status;
+};
+
+template <typename T>
+__device__ __forceinline__ float g_at(const PrepArgs& a, int64_t z, int64_t i, int64_t j) {
+  return to_f32(static_cast<const T*>(a.g)[z * a.matrix_stride + i * a.row_stride + j]);
+}
+
+// Sums of squares in 64 bits: an update of any magnitude has a norm.
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads) ortho_norm_kernel(const PrepArgs a) {
+  __shared__ double red[kNormThreads / 32];
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  const int64_t z = blockIdx.y, p = blockIdx.x;
+  if (z == 0 && p == 0 && threadIdx.x == 0) *a.status = 0;
+  double s = 0.0;
+  for (int64_t i = a.rows * p / a.parts; i < a.rows * (p + 1) / a.parts; ++i) {
+    const T* row = static_cast<const T*>(a.g) + z * a.matrix_stride + i * a.row_stride;
+    for (int64_t j = threadIdx.x; j < a.cols; j += kNormThreads) {
+      const double v = to_f32(row[j]);
+      s = fma(v, v, s);
+    }
+  }
+  s = warp_sum(s);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kNormThreads / 32; ++w) s += red[w];
+    a.part[z * a.parts + p] = s;
+  }
+}
+
+// 2^k that brings values of at most `bound` below 2^15 (bounds past 2^+-100 keep the last scale:
+// what is smaller does not count next to the rest, what is larger has diverged).
+__device__ double pow2_scale(double bound) {
+  int e = 0;
+  if (bound > 0.0 && isfinite(bound)) e = ilogb(bound) + 1;
+  e = e < -100 ? -100 : e > 100 ? 100 : e;
+  return ldexp(1.0, 15 - e);
+}
+
+__device__ double max_on(double top, double c1, double c3, double c5) {
+  // max of |c1 s + c3 s^3 + c5 s^5| over [0, top]: at the end, or where c1 + 3 c3 u + 5 c5 u^2 = 0, u = s^2
+  auto p = [&](double s) { return fabs(s * (c1 + s * s * (c3 + s * s * c5))); };
+  double m = p(top);
+  auto at = [&](double u) {
+    if (u > 0.0 && u < top * top) m = fmax(m, p(sqrt(u)));
+  };
+  const double A = 5.0 * c5, B = 3.0 * c3, disc = B * B - 4.0 * A * c1;
+  if (A == 0.0) {
+    if (B != 0.0) at(-c1 / B);
+  } else if (disc >= 0.0) {
+    at((-B + sqrt(disc)) / (2.0 * A));
+    at((-B - sqrt(disc)) / (2.0 * A));
+  }
+  return m;
+}
+
+// The scales of every step of one matrix; returns that of X_0.  `rho` bounds |X_0|_F.
+__device__ double scale_table(double rho, const PrepArgs& a, StepScale* out) {
+  const double slack = 1.0 + 1e-3;  // for rounding along the way
+  double bound = rho * slack;
+  double sx = pow2_scale(bound);
+  const double first = sx;
+  for (int k = 0; k < a.steps; ++k) {
+    const double ca = a.coef[k][0], cb = a.coef[k][1], cc = a.coef[k][2];
+    const double u = bound * bound;
+    const double sa = pow2_scale(u);
+    // |b u + c u^2| over [0, bound^2]
+    double mb = fabs(u * (cb + cc * u));
+    if (cc != 0.0) {
+      const double peak = -cb / (2.0 * cc);
+      if (peak > 0.0 && peak < u) mb = fmax(mb, fabs(peak * (cb + cc * peak)));
+    }
+    const double sb = pow2_scale(mb * slack);
+    const double next = max_on(bound, ca, cb, cc) * slack;
+    const double sn = k + 1 == a.steps ? 1.0 : pow2_scale(next);
+    if (out != nullptr) {
+      out[k].gram = (float)(sa / (sx * sx));
+      out[k].square = (float)(cc * sb / (sa * sa));
+      out[k].linear = (float)(cb * sb / sa);
+      out[k].product = (float)(sn / (sb * sx));
+      out[k].keep = (float)(ca * sn / sx);
+    }
+    bound = next;
+    sx = sn;
+  }
+  return first;
+}
+
+constexpr int kTile = 64;
+
+// X_0 in both orders, a 64 x 64 tile of G per CTA; the first CTA of a matrix writes its scales.
+template <typename T>
+__global__ void __launch_bounds__(256) ortho_split_kernel(const PrepArgs a) {
+  __shared__ __half s_hi[kTile][kTile + 2], s_lo[kTile][kTile + 2];
+  __shared__ double s_factor;
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  const int64_t z = blockIdx.z;
+  if (threadIdx.x < 32) {
+    double t = 0.0;
+    for (int p = threadIdx.x; p < a.parts; p += 32) t += a.part[z * a.parts + p];
+    t = warp_sum(t);
+    if (threadIdx.x == 0) {
+      const double norm = sqrt(t), den = norm + (double)a.eps;
+      const bool first = blockIdx.x == 0 && blockIdx.y == 0;
+      const double sx = scale_table(den > 0.0 ? norm / den : 0.0, a, first ? a.scale + z * a.steps : nullptr);
+      s_factor = sx / den;
+    }
+  }
+  __syncthreads();
+  const double factor = s_factor;
+  const int64_t i0 = (int64_t)blockIdx.y * kTile, j0 = (int64_t)blockIdx.x * kTile;
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+#pragma unroll 4
+  for (int r = ty; r < kTile; r += 4) {
+    const int64_t i = i0 + r, j = j0 + tx;
+    if (i < a.rows && j < a.cols) {
+      __half hi, lo;
+      split_f16((float)((double)g_at<T>(a, z, i, j) * factor), hi, lo);
+      const int64_t at = z * a.g_matrix + i * a.ld_g + j;
+      a.g_hi[at] = hi;
+      a.g_lo[at] = lo;
+      s_hi[r][tx] = hi;
+      s_lo[r][tx] = lo;
+    }
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int r = ty; r < kTile; r += 4) {
+    const int64_t j = j0 + r, i = i0 + tx;
+    if (i < a.rows && j < a.cols) {
+      const int64_t at = z * a.t_matrix + j * a.ld_t + i;
+      a.t_hi[at] = s_hi[tx][r];
+      a.t_lo[at] = s_lo[tx][r];
+    }
+  }
+}
+
+// ---- host side ----------------------------------------------------------------------------
+
+// One matrix kept as hi and lo in both halves of a buffer.
+struct Split {
+  __half* hi;
+  __half* lo;
+  int64_t rows, cols, ld, matrix;
+};
+
+struct Layout {
+  int64_t r, c;                 // X is r x c, r <= c
+  int64_t ld_c, ld_r;
+  size_t status, part, scale, x, xt0, xt1, a, b, end;
+  int parts;
+};
+
+Layout layout_of(int64_t batch, int64_t rows, int64_t cols, int steps) {
+  Layout L;
+  L.r = std::min(rows, cols);
+  L.c = std::max(rows, cols);
+  L.ld_c = round_up(L.c, 32);
+  L.ld_r = round_up(L.r, 32);
+  // About 32 K values for each CTA of the norm, and no more CTAs than give each SM four.
+  const int64_t want = std::min<int64_t>(ceil_div(rows * cols, 32768), ceil_div(4 * kSmCount, batch > 0 ? batch : 1));
+  L.parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, rows), kMaxNormParts));
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = off;
+    off = (size_t)round_up((int64_t)(off + bytes), (int64_t)kAlign);
+    return o;
+  };
+  L.status = take(64);
+  L.part = take(sizeof(double) * batch * L.parts);
+  L.scale = take(sizeof(StepScale) * batch * steps);
+  const size_t x = sizeof(__half) * 2 * batch * L.r * L.ld_c, xt = sizeof(__half) * 2 * batch * L.c * L.ld_r;
+  const size_t sq = sizeof(__half) * 2 * batch * L.r * L.ld_r;
+  L.x = take(x);
+  L.xt0 = take(xt);
+  L.xt1 = take(steps > 1 ? xt : 0);
+  L.a = take(sq);
+  L.b = take(sq);
+  L.end = off;
+  return L;
+}
+
+Split split_at(void* ws, size_t off, int64_t batch, int64_t rows, int64_t cols, int64_t ld) {
+  Split s;
+  s.hi = ws_at<__half>(ws, off);
+  s.lo = s.hi + batch * rows * ld;
+  s.rows = rows;
+  s.cols = cols;
+  s.ld = ld;
+  s.matrix = rows * ld;
+  return s;
+}
+
+// D = P Q^T: the launch of one product.
+template <bool PAIR, int BN, Out OUT>
+cudaError_t launch_gemm(const Split& p, const Split& q, GemmArgs a, cudaStream_t stream) {
+  using PL = Plan<PAIR, BN, OUT>;
+  CUtensorMap m[4];
+  if (!make_tmap_f16(&m[0], p.hi, p.cols, p.rows, a.batch, p.ld, p.matrix, BK, 128) ||
+      !make_tmap_f16(&m[1], p.lo, p.cols, p.rows, a.batch, p.ld, p.matrix, BK, 128) ||
+      !make_tmap_f16(&m[2], q.hi, q.cols, q.rows, a.batch, q.ld, q.matrix, BK, PL::BROWS) ||
+      !make_tmap_f16(&m[3], q.lo, q.cols, q.rows, a.batch, q.ld, q.matrix, BK, PL::BROWS))
+    return cudaErrorInvalidValue;
+  a.M = p.rows;
+  a.N = q.rows;
+  a.K = p.cols;
+  a.num_kc = (int)ceil_div(a.K, BK);
+  a.tiles_m = (int)ceil_div(a.M, PL::TM);
+  a.tiles_n = (int)ceil_div(a.N, BN);
+  if (OUT == Out::kSymmetric) {
+    a.tiles = 0;
+    for (int tm = 0; tm < a.tiles_m; ++tm)
+      a.tiles += std::min<int64_t>((int64_t)(PL::TM / BN) * (tm + 1), a.tiles_n);
+  } else {
+    a.tiles = (int64_t)a.tiles_m * a.tiles_n;
+  }
+  const int64_t total = a.tiles * a.batch;
+  auto k = ortho_gemm_kernel<PAIR, BN, OUT>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PL::SMEM);
+  if (e != cudaSuccess) return e;
+  const int units = PAIR ? device_sm_count() / 2 : device_sm_count();
+  const unsigned grid = (unsigned)std::min<int64_t>(total, units);
+  if (PAIR) return launch_kernel_cluster(k, dim3(2 * grid), dim3(kThreads), PL::SMEM, 2, stream, m[0], m[1], m[2], m[3], a);
+  return launch_kernel(k, dim3(grid), dim3(kThreads), PL::SMEM, stream, m[0], m[1], m[2], m[3], a);
+}
+
+// Tiles: as large as leaves work for most SMs.
+template <Out OUT>
+cudaError_t launch_product(const Split& p, const Split& q, const GemmArgs& a, cudaStream_t stream) {
+  const int sms = device_sm_count();
+  auto tiles = [&](int64_t tm, int64_t tn) {
+    const int64_t n = ceil_div(p.rows, tm) * ceil_div(q.rows, tn) * a.batch;
+    return OUT == Out::kSymmetric ? n / 2 : n;
+  };
+  if (tiles(256, 256) >= sms / 4) return launch_gemm<true, 256, OUT>(p, q, a, stream);
+  if (tiles(128, 128) >= sms / 2) return launch_gemm<false, 128, OUT>(p, q, a, stream);
+  return launch_gemm<false, 64, OUT>(p, q, a, stream);
+}
+
+}  // namespace
+
+size_t ortho_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int steps) {
+  return layout_of(batch, rows, cols, steps).end;
+}
+
+int ortho_max_steps() { return kMaxSteps; }
+
+cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaStream_t stream) {
+  if (o.batch == 0 || o.rows == 0 || o.cols == 0) return cudaSuccess;
+  const Layout L = layout_of(o.batch, o.rows, o.cols, o.steps);
+  const bool tall = o.rows > o.cols;
+  int* status = ws_at<int>(o.workspace, L.status);
+  StepScale* scale = ws_at<StepScale>(o.workspace, L.scale);
+  const Split x = split_at(o.workspace, L.x, o.batch, L.r, L.c, L.ld_c);
+  Split xt = split_at(o.workspace, L.xt0, o.batch, L.c, L.r, L.ld_r);
+  Split xt_next = split_at(o.workspace, L.xt1, o.batch, L.c, L.r, L.ld_r);
+  const Split ma = split_at(o.workspace, L.a, o.batch, L.r, L.r, L.ld_r);
+  const Split mb = split_at(o.workspace, L.b, o.batch, L.r, L.r, L.ld_r);
+
+  PrepArgs p{};
+  p.g = o.update;
+  p.rows = o.rows;
+  p.cols = o.cols;
+  p.row_stride = o.row_stride;
+  p.matrix_stride = o.matrix_stride;
+  p.dtype = o.dtype;
+  p.tall = tall;
+  p.parts = L.parts;
+  p.steps = o.steps;
+  p.eps = o.eps;
+  for (int k = 0; k < o.steps; ++k)
+    for (int e = 0; e < 3; ++e) p.coef[k][e] = o.coefficients[3 * k + e];
+  p.part = ws_at<double>(o.workspace, L.part);
+  p.scale = scale;
+  const Split& g = tall ? xt : x;
+  const Split& t = tall ? x : xt;
+  p.g_hi = g.hi;
+  p.g_lo = g.lo;
+  p.ld_g = g.ld;
+  p.g_matrix = g.matrix;
+  p.t_hi = t.hi;
+  p.t_lo = t.lo;
+  p.ld_t = t.ld;
+  p.t_matrix = t.matrix;
+  p.status = status;
+  auto prep = [&](auto norm, auto split) {
+    cudaError_t e = launch_kernel(norm, dim3(L.parts, (unsigned)o.batch), dim3(kNormThreads), 0, stream, p);
+    if (e != cudaSuccess) return e;
+    return launch_kernel(split, dim3((unsigned)ceil_div(o.cols, kTile), (unsigned)ceil_div(o.rows, kTile), (unsigned)o.batch),
+                         dim3(256), 0, stream, p);
+  };
+  cudaError_t e = o.dtype == LM_F32    ? prep(ortho_norm_kernel<float>, ortho_split_kernel<float>)
+                  : o.dtype == LM_BF16 ? prep(ortho_norm_kernel<__nv_bfloat16>, ortho_split_kernel<__nv_bfloat16>)
+                                       : prep(ortho_norm_kernel<__half>, ortho_split_kernel<__half>);
+  if (e != cudaSuccess) return e;
+  note_launches(2);
+
+  GemmArgs base{};
+  base.batch = (int)o.batch;
+  base.scale_stride = o.steps;
+  base.status = status;
+  base.timeout_ns = wc.timeout_ns;
+  base.debug_skip_first_load = wc.debug_skip_first_load;
+  for (int k = 0; k < o.steps; ++k) {
+    GemmArgs a = base;
+    a.scale = scale + k;
+    a.kind = 0;
+    a.d_hi = ma.hi;
+    a.d_lo = ma.lo;
+    a.ld_d = ma.ld;
+    a.d_matrix = ma.matrix;
+    if ((e = launch_product<Out::kSymmetric>(x, x, a, stream)) != cudaSuccess) return e;
+    a.kind = 1;
+    a.add_hi = ma.hi;
+    a.add_lo = ma.lo;
+    a.d_hi = mb.hi;
+    a.d_lo = mb.lo;
+    if ((e = launch_product<Out::kSymmetric>(ma, ma, a, stream)) != cudaSuccess) return e;
+    a = base;
+    a.scale = scale + k;
+    a.kind = 2;
+    if (k + 1 < o.steps) {
+      // X in place: each value is read by the thread that replaces it.
+      a.add_hi = x.hi;
+      a.add_lo = x.lo;
+      a.d_hi = x.hi;
+      a.d_lo = x.lo;
+      a.ld_d = x.ld;
+      a.d_matrix = x.matrix;
+      a.t_hi = xt_next.hi;
+      a.t_lo = xt_next.lo;
+      a.ld_t = xt_next.ld;
+      a.t_matrix = xt_next.matrix;
+      if ((e = launch_product<Out::kBoth>(mb, xt, a, stream)) != cudaSuccess) return e;
+      std::swap(xt, xt_next);
+    } else {
+      // The last product runs in the order that lets the lanes of a warp write the result's rows.
+      const Split& add = tall ? x : xt;
+      a.add_hi = add.hi;
+      a.add_lo = add.lo;
+      a.ld_d = add.ld;
+      a.d_matrix = add.matrix;
+      a.out = o.out;
+      a.ld_out = o.cols;
+      a.out_matrix = o.rows * o.cols;
+      a.out_dtype = o.dtype;
+      e = tall ? launch_product<Out::kFinal>(mb, xt, a, stream) : launch_product<Out::kFinal>(xt, mb, a, stream);
+      if (e != cudaSuccess) return e;
+    }
+    note_launches(3);
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace lm
+}  // namespace rbf

@@ -586,6 +586,21 @@ bool make_tmap_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t co
   return r == CUDA_SUCCESS;
 }
 
+bool make_tmap_f16(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
+                   uint64_t matrices, uint64_t ld, uint64_t matrix, uint32_t box_cols,
+                   uint32_t box_rows) {
+  const EncodeTiledFn enc = encode_tiled();
+  if (enc == nullptr) return false;
+  cuuint64_t dims[3] = {cols, rows, matrices};
+  cuuint64_t strides[2] = {ld * 2, matrix * 2};
+  cuuint32_t box[3] = {box_cols, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides,
+                   box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 int device_sm_count() {
   int dev = 0, n = kSmCount;
   if (cudaGetDevice(&dev) == cudaSuccess)

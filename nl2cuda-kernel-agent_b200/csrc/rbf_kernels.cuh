@@ -109,6 +109,11 @@ cudaError_t launch_prep(const float* X, const float* Y, int64_t N, int64_t M, in
 bool make_tmap_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                   uint64_t pitch_elems, uint32_t box_cols, uint32_t box_rows,
                   int swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
+// 3-D fp16 tensor map of `matrices` row-major rows x cols matrices (row pitch ld, matrix pitch
+// `matrix`, in elements), 128-byte swizzle, zero fill out of bounds; a box is one matrix's.
+bool make_tmap_f16(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
+                   uint64_t matrices, uint64_t ld, uint64_t matrix, uint32_t box_cols,
+                   uint32_t box_rows);
 int device_sm_count();
 
 // rbf_bwd_tc.cu: the fused tcgen05 3xTF32 backward (zeroes dX, dY, then accumulates into

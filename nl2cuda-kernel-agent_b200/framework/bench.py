@@ -115,21 +115,27 @@ def compare(case, candidate, device=None, seed=0, baseline=None):
     res = {}
     for name, fn in [("baseline(torch.compile)", base), ("candidate", candidate)]:
         f = _forward_stats(fn, inputs, case.params)
-        b = _backward_stats(fn, inputs, case.params, case.grad_inputs, G)
+        # A case without gradient inputs has no backward pass to time.
+        b = (_backward_stats(fn, inputs, case.params, case.grad_inputs, G) if case.grad_inputs
+             else None)
         res[name] = (f, b)
         lines.append(f"\n[{name}]")
-        for s in (f, b):
+        for s in (f, b) if b else (f,):
             lines.append(f"  {s['kind']:8s}: {s['geomean_ms']:.4f} ms  CV={s['cv'] * 100:.2f}%  "
                          f"x{s['attempts']}  {'ok' if s['ok'] else 'CV over threshold'}")
     (bf, bb), (cf, cb) = res["baseline(torch.compile)"], res["candidate"]
-    fs, bs = bf["geomean_ms"] / cf["geomean_ms"], bb["geomean_ms"] / cb["geomean_ms"]
+    fs = bf["geomean_ms"] / cf["geomean_ms"]
     lines.append("\n[speed-up candidate vs baseline]")
     lines.append(f"  forward : {fs:.4f}x (need >= {p.speedup_target}x) "
                  f"{'PASS' if fs >= p.speedup_target else 'FAIL'}")
-    lines.append(f"  backward: {bs:.4f}x (need >= {p.speedup_target}x) "
-                 f"{'PASS' if bs >= p.speedup_target else 'FAIL'}")
-    cv_ok = all(s["ok"] for s in (bf, bb, cf, cb))
-    passed = fs >= p.speedup_target and bs >= p.speedup_target and cv_ok
+    passed = fs >= p.speedup_target
+    if cb is not None:
+        bs = bb["geomean_ms"] / cb["geomean_ms"]
+        lines.append(f"  backward: {bs:.4f}x (need >= {p.speedup_target}x) "
+                     f"{'PASS' if bs >= p.speedup_target else 'FAIL'}")
+        passed = passed and bs >= p.speedup_target
+    cv_ok = all(s["ok"] for s in (bf, bb, cf, cb) if s is not None)
+    passed = passed and cv_ok
     if not cv_ok:
         lines.append("  CV over threshold: result void, re-measure")
     lines.append(f"\n=== gate: {'PASS' if passed else 'FAIL'} ===")
