@@ -20,9 +20,15 @@
 // on the device, so zero, tiny and diverging updates need no host round trip.  Powers of two, so
 // scaling adds no error.
 //
+// The tensor core truncates each addition to its fp32 accumulator, so a long sum of one sign comes out
+// low by half a unit per MMA: 1.8e-5 of the result at a depth of 2601.  So an accumulator takes a
+// run of slices only, and the epilogue warps add these partial sums in registers, rounded to nearest.
+// A run is 256 deep for fp32 results (error 4.8e-6 there, the fp32 library product's is 3.3e-6), 1024
+// for fp16 and 2048 for bf16, whose own rounding is far larger: short runs cost up to 9% of the time.
+//
 // Kernel (persistent): warp 0 loads operand slices by TMA (64 deep, 128-byte swizzle, hi and lo of
 // both operands) into a ring of stages; one thread of warp 1 issues 3 x 4 MMAs per stage into one of
-// two TMEM accumulators; warps 2..9 read the other one, apply the epilogue and store.  Large
+// two TMEM accumulators; warps 4..11 read the other one, apply the epilogue and store.  Large
 // products run on CTA pairs (cta_group::2): a 256 x 256 tile reads 64 KiB of operands per CTA and
 // slice for 12 MMAs, two thirds of what a single CTA's 128 x 256 tile would.  No multicast.
 // Every mbarrier wait is bounded, as in rbf_fwd_tc.cu.
@@ -30,6 +36,7 @@
 
 #include <algorithm>
 
+#define RBF_WAIT_INLINE  // a call would tie up registers across the register split below
 #include "lm_common.cuh"
 #include "lm_kernels.cuh"
 
@@ -39,7 +46,11 @@ namespace {
 
 constexpr int BK = 64;                         // operand depth of a stage: 128 bytes of fp16
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kThreads = 32 * (4 + kEpiWarps);  // a warpgroup for the loads and MMAs, two for the epilogue
+// Registers per thread: launched with kRegs each, then the first warpgroup passes most of its own to
+// the other two, which hold 128 partial sums each (kRegsLow + 2 kRegsHigh = 3 kRegs).
+constexpr int kRegs = 168, kRegsLow = 40, kRegsHigh = 232;
+static_assert(kRegsLow + 2 * kRegsHigh <= 3 * kRegs && kThreads == 384, "register split");
 constexpr size_t kSmemMax = 232448;
 
 // Scale factors of one step of one matrix (see scale_table).
@@ -56,6 +67,7 @@ struct GemmArgs {
   int tiles_m, tiles_n, batch;
   int64_t tiles;            // of one matrix
   int num_kc;
+  int run;                  // slices that share a TMEM accumulator
   // D = alpha * accumulator + beta * (add_hi + add_lo), alpha and beta from the scale table
   const StepScale* scale;   // of matrix 0
   int scale_stride;         // StepScales between matrices
@@ -181,108 +193,117 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t unit = PAIR ? (blockIdx.x >> 1) : blockIdx.x;
   const int64_t units = PAIR ? (gridDim.x >> 1) : gridDim.x;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0, issued = 0, last = 0;
-      bool ok = true, skipped = false;
-      for (int64_t t = unit; t < total && ok; t += units) {
-        const int z = (int)(t / a.tiles);
-        int tm, tn;
-        tile_of<P::TM, BN, SYM>(t - z * a.tiles, a, tm, tn);
-        const int i0 = tm * P::TM + (int)rank * 128;
-        const int j0 = tn * BN + (int)rank * (PAIR ? P::BROWS : 0);
-        for (int kc = 0; kc < a.num_kc; ++kc) {
-          if (!ptx::mbar_wait_bounded(&empty[stage], phase ^ 1, a.status, a.timeout_ns)) { ok = false; break; }
-          if (a.debug_skip_first_load && !skipped && blockIdx.x == 0) {
-            skipped = true;  // test hook: this stage never fills, so its consumer times out
-          } else {
-            uint8_t* s = smem + stage * P::STAGE;
-            if (leader) ptx::mbar_arrive_expect_tx(&full[stage], (PAIR ? 2 : 1) * P::STAGE);
-            if (PAIR) {
-              const uint32_t fc = ptx::map_to_rank(&full[stage], 0);
-              ptx::tma_load_3d_pair(s, &tm_phi, kc * BK, i0, z, fc);
-              ptx::tma_load_3d_pair(s + P::A_BYTES, &tm_plo, kc * BK, i0, z, fc);
-              ptx::tma_load_3d_pair(s + 2 * P::A_BYTES, &tm_qhi, kc * BK, j0, z, fc);
-              ptx::tma_load_3d_pair(s + 2 * P::A_BYTES + P::B_BYTES, &tm_qlo, kc * BK, j0, z, fc);
+  if (warp < 4) {
+    ptx::regs_shrink<kRegsLow>();
+    if (warp == 0) {
+      // ------------------------------------------------------------ TMA producer
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0, issued = 0, last = 0;
+        bool ok = true, skipped = false;
+        for (int64_t t = unit; t < total && ok; t += units) {
+          const int z = (int)(t / a.tiles);
+          int tm, tn;
+          tile_of<P::TM, BN, SYM>(t - z * a.tiles, a, tm, tn);
+          const int i0 = tm * P::TM + (int)rank * 128;
+          const int j0 = tn * BN + (int)rank * (PAIR ? P::BROWS : 0);
+          for (int kc = 0; kc < a.num_kc; ++kc) {
+            if (!ptx::mbar_wait_bounded(&empty[stage], phase ^ 1, a.status, a.timeout_ns)) { ok = false; break; }
+            if (a.debug_skip_first_load && !skipped && blockIdx.x == 0) {
+              skipped = true;  // test hook: this stage never fills, so its consumer times out
             } else {
-              ptx::tma_load_3d(s, &tm_phi, kc * BK, i0, z, &full[stage]);
-              ptx::tma_load_3d(s + P::A_BYTES, &tm_plo, kc * BK, i0, z, &full[stage]);
-              ptx::tma_load_3d(s + 2 * P::A_BYTES, &tm_qhi, kc * BK, j0, z, &full[stage]);
-              ptx::tma_load_3d(s + 2 * P::A_BYTES + P::B_BYTES, &tm_qlo, kc * BK, j0, z, &full[stage]);
+              uint8_t* s = smem + stage * P::STAGE;
+              if (leader) ptx::mbar_arrive_expect_tx(&full[stage], (PAIR ? 2 : 1) * P::STAGE);
+              if (PAIR) {
+                const uint32_t fc = ptx::map_to_rank(&full[stage], 0);
+                ptx::tma_load_3d_pair(s, &tm_phi, kc * BK, i0, z, fc);
+                ptx::tma_load_3d_pair(s + P::A_BYTES, &tm_plo, kc * BK, i0, z, fc);
+                ptx::tma_load_3d_pair(s + 2 * P::A_BYTES, &tm_qhi, kc * BK, j0, z, fc);
+                ptx::tma_load_3d_pair(s + 2 * P::A_BYTES + P::B_BYTES, &tm_qlo, kc * BK, j0, z, fc);
+              } else {
+                ptx::tma_load_3d(s, &tm_phi, kc * BK, i0, z, &full[stage]);
+                ptx::tma_load_3d(s + P::A_BYTES, &tm_plo, kc * BK, i0, z, &full[stage]);
+                ptx::tma_load_3d(s + 2 * P::A_BYTES, &tm_qhi, kc * BK, j0, z, &full[stage]);
+                ptx::tma_load_3d(s + 2 * P::A_BYTES + P::B_BYTES, &tm_qlo, kc * BK, j0, z, &full[stage]);
+              }
+              if (leader) {
+                issued |= 1u << stage;
+                last = (last & ~(1u << stage)) | (phase << stage);
+              }
             }
-            if (leader) {
-              issued |= 1u << stage;
-              last = (last & ~(1u << stage)) | (phase << stage);
+            if (++stage == P::STAGES) {
+              stage = 0;
+              phase ^= 1;
             }
-          }
-          if (++stage == P::STAGES) {
-            stage = 0;
-            phase ^= 1;
           }
         }
+        // Error path: let every load issued land before the CTA exits (the leader's barriers count
+        // both CTAs' bytes, and the final cluster barrier holds the peer until then).
+        if (!ok)
+          for (int s = 0; s < P::STAGES; ++s)
+            if (issued >> s & 1u) ptx::mbar_wait_bounded(&full[s], (last >> s) & 1u, a.status, a.timeout_ns);
       }
-      // Error path: let every load issued land before the CTA exits (the leader's barriers count
-      // both CTAs' bytes, and the final cluster barrier holds the peer until then).
-      if (!ok)
-        for (int s = 0; s < P::STAGES; ++s)
-          if (issued >> s & 1u) ptx::mbar_wait_bounded(&full[s], (last >> s) & 1u, a.status, a.timeout_ns);
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0 && leader) {
-      constexpr uint32_t idesc = ptx::idesc_f16(P::TM, BN);
-      auto commit = [](uint64_t* bar) {
-        if (PAIR) ptx::mma_commit_pair(bar);
-        else ptx::mma_commit(bar);
-      };
-      auto mma = [](uint32_t d, uint64_t x, uint64_t y, uint32_t acc) {
-        if (PAIR) ptx::mma_f16_ss_pair(d, x, y, idesc, acc);
-        else ptx::mma_f16_ss(d, x, y, idesc, acc);
-      };
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool ok = true;
-      for (int64_t t = unit; t < total && ok; t += units) {
-        if (!ptx::mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1, a.status, a.timeout_ns)) break;
-        ptx::tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(acc * BN);
-        for (int kc = 0; kc < a.num_kc; ++kc) {
-          if (!ptx::mbar_wait_bounded(&full[stage], phase, a.status, a.timeout_ns)) { ok = false; break; }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer
+      if (lane == 0 && leader) {
+        constexpr uint32_t idesc = ptx::idesc_f16(P::TM, BN);
+        auto commit = [](uint64_t* bar) {
+          if (PAIR) ptx::mma_commit_pair(bar);
+          else ptx::mma_commit(bar);
+        };
+        auto mma = [](uint32_t d, uint64_t x, uint64_t y, uint32_t acc) {
+          if (PAIR) ptx::mma_f16_ss_pair(d, x, y, idesc, acc);
+          else ptx::mma_f16_ss(d, x, y, idesc, acc);
+        };
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        // A unit of work is one run of a.run stages of a tile: each has an accumulator of its own.
+        const int runs = (a.num_kc + a.run - 1) / a.run;
+        const int64_t mine = unit < total ? (total - unit + units - 1) / units : 0;
+        for (int64_t w = 0; w < mine * runs && ok; ++w) {
+          if (!ptx::mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1, a.status, a.timeout_ns)) break;
           ptx::tc_fence_after();
-          const uint32_t s = ptx::smem_u32(smem + stage * P::STAGE);
+          const uint32_t d = tmem + (uint32_t)(acc * BN);
+          const int run = (int)(w % runs);
+          const int depth = min(a.run, a.num_kc - run * a.run);
+          for (int kc = 0; kc < depth; ++kc) {
+            if (!ptx::mbar_wait_bounded(&full[stage], phase, a.status, a.timeout_ns)) { ok = false; break; }
+            ptx::tc_fence_after();
+            const uint32_t s = ptx::smem_u32(smem + stage * P::STAGE);
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            const uint32_t off = (uint32_t)k * 32;  // 16 fp16 along the swizzled row
-            const uint64_t phi = ptx::smem_desc(s + off, 16, 1024, 2);
-            const uint64_t plo = ptx::smem_desc(s + P::A_BYTES + off, 16, 1024, 2);
-            const uint64_t qhi = ptx::smem_desc(s + 2 * P::A_BYTES + off, 16, 1024, 2);
-            const uint64_t qlo = ptx::smem_desc(s + 2 * P::A_BYTES + P::B_BYTES + off, 16, 1024, 2);
-            mma(d, phi, qhi, (kc | k) != 0);
-            mma(d, phi, qlo, 1);
-            mma(d, plo, qhi, 1);
+            for (int k = 0; k < BK / 16; ++k) {
+              const uint32_t off = (uint32_t)k * 32;  // 16 fp16 along the swizzled row
+              const uint64_t phi = ptx::smem_desc(s + off, 16, 1024, 2);
+              const uint64_t plo = ptx::smem_desc(s + P::A_BYTES + off, 16, 1024, 2);
+              const uint64_t qhi = ptx::smem_desc(s + 2 * P::A_BYTES + off, 16, 1024, 2);
+              const uint64_t qlo = ptx::smem_desc(s + 2 * P::A_BYTES + P::B_BYTES + off, 16, 1024, 2);
+              mma(d, phi, qhi, (kc | k) != 0);
+              mma(d, phi, qlo, 1);
+              mma(d, plo, qhi, 1);
+            }
+            commit(&empty[stage]);
+            if (++stage == P::STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
-          commit(&empty[stage]);
-          if (++stage == P::STAGES) {
-            stage = 0;
-            phase ^= 1;
+          if (!ok) break;
+          commit(&acc_full[acc]);
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1;
           }
         }
-        if (!ok) break;
-        commit(&acc_full[acc]);
-        if (++acc == 2) {
-          acc = 0;
-          acc_phase ^= 1;
-        }
+        commit(drain);  // every MMA issued so far finishes before TMEM is freed
+        ptx::mbar_wait_bounded(drain, 0, a.status, a.timeout_ns);
       }
-      commit(drain);  // every MMA issued so far finishes before TMEM is freed
-      ptx::mbar_wait_bounded(drain, 0, a.status, a.timeout_ns);
     }
   } else {
+    ptx::regs_grow<kRegsHigh>();
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;           // TMEM lane quadrant this warp may access
-    const int h = (warp - 2) >> 2;    // half of the tile's columns
+    const int h = (warp - 4) >> 2;    // half of the tile's columns
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int64_t t = unit; t < total; t += units) {
@@ -293,17 +314,55 @@ __global__ void __launch_bounds__(kThreads, 1)
       const StepScale sc = a.scale[(int64_t)z * a.scale_stride];
       const float alpha = a.kind == 0 ? sc.gram : a.kind == 1 ? sc.square : sc.product;
       const float beta = a.kind == 0 ? 0.f : a.kind == 1 ? sc.linear : sc.keep;
-      if (!ptx::mbar_wait_bounded(&acc_full[acc], acc_phase, a.status, a.timeout_ns)) break;
-      ptx::tc_fence_after();
+      // All runs but the last are added up in registers; the last one's accumulator takes the total,
+      // so that the stores below go over it 32 columns at a time.
+      const int runs = (a.num_kc + a.run - 1) / a.run;
+      const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * (BN / 2));
+      float sum[BN / 2];
+      bool ok = true;
+      for (int run = 0; run < runs; ++run) {
+        if (!ptx::mbar_wait_bounded(&acc_full[acc], acc_phase, a.status, a.timeout_ns)) { ok = false; break; }
+        ptx::tc_fence_after();
+        if (runs == 1) break;
+#pragma unroll
+        for (int c = 0; c < BN / 64; ++c) {
+          uint32_t v[32];
+          const uint32_t at = lanes + (uint32_t)(acc * BN + c * 32);
+          ptx::tmem_ld32(at, v);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            sum[c * 32 + e] = run == 0 ? __uint_as_float(v[e]) : sum[c * 32 + e] + __uint_as_float(v[e]);
+          if (run + 1 == runs) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(sum[c * 32 + e]);
+            ptx::tmem_st32(at, v);
+          }
+        }
+        if (run + 1 == runs) {
+          ptx::tmem_wait_st();
+          break;
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) ptx::mbar_arrive_cluster(ptx::map_to_rank(&acc_empty[acc], 0));
+          else ptx::mbar_arrive(&acc_empty[acc]);
+        }
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+      }
+      if (!ok) break;
 #pragma unroll 1
       for (int c = 0; c < BN / 64; ++c) {
-        const int col = h * (BN / 2) + c * 32;
-        const int64_t j0 = (int64_t)tn * BN + col;
+        const int64_t j0 = (int64_t)tn * BN + h * (BN / 2) + c * 32;
         uint32_t v[32];
         __syncwarp();  // the TMEM load is a whole warp's
-        ptx::tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + col), v);
+        ptx::tmem_ld32(lanes + (uint32_t)(acc * BN + c * 32), v);
         ptx::tmem_wait_ld();
-        if (c == BN / 64 - 1) {  // the accumulator goes back before the stores
+        if (c == BN / 64 - 1) {  // the accumulator goes back before the last stores
           ptx::tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -624,6 +683,12 @@ cudaError_t launch_gemm(const Split& p, const Split& q, GemmArgs a, cudaStream_t
   auto k = ortho_gemm_kernel<PAIR, BN, OUT>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PL::SMEM);
   if (e != cudaSuccess) return e;
+  // The register split must fit into what the block is launched with, or it would wait for ever.
+  static const int regs = [&] {
+    cudaFuncAttributes fa{};
+    return cudaFuncGetAttributes(&fa, k) == cudaSuccess ? fa.numRegs : 0;
+  }();
+  if (regs < kRegs) return cudaErrorInvalidConfiguration;
   const int units = PAIR ? device_sm_count() / 2 : device_sm_count();
   const unsigned grid = (unsigned)std::min<int64_t>(total, units);
   if (PAIR) return launch_kernel_cluster(k, dim3(2 * grid), dim3(kThreads), PL::SMEM, 2, stream, m[0], m[1], m[2], m[3], a);
@@ -704,6 +769,7 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
   GemmArgs base{};
   base.batch = (int)o.batch;
   base.scale_stride = o.steps;
+  base.run = o.dtype == LM_F32 ? 4 : o.dtype == LM_F16 ? 16 : 32;
   base.status = status;
   base.timeout_ns = wc.timeout_ns;
   base.debug_skip_first_load = wc.debug_skip_first_load;

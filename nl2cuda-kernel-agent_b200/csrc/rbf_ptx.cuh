@@ -264,6 +264,13 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
       : "memory");
 }
 
+// Registers per thread of this warpgroup from here on (all its warps execute it).  The growing
+// groups wait for what the shrinking ones release, out of what the block was launched with.
+template <int N>
+__device__ __forceinline__ void regs_grow() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_shrink() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // ---------------------------------------------------------------- CTA pairs (cta_group::2)
 // A cluster of two CTAs on one TPC shares each MMA: the even-ranked CTA issues
 // tcgen05.mma.cta_group::2 with M = 256 (128 rows of A from each CTA's shared memory, at the same
