@@ -7,7 +7,7 @@
 // All three products run as D = P Q^T with both operands K-major, on tcgen05.mma kind::f16: A takes
 // X twice, A^2 takes A twice (A is symmetric), and B X takes B and X^T, so every step keeps X in
 // both orders.  A and B are symmetric: only tiles that touch the lower triangle are computed, and
-// each value is stored at (i, j) and (j, i).  Flops of a step: r^2 c + r^3 + 2 r^2 c.
+// each block of 32 x 32 below the diagonal is stored at (i, j) and turned around at (j, i).  Flops of a step: r^2 c + r^3 + 2 r^2 c.
 //
 // Precision: 3 x fp16.  An operand v is kept as v * 2^k = hi + lo, hi = fp16(v 2^k) and
 // lo = fp16(v 2^k - hi), and P Q^T = hi hi^T + hi lo^T + lo hi^T in fp32: 22 bits of each operand,
@@ -27,10 +27,12 @@
 // for fp16 and 2048 for bf16, whose own rounding is far larger: short runs cost up to 9% of the time.
 //
 // Kernel (persistent): warp 0 loads operand slices by TMA (64 deep, 128-byte swizzle, hi and lo of
-// both operands) into a ring of stages; one thread of warp 1 issues 3 x 4 MMAs per stage into one of
-// two TMEM accumulators; warps 4..11 read the other one, apply the epilogue and store.  Large
-// products run on CTA pairs (cta_group::2): a 256 x 256 tile reads 64 KiB of operands per CTA and
-// slice for 12 MMAs, two thirds of what a single CTA's 128 x 256 tile would.  No multicast.
+// both operands) into a ring of stages; warp 1 issues 3 x 4 MMAs per stage into one of
+// two TMEM accumulators; warps 4..11 read the other one, apply the epilogue and store.  All
+// on CTA pairs (cta_group::2), tiles of 256 x 256, 128 or 64: a CTA of the pair loads its 128 rows of P
+// and half of the tile's rows of Q, for 256 x 256 two thirds of what a single CTA's 128 x 256 tile
+// takes.  That counts: an SM takes in about 64 bytes a cycle, so narrower tiles wait for their
+// operands.  No multicast.
 // Every mbarrier wait is bounded, as in rbf_fwd_tc.cu.
 #include <cuda.h>
 
@@ -44,6 +46,7 @@ namespace rbf {
 namespace lm {
 namespace {
 
+constexpr int kTileRows = 256;                 // of a CTA pair's tile, 128 rows per CTA
 constexpr int BK = 64;                         // operand depth of a stage: 128 bytes of fp16
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 32 * (4 + kEpiWarps);  // a warpgroup for the loads and MMAs, two for the epilogue
@@ -52,6 +55,9 @@ constexpr int kThreads = 32 * (4 + kEpiWarps);  // a warpgroup for the loads and
 constexpr int kRegs = 168, kRegsLow = 40, kRegsHigh = 232;
 static_assert(kRegsLow + 2 * kRegsHigh <= 3 * kRegs && kThreads == 384, "register split");
 constexpr size_t kSmemMax = 232448;
+// Each epilogue warp turns 16 columns x 32 rows around at a time; the pitch keeps 16-byte reads of
+// eight columns on different banks.
+constexpr int kTurnPitch = 36, kTurnWords = 16 * kTurnPitch;
 
 // Scale factors of one step of one matrix (see scale_table).
 struct StepScale {
@@ -63,7 +69,7 @@ struct StepScale {
 enum class Out { kSymmetric, kBoth, kFinal };
 
 struct GemmArgs {
-  int64_t M, N, K;          // D [M, N] per matrix
+  int64_t M, N;             // D [M, N] per matrix
   int tiles_m, tiles_n, batch;
   int64_t tiles;            // of one matrix
   int num_kc;
@@ -76,7 +82,7 @@ struct GemmArgs {
   const __half* add_lo;
   __half* d_hi;             // row-major [M, ld_d]
   __half* d_lo;
-  __half* t_hi;             // transposed [N, ld_t]
+  __half* t_hi;             // transposed [N, ld_t]; pitches are multiples of 32
   __half* t_lo;
   int64_t ld_d, ld_t, d_matrix, t_matrix;  // strides of rows and of matrices, in elements
   void* out;                // kFinal: out[col * ld_out + row], type out_dtype
@@ -88,8 +94,8 @@ struct GemmArgs {
 };
 
 // Tile t of a matrix.  Symmetric products: only tiles with a row >= their first column, so
-// `per` = TM / TN more column tiles for each further row tile.
-template <int TM, int TN, bool SYM>
+// `per` more column tiles for each further row tile.
+template <int BN, bool SYM>
 __device__ __forceinline__ void tile_of(int64_t t, const GemmArgs& a, int& tm, int& tn) {
   if (!SYM) {
     // Bands of 8 row tiles, so that the tiles in flight share both operands in L2.
@@ -103,7 +109,7 @@ __device__ __forceinline__ void tile_of(int64_t t, const GemmArgs& a, int& tm, i
     tn = (int)(in / rows);
     return;
   }
-  constexpr int per = TM / TN;
+  constexpr int per = kTileRows / BN;
   int row = 0;
   int64_t left = t;
   while (true) {
@@ -116,31 +122,39 @@ __device__ __forceinline__ void tile_of(int64_t t, const GemmArgs& a, int& tm, i
   tn = (int)left;
 }
 
+// Eight (hi, lo) pairs as eight hi and eight lo.
+__device__ __forceinline__ void unzip(const uint32_t* w, uint4& hi, uint4& lo) {
+  hi = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410),
+                  __byte_perm(w[4], w[5], 0x5410), __byte_perm(w[6], w[7], 0x5410));
+  lo = make_uint4(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632),
+                  __byte_perm(w[4], w[5], 0x7632), __byte_perm(w[6], w[7], 0x7632));
+}
+
 __device__ __forceinline__ void split_f16(float x, __half& hi, __half& lo) {
   hi = __float2half_rn(x);
   lo = __float2half_rn(x - __half2float(hi));
 }
 
-template <bool PAIR, int BN, Out OUT>
+template <int BN>
 struct Plan {
-  static constexpr int TM = PAIR ? 256 : 128;          // rows of a tile
-  static constexpr int BROWS = PAIR ? BN / 2 : BN;     // rows of Q each CTA loads
+  static constexpr int BROWS = BN / 2;   // rows of Q each CTA loads
   static constexpr uint32_t A_BYTES = 128 * BK * 2;
   static constexpr uint32_t B_BYTES = BROWS * BK * 2;
   static constexpr uint32_t STAGE = 2 * (A_BYTES + B_BYTES);
-  static constexpr int STAGES = (int)((kSmemMax - 2048) / STAGE) > 6 ? 6 : (int)((kSmemMax - 2048) / STAGE);
-  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 256;
+  static constexpr size_t FIXED = 1024 + 256 + sizeof(uint32_t) * kEpiWarps * kTurnWords;
+  static constexpr int STAGES = (int)((kSmemMax - FIXED) / STAGE);
+  static constexpr size_t SMEM = FIXED + (size_t)STAGES * STAGE;
   static constexpr uint32_t TCOLS = 2 * BN;
   static_assert(STAGES >= 2 && SMEM <= kSmemMax, "stages");
 };
 
-template <bool PAIR, int BN, Out OUT>
+template <int BN, Out OUT>
 __global__ void __launch_bounds__(kThreads, 1)
     ortho_gemm_kernel(const __grid_constant__ CUtensorMap tm_phi,
                       const __grid_constant__ CUtensorMap tm_plo,
                       const __grid_constant__ CUtensorMap tm_qhi,
                       const __grid_constant__ CUtensorMap tm_qlo, const GemmArgs a) {
-  using P = Plan<PAIR, BN, OUT>;
+  using P = Plan<BN>;
   constexpr bool SYM = OUT == Out::kSymmetric;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -154,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? ptx::cluster_ctarank() : 0;
+  const uint32_t rank = ptx::cluster_ctarank();
   const bool leader = rank == 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < P::STAGES; ++s) {
@@ -163,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       ptx::mbar_init(&acc_full[b], 1);
-      ptx::mbar_init(&acc_empty[b], PAIR ? 2 * kEpiWarps : kEpiWarps);
+      ptx::mbar_init(&acc_empty[b], 2 * kEpiWarps);
     }
     ptx::mbar_init(drain, 1);
     ptx::fence_mbar_init();
@@ -174,15 +188,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     ptx::prefetch_tensormap(&tm_qhi);
     ptx::prefetch_tensormap(&tm_qlo);
   }
-  if (PAIR) ptx::cluster_sync();  // the peer's barriers exist before any remote arrive
+  ptx::cluster_sync();  // the peer's barriers exist before any remote arrive
   if (warp == 1) {
-    if (PAIR) {
-      ptx::tmem_alloc_pair(tmem_slot, P::TCOLS);
-      ptx::tmem_relinquish_pair();
-    } else {
-      ptx::tmem_alloc(tmem_slot, P::TCOLS);
-      ptx::tmem_relinquish();
-    }
+    ptx::tmem_alloc_pair(tmem_slot, P::TCOLS);
+    ptx::tmem_relinquish_pair();
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -190,8 +199,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   ptx::griddep_wait();  // the operands come from the previous kernel
   const int64_t total = a.tiles * a.batch;
-  const int64_t unit = PAIR ? (blockIdx.x >> 1) : blockIdx.x;
-  const int64_t units = PAIR ? (gridDim.x >> 1) : gridDim.x;
+  const int64_t unit = blockIdx.x >> 1;
+  const int64_t units = gridDim.x >> 1;
 
   if (warp < 4) {
     ptx::regs_shrink<kRegsLow>();
@@ -204,28 +213,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int64_t t = unit; t < total && ok; t += units) {
           const int z = (int)(t / a.tiles);
           int tm, tn;
-          tile_of<P::TM, BN, SYM>(t - z * a.tiles, a, tm, tn);
-          const int i0 = tm * P::TM + (int)rank * 128;
-          const int j0 = tn * BN + (int)rank * (PAIR ? P::BROWS : 0);
+          tile_of<BN, SYM>(t - z * a.tiles, a, tm, tn);
+          const int i0 = tm * kTileRows + (int)rank * 128;
+          const int j0 = tn * BN + (int)rank * P::BROWS;
           for (int kc = 0; kc < a.num_kc; ++kc) {
             if (!ptx::mbar_wait_bounded(&empty[stage], phase ^ 1, a.status, a.timeout_ns)) { ok = false; break; }
             if (a.debug_skip_first_load && !skipped && blockIdx.x == 0) {
               skipped = true;  // test hook: this stage never fills, so its consumer times out
             } else {
               uint8_t* s = smem + stage * P::STAGE;
-              if (leader) ptx::mbar_arrive_expect_tx(&full[stage], (PAIR ? 2 : 1) * P::STAGE);
-              if (PAIR) {
-                const uint32_t fc = ptx::map_to_rank(&full[stage], 0);
-                ptx::tma_load_3d_pair(s, &tm_phi, kc * BK, i0, z, fc);
-                ptx::tma_load_3d_pair(s + P::A_BYTES, &tm_plo, kc * BK, i0, z, fc);
-                ptx::tma_load_3d_pair(s + 2 * P::A_BYTES, &tm_qhi, kc * BK, j0, z, fc);
-                ptx::tma_load_3d_pair(s + 2 * P::A_BYTES + P::B_BYTES, &tm_qlo, kc * BK, j0, z, fc);
-              } else {
-                ptx::tma_load_3d(s, &tm_phi, kc * BK, i0, z, &full[stage]);
-                ptx::tma_load_3d(s + P::A_BYTES, &tm_plo, kc * BK, i0, z, &full[stage]);
-                ptx::tma_load_3d(s + 2 * P::A_BYTES, &tm_qhi, kc * BK, j0, z, &full[stage]);
-                ptx::tma_load_3d(s + 2 * P::A_BYTES + P::B_BYTES, &tm_qlo, kc * BK, j0, z, &full[stage]);
-              }
+              if (leader) ptx::mbar_arrive_expect_tx(&full[stage], 2 * P::STAGE);
+              const uint32_t fc = ptx::map_to_rank(&full[stage], 0);
+              ptx::tma_load_3d_pair(s, &tm_phi, kc * BK, i0, z, fc);
+              ptx::tma_load_3d_pair(s + P::A_BYTES, &tm_plo, kc * BK, i0, z, fc);
+              ptx::tma_load_3d_pair(s + 2 * P::A_BYTES, &tm_qhi, kc * BK, j0, z, fc);
+              ptx::tma_load_3d_pair(s + 2 * P::A_BYTES + P::B_BYTES, &tm_qlo, kc * BK, j0, z, fc);
               if (leader) {
                 issued |= 1u << stage;
                 last = (last & ~(1u << stage)) | (phase << stage);
@@ -244,58 +246,54 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (issued >> s & 1u) ptx::mbar_wait_bounded(&full[s], (last >> s) & 1u, a.status, a.timeout_ns);
       }
     } else if (warp == 1) {
-      // ------------------------------------------------------------ MMA issuer
-      if (lane == 0 && leader) {
-        constexpr uint32_t idesc = ptx::idesc_f16(P::TM, BN);
-        auto commit = [](uint64_t* bar) {
-          if (PAIR) ptx::mma_commit_pair(bar);
-          else ptx::mma_commit(bar);
-        };
-        auto mma = [](uint32_t d, uint64_t x, uint64_t y, uint32_t acc) {
-          if (PAIR) ptx::mma_f16_ss_pair(d, x, y, idesc, acc);
-          else ptx::mma_f16_ss(d, x, y, idesc, acc);
-        };
+      // ------------------------------------------------------------ MMA issuer (the whole warp)
+      if (leader) {
+        constexpr uint32_t idesc = ptx::idesc_f16(kTileRows, BN);
+        const uint32_t elected = ptx::elect_one();
+        const uint64_t base = ptx::smem_desc(ptx::smem_u32(smem), 16, 1024, 2);
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
         // A unit of work is one run of a.run stages of a tile: each has an accumulator of its own.
         const int runs = (a.num_kc + a.run - 1) / a.run;
-        const int64_t mine = unit < total ? (total - unit + units - 1) / units : 0;
-        for (int64_t w = 0; w < mine * runs && ok; ++w) {
-          if (!ptx::mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1, a.status, a.timeout_ns)) break;
-          ptx::tc_fence_after();
-          const uint32_t d = tmem + (uint32_t)(acc * BN);
-          const int run = (int)(w % runs);
-          const int depth = min(a.run, a.num_kc - run * a.run);
-          for (int kc = 0; kc < depth; ++kc) {
-            if (!ptx::mbar_wait_bounded(&full[stage], phase, a.status, a.timeout_ns)) { ok = false; break; }
+        for (int64_t t = unit; t < total && ok; t += units) {
+          for (int run = 0; run < runs && ok; ++run) {
+            if (!ptx::mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1, a.status, a.timeout_ns)) { ok = false; break; }
             ptx::tc_fence_after();
-            const uint32_t s = ptx::smem_u32(smem + stage * P::STAGE);
+            const uint32_t d = tmem + (uint32_t)(acc * BN);
+            const int depth = min(a.run, a.num_kc - run * a.run);
+            for (int kc = 0; kc < depth; ++kc) {
+              if (!ptx::mbar_wait_bounded(&full[stage], phase, a.status, a.timeout_ns)) { ok = false; break; }
+              ptx::tc_fence_after();
+              // Descriptors of the stage's four operands: the address field counts 16 bytes.
+              const uint64_t phi = base + (uint32_t)stage * (P::STAGE >> 4);
+              const uint64_t plo = phi + (P::A_BYTES >> 4);
+              const uint64_t qhi = phi + (2 * P::A_BYTES >> 4);
+              const uint64_t qlo = phi + ((2 * P::A_BYTES + P::B_BYTES) >> 4);
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k) {
-              const uint32_t off = (uint32_t)k * 32;  // 16 fp16 along the swizzled row
-              const uint64_t phi = ptx::smem_desc(s + off, 16, 1024, 2);
-              const uint64_t plo = ptx::smem_desc(s + P::A_BYTES + off, 16, 1024, 2);
-              const uint64_t qhi = ptx::smem_desc(s + 2 * P::A_BYTES + off, 16, 1024, 2);
-              const uint64_t qlo = ptx::smem_desc(s + 2 * P::A_BYTES + P::B_BYTES + off, 16, 1024, 2);
-              mma(d, phi, qhi, (kc | k) != 0);
-              mma(d, phi, qlo, 1);
-              mma(d, plo, qhi, 1);
+              for (int k = 0; k < BK / 16; ++k) {  // 16 fp16 are 32 bytes along the swizzled row
+                ptx::mma_f16_ss_pair(d, phi + 2 * k, qhi + 2 * k, idesc, (kc | k) != 0, elected);
+                ptx::mma_f16_ss_pair(d, phi + 2 * k, qlo + 2 * k, idesc, 1, elected);
+                ptx::mma_f16_ss_pair(d, plo + 2 * k, qhi + 2 * k, idesc, 1, elected);
+              }
+              if (elected) ptx::mma_commit_pair(&empty[stage]);
+              __syncwarp();
+              if (++stage == P::STAGES) {
+                stage = 0;
+                phase ^= 1;
+              }
             }
-            commit(&empty[stage]);
-            if (++stage == P::STAGES) {
-              stage = 0;
-              phase ^= 1;
+            if (!ok) break;
+            if (elected) ptx::mma_commit_pair(&acc_full[acc]);
+            __syncwarp();
+            if (++acc == 2) {
+              acc = 0;
+              acc_phase ^= 1;
             }
-          }
-          if (!ok) break;
-          commit(&acc_full[acc]);
-          if (++acc == 2) {
-            acc = 0;
-            acc_phase ^= 1;
           }
         }
-        commit(drain);  // every MMA issued so far finishes before TMEM is freed
+        if (elected) ptx::mma_commit_pair(drain);  // every MMA issued so far finishes before TMEM is freed
+        __syncwarp();
         ptx::mbar_wait_bounded(drain, 0, a.status, a.timeout_ns);
       }
     }
@@ -304,13 +302,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;           // TMEM lane quadrant this warp may access
     const int h = (warp - 4) >> 2;    // half of the tile's columns
+    uint32_t* turn = reinterpret_cast<uint32_t*>(smem + P::STAGES * P::STAGE + 256) + (warp - 4) * kTurnWords;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int64_t t = unit; t < total; t += units) {
       const int z = (int)(t / a.tiles);
       int tm, tn;
-      tile_of<P::TM, BN, SYM>(t - z * a.tiles, a, tm, tn);
-      const int64_t i = (int64_t)tm * P::TM + rank * 128 + q * 32 + lane;
+      tile_of<BN, SYM>(t - z * a.tiles, a, tm, tn);
+      const int64_t i0 = (int64_t)tm * kTileRows + rank * 128 + q * 32;
+      const int64_t i = i0 + lane;
       const StepScale sc = a.scale[(int64_t)z * a.scale_stride];
       const float alpha = a.kind == 0 ? sc.gram : a.kind == 1 ? sc.square : sc.product;
       const float beta = a.kind == 0 ? 0.f : a.kind == 1 ? sc.linear : sc.keep;
@@ -345,82 +345,86 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if (PAIR) ptx::mbar_arrive_cluster(ptx::map_to_rank(&acc_empty[acc], 0));
-          else ptx::mbar_arrive(&acc_empty[acc]);
-        }
+        if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(&acc_empty[acc], 0));
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1;
         }
       }
       if (!ok) break;
+      // Eight columns at a time, in a loop that is not unrolled: instructions that run once in a launch
+      // are fetched from L2, and took most of a small product's time when this was straight-line.
 #pragma unroll 1
-      for (int c = 0; c < BN / 64; ++c) {
-        const int64_t j0 = (int64_t)tn * BN + h * (BN / 2) + c * 32;
-        uint32_t v[32];
+      for (int g = 0; g < BN / 16; ++g) {
+        const int64_t j0 = (int64_t)tn * BN + h * (BN / 2) + g * 8;
+        uint32_t v[8];
         __syncwarp();  // the TMEM load is a whole warp's
-        ptx::tmem_ld32(lanes + (uint32_t)(acc * BN + c * 32), v);
+        ptx::tmem_ld8(lanes + (uint32_t)(acc * BN + g * 8), v);
         ptx::tmem_wait_ld();
-        if (c == BN / 64 - 1) {  // the accumulator goes back before the last stores
+        if (g == BN / 16 - 1) {  // the accumulator goes back before the last stores
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            if (PAIR) ptx::mbar_arrive_cluster(ptx::map_to_rank(&acc_empty[acc], 0));
-            else ptx::mbar_arrive(&acc_empty[acc]);
-          }
+          if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(&acc_empty[acc], 0));
         }
-        if (j0 >= a.N || i >= a.M) continue;
-        if (SYM && j0 > i) continue;
-        float f[32];
+        // Blocks of 32 x 32, one row a lane: below the diagonal, on it, or above it.  These tests come
+        // out the same for the whole warp.
+        const int64_t block = j0 & ~(int64_t)31;
+        if (j0 >= a.N || i0 >= a.M || (SYM && block > i0)) continue;
+        float f[8];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = alpha * __uint_as_float(v[e]);
-        if (a.add_hi != nullptr) {
-          // ld_d is a multiple of 32, so a chunk of 32 columns lies inside its row.
+        for (int e = 0; e < 8; ++e) f[e] = alpha * __uint_as_float(v[e]);
+        if (a.add_hi != nullptr && i < a.M) {
+          // Row pitches are multiples of 32, so eight columns lie inside their row.
           const int64_t at = z * a.d_matrix + i * a.ld_d + j0;
+          const Pack<__half, 8> hi = *reinterpret_cast<const Pack<__half, 8>*>(a.add_hi + at);
+          const Pack<__half, 8> lo = *reinterpret_cast<const Pack<__half, 8>*>(a.add_lo + at);
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const Pack<__half, 8> hi = *reinterpret_cast<const Pack<__half, 8>*>(a.add_hi + at + 8 * g);
-            const Pack<__half, 8> lo = *reinterpret_cast<const Pack<__half, 8>*>(a.add_lo + at + 8 * g);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              f[8 * g + e] = fmaf(beta, __half2float(hi.v[e]) + __half2float(lo.v[e]), f[8 * g + e]);
-          }
+          for (int e = 0; e < 8; ++e) f[e] = fmaf(beta, __half2float(hi.v[e]) + __half2float(lo.v[e]), f[e]);
         }
         if constexpr (OUT == Out::kFinal) {
+          if (i < a.M) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (j0 + e < a.N) store_as(a.out, z * a.out_matrix + (j0 + e) * a.ld_out + i, a.out_dtype, f[e]);
-        } else {
-          Pack<__half, 32> hi, lo;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) split_f16(f[e], hi.v[e], lo.v[e]);
-          __half* dh = a.d_hi + z * a.d_matrix + i * a.ld_d + j0;
-          __half* dl = a.d_lo + z * a.d_matrix + i * a.ld_d + j0;
-          if (!SYM || j0 + 31 <= i) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              *reinterpret_cast<uint4*>(dh + 8 * g) = reinterpret_cast<const uint4*>(&hi)[g];
-              *reinterpret_cast<uint4*>(dl + 8 * g) = reinterpret_cast<const uint4*>(&lo)[g];
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (j0 + e <= i) {
-                dh[e] = hi.v[e];
-                dl[e] = lo.v[e];
-              }
+            for (int e = 0; e < 8; ++e)
+              if (j0 + e < a.N) store_as(a.out, z * a.out_matrix + (j0 + e) * a.ld_out + i, a.out_dtype, f[e]);
           }
-          // The other order: the lanes of a warp write 32 consecutive values.
-          __half* th = (SYM ? a.d_hi : a.t_hi) + z * (SYM ? a.d_matrix : a.t_matrix) + i;
-          __half* tl = (SYM ? a.d_lo : a.t_lo) + z * (SYM ? a.d_matrix : a.t_matrix) + i;
-          const int64_t ld = SYM ? a.ld_d : a.ld_t;
+        } else {
+          uint32_t both[8];  // hi in the low half, lo in the high half
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (j0 + e < (SYM ? i : a.N)) {
-              th[(j0 + e) * ld] = hi.v[e];
-              tl[(j0 + e) * ld] = lo.v[e];
+          for (int e = 0; e < 8; ++e) {
+            __half hi, lo;
+            split_f16(f[e], hi, lo);
+            both[e] = (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
+          }
+          uint4 hi, lo;
+          if (i < a.M) {
+            unzip(both, hi, lo);
+            const int64_t at = z * a.d_matrix + i * a.ld_d + j0;
+            *reinterpret_cast<uint4*>(a.d_hi + at) = hi;
+            *reinterpret_cast<uint4*>(a.d_lo + at) = lo;
+          }
+          if (SYM && block == i0) continue;  // a block on the diagonal is computed whole
+          // The other order, turned around in shared memory 16 columns at a time: lane l then holds
+          // half of column l % 16.
+#pragma unroll
+          for (int e = 0; e < 8; ++e) turn[((g & 1) * 8 + e) * kTurnPitch + lane] = both[e];
+          if ((g & 1) == 0 && j0 + 8 < a.N) continue;
+          __syncwarp();
+          const int col = lane & 15, part = lane >> 4;
+          const int64_t j = (j0 & ~(int64_t)15) + col;
+          __half* th = (SYM ? a.d_hi : a.t_hi) + z * (SYM ? a.d_matrix : a.t_matrix);
+          __half* tl = (SYM ? a.d_lo : a.t_lo) + z * (SYM ? a.d_matrix : a.t_matrix);
+          const int64_t at = j * (SYM ? a.ld_d : a.ld_t) + i0 + part * 16;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            uint32_t w[8];
+            *reinterpret_cast<uint4*>(&w[0]) = *reinterpret_cast<const uint4*>(&turn[col * kTurnPitch + part * 16 + 8 * k]);
+            *reinterpret_cast<uint4*>(&w[4]) = *reinterpret_cast<const uint4*>(&turn[col * kTurnPitch + part * 16 + 8 * k + 4]);
+            unzip(w, hi, lo);
+            if (j < a.N) {
+              *reinterpret_cast<uint4*>(th + at + 8 * k) = hi;
+              *reinterpret_cast<uint4*>(tl + at + 8 * k) = lo;
             }
+          }
         }
       }
       if (++acc == 2) {
@@ -432,11 +436,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   ptx::griddep_launch_dependents();
   ptx::tc_fence_before();
   __syncthreads();
-  if (PAIR) ptx::cluster_sync();  // neither CTA leaves before both are done with each other's memory
+  ptx::cluster_sync();  // neither CTA leaves before both are done with each other's memory
   if (warp == 1) {
     ptx::tc_fence_after();
-    if (PAIR) ptx::tmem_dealloc_pair(tmem, P::TCOLS);
-    else ptx::tmem_dealloc(tmem, P::TCOLS);
+    ptx::tmem_dealloc_pair(tmem, P::TCOLS);
   }
 }
 
@@ -444,7 +447,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 constexpr int kMaxSteps = 32;
 constexpr int kNormThreads = 256;
-constexpr int kMaxNormParts = 256;
 
 struct PrepArgs {
   const void* g;
@@ -462,33 +464,51 @@ struct PrepArgs {
   int* status;
 };
 
-template <typename T>
-__device__ __forceinline__ float g_at(const PrepArgs& a, int64_t z, int64_t i, int64_t j) {
-  return to_f32(static_cast<const T*>(a.g)[z * a.matrix_stride + i * a.row_stride + j]);
-}
+// Sums of squares in 64 bits: an update of any magnitude has a norm.  A warp takes pieces of
+// kNormPiece packs a lane of one row.
+constexpr int kNormPiece = 4;
 
-// Sums of squares in 64 bits: an update of any magnitude has a norm.
-template <typename T>
+template <typename T, int VEC>
 __global__ void __launch_bounds__(kNormThreads) ortho_norm_kernel(const PrepArgs a) {
   __shared__ double red[kNormThreads / 32];
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
-  const int64_t z = blockIdx.y, p = blockIdx.x;
-  if (z == 0 && p == 0 && threadIdx.x == 0) *a.status = 0;
+  const int64_t z = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (z == 0 && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
+  constexpr int piece = 32 * kNormPiece * VEC;
+  const int64_t per_row = (a.cols + piece - 1) / piece, items = per_row * a.rows;
+  const int64_t warps = (int64_t)a.parts * (kNormThreads / 32);
   double s = 0.0;
-  for (int64_t i = a.rows * p / a.parts; i < a.rows * (p + 1) / a.parts; ++i) {
+  for (int64_t it = (int64_t)blockIdx.x * (kNormThreads / 32) + warp; it < items; it += warps) {
+    const int64_t i = it / per_row;
+    const int64_t j0 = (it - i * per_row) * piece + lane * VEC;
     const T* row = static_cast<const T*>(a.g) + z * a.matrix_stride + i * a.row_stride;
-    for (int64_t j = threadIdx.x; j < a.cols; j += kNormThreads) {
-      const double v = to_f32(row[j]);
-      s = fma(v, v, s);
+    Pack<T, VEC> p[kNormPiece];
+#pragma unroll
+    for (int u = 0; u < kNormPiece; ++u) {
+      const int64_t j = j0 + u * 32 * VEC;
+      if (j < a.cols) {
+        p[u] = *reinterpret_cast<const Pack<T, VEC>*>(row + j);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) p[u].v[e] = from_f32<T>(0.f);
+      }
     }
+#pragma unroll
+    for (int u = 0; u < kNormPiece; ++u)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const double v = to_f32(p[u].v[e]);
+        s = fma(v, v, s);
+      }
   }
   s = warp_sum(s);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  if (lane == 0) red[warp] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < kNormThreads / 32; ++w) s += red[w];
-    a.part[z * a.parts + p] = s;
+    a.part[z * a.parts + blockIdx.x] = s;
   }
 }
 
@@ -518,12 +538,14 @@ __device__ double max_on(double top, double c1, double c3, double c5) {
   return m;
 }
 
-// The scales of every step of one matrix; returns that of X_0.  `rho` bounds |X_0|_F.
-__device__ double scale_table(double rho, const PrepArgs& a, StepScale* out) {
-  const double slack = 1.0 + 1e-3;  // for rounding along the way
-  double bound = rho * slack;
-  double sx = pow2_scale(bound);
-  const double first = sx;
+constexpr double kSlack = 1.0 + 1e-3;  // on the bounds, for rounding along the way
+
+__device__ double first_scale(double rho) { return pow2_scale(rho * kSlack); }
+
+// The scales of every step of one matrix; rho is |X_0|_F.
+__device__ void scale_table(double rho, const PrepArgs& a, StepScale* out) {
+  double bound = rho * kSlack;
+  double sx = first_scale(rho);
   for (int k = 0; k < a.steps; ++k) {
     const double ca = a.coef[k][0], cb = a.coef[k][1], cc = a.coef[k][2];
     const double u = bound * bound;
@@ -534,68 +556,101 @@ __device__ double scale_table(double rho, const PrepArgs& a, StepScale* out) {
       const double peak = -cb / (2.0 * cc);
       if (peak > 0.0 && peak < u) mb = fmax(mb, fabs(peak * (cb + cc * peak)));
     }
-    const double sb = pow2_scale(mb * slack);
-    const double next = max_on(bound, ca, cb, cc) * slack;
+    const double sb = pow2_scale(mb * kSlack);
+    const double next = max_on(bound, ca, cb, cc) * kSlack;
     const double sn = k + 1 == a.steps ? 1.0 : pow2_scale(next);
-    if (out != nullptr) {
-      out[k].gram = (float)(sa / (sx * sx));
-      out[k].square = (float)(cc * sb / (sa * sa));
-      out[k].linear = (float)(cb * sb / sa);
-      out[k].product = (float)(sn / (sb * sx));
-      out[k].keep = (float)(ca * sn / sx);
-    }
+    out[k].gram = (float)(sa / (sx * sx));
+    out[k].square = (float)(cc * sb / (sa * sa));
+    out[k].linear = (float)(cb * sb / sa);
+    out[k].product = (float)(sn / (sb * sx));
+    out[k].keep = (float)(ca * sn / sx);
     bound = next;
     sx = sn;
   }
-  return first;
 }
 
 constexpr int kTile = 64;
+constexpr int kTilePitch = kTile + 1;
 
 // X_0 in both orders, a 64 x 64 tile of G per CTA; the first CTA of a matrix writes its scales.
-template <typename T>
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256) ortho_split_kernel(const PrepArgs a) {
-  __shared__ __half s_hi[kTile][kTile + 2], s_lo[kTile][kTile + 2];
+  __shared__ uint32_t tile[kTile * kTilePitch];  // hi in the low half, lo in the high half
   __shared__ double s_factor;
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   const int64_t z = blockIdx.z;
+  const int64_t i0 = (int64_t)blockIdx.y * kTile, j0 = (int64_t)blockIdx.x * kTile;
+  // 8 columns of two rows a thread; the loads do not wait for the norm.
+  const int cx = (threadIdx.x & 7) * 8, ry = threadIdx.x >> 3;
+  Pack<T, 8> p[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int64_t i = i0 + ry + 32 * u;
+    const T* row = static_cast<const T*>(a.g) + z * a.matrix_stride + i * a.row_stride;
+#pragma unroll
+    for (int e = 0; e < 8; e += VEC) {
+      const int64_t j = j0 + cx + e;
+      if (i < a.rows && j < a.cols) {
+        const Pack<T, VEC> q = *reinterpret_cast<const Pack<T, VEC>*>(row + j);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) p[u].v[e + k] = q.v[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) p[u].v[e + k] = from_f32<T>(0.f);
+      }
+    }
+  }
   if (threadIdx.x < 32) {
     double t = 0.0;
-    for (int p = threadIdx.x; p < a.parts; p += 32) t += a.part[z * a.parts + p];
+    for (int k = threadIdx.x; k < a.parts; k += 32) t += a.part[z * a.parts + k];
     t = warp_sum(t);
     if (threadIdx.x == 0) {
       const double norm = sqrt(t), den = norm + (double)a.eps;
       const bool first = blockIdx.x == 0 && blockIdx.y == 0;
-      const double sx = scale_table(den > 0.0 ? norm / den : 0.0, a, first ? a.scale + z * a.steps : nullptr);
-      s_factor = sx / den;
+      const double rho = den > 0.0 ? norm / den : 0.0;
+      s_factor = first_scale(rho) / den;
+      if (first) scale_table(rho, a, a.scale + z * a.steps);
     }
   }
   __syncthreads();
   const double factor = s_factor;
-  const int64_t i0 = (int64_t)blockIdx.y * kTile, j0 = (int64_t)blockIdx.x * kTile;
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-#pragma unroll 4
-  for (int r = ty; r < kTile; r += 4) {
-    const int64_t i = i0 + r, j = j0 + tx;
-    if (i < a.rows && j < a.cols) {
+  // In fp32 where the factor has its full precision there (one more rounding, the same for all).
+  const bool wide = !(fabs(factor) > 1e-30 && fabs(factor) < 1e30);
+  const float narrow = (float)factor;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int64_t i = i0 + ry + 32 * u;
+    uint32_t both[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float g = to_f32(p[u].v[e]);
       __half hi, lo;
-      split_f16((float)((double)g_at<T>(a, z, i, j) * factor), hi, lo);
-      const int64_t at = z * a.g_matrix + i * a.ld_g + j;
-      a.g_hi[at] = hi;
-      a.g_lo[at] = lo;
-      s_hi[r][tx] = hi;
-      s_lo[r][tx] = lo;
+      split_f16(wide ? (float)((double)g * factor) : g * narrow, hi, lo);
+      both[e] = (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
+      tile[(ry + 32 * u) * kTilePitch + cx + e] = both[e];
+    }
+    if (i < a.rows && j0 + cx < a.cols) {  // up to the pitch, a multiple of 32
+      uint4 hi, lo;
+      unzip(both, hi, lo);
+      const int64_t at = z * a.g_matrix + i * a.ld_g + j0 + cx;
+      *reinterpret_cast<uint4*>(a.g_hi + at) = hi;
+      *reinterpret_cast<uint4*>(a.g_lo + at) = lo;
     }
   }
   __syncthreads();
-#pragma unroll 4
-  for (int r = ty; r < kTile; r += 4) {
-    const int64_t j = j0 + r, i = i0 + tx;
-    if (i < a.rows && j < a.cols) {
-      const int64_t at = z * a.t_matrix + j * a.ld_t + i;
-      a.t_hi[at] = s_hi[tx][r];
-      a.t_lo[at] = s_lo[tx][r];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int64_t j = j0 + ry + 32 * u;
+    if (j < a.cols && i0 + cx < a.rows) {
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = tile[(cx + e) * kTilePitch + ry + 32 * u];
+      uint4 hi, lo;
+      unzip(w, hi, lo);
+      const int64_t at = z * a.t_matrix + j * a.ld_t + i0 + cx;
+      *reinterpret_cast<uint4*>(a.t_hi + at) = hi;
+      *reinterpret_cast<uint4*>(a.t_lo + at) = lo;
     }
   }
 }
@@ -622,9 +677,9 @@ Layout layout_of(int64_t batch, int64_t rows, int64_t cols, int steps) {
   L.c = std::max(rows, cols);
   L.ld_c = round_up(L.c, 32);
   L.ld_r = round_up(L.r, 32);
-  // About 32 K values for each CTA of the norm, and no more CTAs than give each SM four.
-  const int64_t want = std::min<int64_t>(ceil_div(rows * cols, 32768), ceil_div(4 * kSmCount, batch > 0 ? batch : 1));
-  L.parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, rows), kMaxNormParts));
+  // About 8 K values for each CTA of the norm, and no more CTAs than give each SM four.
+  const int64_t want = std::min<int64_t>(ceil_div(rows * cols, 8192), ceil_div(4 * kSmCount, batch > 0 ? batch : 1));
+  L.parts = (int)std::max<int64_t>(1, want);
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t o = off;
@@ -656,10 +711,19 @@ Split split_at(void* ws, size_t off, int64_t batch, int64_t rows, int64_t cols, 
   return s;
 }
 
+template <int BN, Out OUT>
+int64_t tiles_of(int64_t M, int64_t N) {
+  const int64_t m = ceil_div(M, kTileRows), n = ceil_div(N, BN);
+  if (OUT != Out::kSymmetric) return m * n;
+  int64_t t = 0;
+  for (int64_t i = 0; i < m; ++i) t += std::min<int64_t>((kTileRows / BN) * (i + 1), n);
+  return t;
+}
+
 // D = P Q^T: the launch of one product.
-template <bool PAIR, int BN, Out OUT>
+template <int BN, Out OUT>
 cudaError_t launch_gemm(const Split& p, const Split& q, GemmArgs a, cudaStream_t stream) {
-  using PL = Plan<PAIR, BN, OUT>;
+  using PL = Plan<BN>;
   CUtensorMap m[4];
   if (!make_tmap_f16(&m[0], p.hi, p.cols, p.rows, a.batch, p.ld, p.matrix, BK, 128) ||
       !make_tmap_f16(&m[1], p.lo, p.cols, p.rows, a.batch, p.ld, p.matrix, BK, 128) ||
@@ -668,19 +732,12 @@ cudaError_t launch_gemm(const Split& p, const Split& q, GemmArgs a, cudaStream_t
     return cudaErrorInvalidValue;
   a.M = p.rows;
   a.N = q.rows;
-  a.K = p.cols;
-  a.num_kc = (int)ceil_div(a.K, BK);
-  a.tiles_m = (int)ceil_div(a.M, PL::TM);
+  a.num_kc = (int)ceil_div(p.cols, BK);
+  a.tiles_m = (int)ceil_div(a.M, kTileRows);
   a.tiles_n = (int)ceil_div(a.N, BN);
-  if (OUT == Out::kSymmetric) {
-    a.tiles = 0;
-    for (int tm = 0; tm < a.tiles_m; ++tm)
-      a.tiles += std::min<int64_t>((int64_t)(PL::TM / BN) * (tm + 1), a.tiles_n);
-  } else {
-    a.tiles = (int64_t)a.tiles_m * a.tiles_n;
-  }
+  a.tiles = tiles_of<BN, OUT>(a.M, a.N);
   const int64_t total = a.tiles * a.batch;
-  auto k = ortho_gemm_kernel<PAIR, BN, OUT>;
+  auto k = ortho_gemm_kernel<BN, OUT>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PL::SMEM);
   if (e != cudaSuccess) return e;
   // The register split must fit into what the block is launched with, or it would wait for ever.
@@ -689,23 +746,25 @@ cudaError_t launch_gemm(const Split& p, const Split& q, GemmArgs a, cudaStream_t
     return cudaFuncGetAttributes(&fa, k) == cudaSuccess ? fa.numRegs : 0;
   }();
   if (regs < kRegs) return cudaErrorInvalidConfiguration;
-  const int units = PAIR ? device_sm_count() / 2 : device_sm_count();
-  const unsigned grid = (unsigned)std::min<int64_t>(total, units);
-  if (PAIR) return launch_kernel_cluster(k, dim3(2 * grid), dim3(kThreads), PL::SMEM, 2, stream, m[0], m[1], m[2], m[3], a);
-  return launch_kernel(k, dim3(grid), dim3(kThreads), PL::SMEM, stream, m[0], m[1], m[2], m[3], a);
+  const unsigned grid = (unsigned)std::min<int64_t>(total, device_sm_count() / 2);
+  return launch_kernel_cluster(k, dim3(2 * grid), dim3(kThreads), PL::SMEM, 2, stream, m[0], m[1], m[2], m[3], a);
 }
 
-// Tiles: as large as leaves work for most SMs.
+// The tile width with the least estimated time.  A slice of 64 costs a pair the larger of its 12 MMAs
+// (6 BN cycles) and its operands' way into shared memory (64 bytes a cycle and CTA: 1024, 768 and 640
+// cycles for BN = 256, 128 and 64); a wave of tiles ends with an epilogue that nothing hides.
 template <Out OUT>
 cudaError_t launch_product(const Split& p, const Split& q, const GemmArgs& a, cudaStream_t stream) {
-  const int sms = device_sm_count();
-  auto tiles = [&](int64_t tm, int64_t tn) {
-    const int64_t n = ceil_div(p.rows, tm) * ceil_div(q.rows, tn) * a.batch;
-    return OUT == Out::kSymmetric ? n / 2 : n;
+  const int64_t pairs = device_sm_count() / 2, depth = ceil_div(p.cols, BK);
+  auto cost = [&](int64_t tiles, int64_t slice, int64_t tail) {
+    return ceil_div(tiles * a.batch, pairs) * depth * slice + tail;
   };
-  if (tiles(256, 256) >= sms / 4) return launch_gemm<true, 256, OUT>(p, q, a, stream);
-  if (tiles(128, 128) >= sms / 2) return launch_gemm<false, 128, OUT>(p, q, a, stream);
-  return launch_gemm<false, 64, OUT>(p, q, a, stream);
+  const int64_t c256 = cost(tiles_of<256, OUT>(p.rows, q.rows), 1536, 8000);
+  const int64_t c128 = cost(tiles_of<128, OUT>(p.rows, q.rows), 768, 4000);
+  const int64_t c64 = cost(tiles_of<64, OUT>(p.rows, q.rows), 640, 2000);
+  if (c256 <= c128 && c256 <= c64) return launch_gemm<256, OUT>(p, q, a, stream);
+  if (c128 <= c64) return launch_gemm<128, OUT>(p, q, a, stream);
+  return launch_gemm<64, OUT>(p, q, a, stream);
 }
 
 }  // namespace
@@ -760,9 +819,17 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
     return launch_kernel(split, dim3((unsigned)ceil_div(o.cols, kTile), (unsigned)ceil_div(o.rows, kTile), (unsigned)o.batch),
                          dim3(256), 0, stream, p);
   };
-  cudaError_t e = o.dtype == LM_F32    ? prep(ortho_norm_kernel<float>, ortho_split_kernel<float>)
-                  : o.dtype == LM_BF16 ? prep(ortho_norm_kernel<__nv_bfloat16>, ortho_split_kernel<__nv_bfloat16>)
-                                       : prep(ortho_norm_kernel<__half>, ortho_split_kernel<__half>);
+  const int64_t es = (int64_t)elem_bytes(o.dtype);
+  const bool packs = (o.cols * es) % 16 == 0 && (o.row_stride * es) % 16 == 0 &&
+                     (o.batch == 1 || (o.matrix_stride * es) % 16 == 0) &&
+                     reinterpret_cast<uintptr_t>(o.update) % 16 == 0;
+  auto by_pack = [&](auto t) {
+    using T = decltype(t);
+    constexpr int V = 16 / sizeof(T);
+    return packs ? prep(ortho_norm_kernel<T, V>, ortho_split_kernel<T, V>)
+                 : prep(ortho_norm_kernel<T, 1>, ortho_split_kernel<T, 1>);
+  };
+  cudaError_t e = o.dtype == LM_F32 ? by_pack(float{}) : o.dtype == LM_BF16 ? by_pack(__nv_bfloat16{}) : by_pack(__half{});
   if (e != cudaSuccess) return e;
   note_launches(2);
 
