@@ -26,7 +26,10 @@
 // A run is 256 deep for fp32 results (error 4.8e-6 there, the fp32 library product's is 3.3e-6), 1024
 // for fp16 and 2048 for bf16, whose own rounding is far larger: short runs cost up to 9% of the time.
 //
-// Kernel (persistent): warp 0 loads operand slices by TMA (64 deep, 128-byte swizzle, hi and lo of
+// Kernel: one launch runs the whole iteration (cooperative, one CTA per SM).  A product's tiles are
+// shared out over the CTA pairs; each CTA counts itself in when its part is stored, and the loads of
+// the next product wait until all have.  Against a launch for each product, which the next one's
+// start had to follow, (11 us from one to the next) this takes 8 us for a batch of four of 256 x 256.  Warp 0 loads operand slices by TMA (64 deep, 128-byte swizzle, hi and lo of
 // both operands) into a ring of stages; warp 1 issues 3 x 4 MMAs per stage into one of
 // two TMEM accumulators; warps 4..11 read the other one, apply the epilogue and store.  All
 // on CTA pairs (cta_group::2), tiles of 256 x 256, 128 or 64: a CTA of the pair loads its 128 rows of P
@@ -55,9 +58,7 @@ constexpr int kThreads = 32 * (4 + kEpiWarps);  // a warpgroup for the loads and
 constexpr int kRegs = 168, kRegsLow = 40, kRegsHigh = 232;
 static_assert(kRegsLow + 2 * kRegsHigh <= 3 * kRegs && kThreads == 384, "register split");
 constexpr size_t kSmemMax = 232448;
-// Each epilogue warp turns 16 columns x 32 rows around at a time; the pitch keeps 16-byte reads of
-// eight columns on different banks.
-constexpr int kTurnPitch = 36, kTurnWords = 16 * kTurnPitch;
+constexpr int kTurnWords = 32 * 32;             // an epilogue warp's block in shared memory
 
 // Scale factors of one step of one matrix (see scale_table).
 struct StepScale {
@@ -66,18 +67,18 @@ struct StepScale {
   float product, keep;    // X_next from the accumulator of B X, and from X
 };
 
-enum class Out { kSymmetric, kBoth, kFinal };
+enum { kSymmetric = 0, kBoth = 1, kFinal = 2 };
 
+// One product D = P Q^T of every matrix of the batch.
 struct GemmArgs {
   int64_t M, N;             // D [M, N] per matrix
-  int tiles_m, tiles_n, batch;
-  int64_t tiles;            // of one matrix
-  int num_kc;
-  int run;                  // slices that share a TMEM accumulator
+  int tiles;                // of one matrix
+  int tiles_m, tiles_n;
+  int num_kc;               // slices of the depth
+  int out_kind;             // kSymmetric, kBoth, kFinal
+  int kind;                 // of the scales: 0 gram, 1 square, 2 product
+  int out_dtype;
   // D = alpha * accumulator + beta * (add_hi + add_lo), alpha and beta from the scale table
-  const StepScale* scale;   // of matrix 0
-  int scale_stride;         // StepScales between matrices
-  int kind;                 // 0 gram, 1 square, 2 product
   const __half* add_hi;     // row-major [M, ld_d] (NULL: no addend)
   const __half* add_lo;
   __half* d_hi;             // row-major [M, ld_d]
@@ -87,39 +88,72 @@ struct GemmArgs {
   int64_t ld_d, ld_t, d_matrix, t_matrix;  // strides of rows and of matrices, in elements
   void* out;                // kFinal: out[col * ld_out + row], type out_dtype
   int64_t ld_out, out_matrix;
-  int out_dtype;
+};
+
+// The whole iteration: for each step gram, square and one of the two products (X^T alternates
+// between two buffers), the last step's being `final`.
+enum { kGram = 0, kSquare = 1, kProduct = 2, kLast = 4, kProducts = 5 };
+struct IterArgs {
+  CUtensorMap map[kProducts][4];  // P hi, P lo, Q hi, Q lo
+  GemmArgs gemm[kProducts];
+  const StepScale* scale;         // [batch][steps]
+  unsigned* arrived;              // CTAs that have finished a product, counted over all products
   int* status;
   unsigned long long timeout_ns;
+  int steps, batch;
+  int run;                        // slices that share a TMEM accumulator
   int debug_skip_first_load;
 };
+static_assert(sizeof(IterArgs) <= 4096, "kernel parameters");
+
+__device__ __forceinline__ int product_index(int p, int steps) {
+  const int step = p / 3, w = p - 3 * step;
+  if (w < 2) return w;
+  return step + 1 == steps ? kLast : kProduct + (step & 1);
+}
+
+// Wait (bounded) until `want` CTAs have arrived; what they wrote before is visible after it.
+// `pause`: between polls, where nothing hangs on the first moment.
+template <bool pause>
+__device__ __forceinline__ bool wait_arrived(const unsigned* arrived, unsigned want, int* status,
+                                             unsigned long long timeout_ns) {
+  const unsigned long long t0 = ptx::globaltimer();
+  while (true) {
+    unsigned v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(arrived) : "memory");
+    if (v >= want) return true;
+    if (pause) __nanosleep(64);
+    if (ptx::globaltimer() - t0 > timeout_ns) {
+      atomicExch(status, 7);
+      return false;
+    }
+  }
+}
 
 // Tile t of a matrix.  Symmetric products: only tiles with a row >= their first column, so
 // `per` more column tiles for each further row tile.
-template <int BN, bool SYM>
-__device__ __forceinline__ void tile_of(int64_t t, const GemmArgs& a, int& tm, int& tn) {
-  if (!SYM) {
+template <int BN>
+__device__ __forceinline__ void tile_of(int t, int out_kind, int tiles_m, int tiles_n, int& tm, int& tn) {
+  if (out_kind != kSymmetric) {
     // Bands of 8 row tiles, so that the tiles in flight share both operands in L2.
-    const int band = 8;
-    const int64_t per_band = (int64_t)band * a.tiles_n;
-    const int64_t bi = t / per_band;
-    const int64_t in = t - bi * per_band;
-    const int left = a.tiles_m - (int)bi * band;
-    const int rows = left < band ? left : band;
-    tm = (int)bi * band + (int)(in % rows);
-    tn = (int)(in / rows);
+    constexpr int band = 8;
+    const int bi = t / (band * tiles_n);
+    const int in = t - bi * band * tiles_n;
+    const int rows = min(tiles_m - bi * band, band);
+    tn = in / rows;
+    tm = bi * band + in - tn * rows;
     return;
   }
   constexpr int per = kTileRows / BN;
-  int row = 0;
-  int64_t left = t;
+  int row = 0, left = t;
   while (true) {
-    const int64_t n = min((int64_t)per * (row + 1), (int64_t)a.tiles_n);
+    const int n = min(per * (row + 1), tiles_n);
     if (left < n) break;
     left -= n;
     ++row;
   }
   tm = row;
-  tn = (int)left;
+  tn = left;
 }
 
 // Eight (hi, lo) pairs as eight hi and eight lo.
@@ -148,14 +182,9 @@ struct Plan {
   static_assert(STAGES >= 2 && SMEM <= kSmemMax, "stages");
 };
 
-template <int BN, Out OUT>
-__global__ void __launch_bounds__(kThreads, 1)
-    ortho_gemm_kernel(const __grid_constant__ CUtensorMap tm_phi,
-                      const __grid_constant__ CUtensorMap tm_plo,
-                      const __grid_constant__ CUtensorMap tm_qhi,
-                      const __grid_constant__ CUtensorMap tm_qlo, const GemmArgs a) {
+template <int BN>
+__global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constant__ IterArgs it) {
   using P = Plan<BN>;
-  constexpr bool SYM = OUT == Out::kSymmetric;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -165,6 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* acc_empty = acc_full + 2;                                         // [2] epilogue -> MMA
   uint64_t* drain = acc_empty + 2;                                            // MMA teardown
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  unsigned* stored = tmem_slot + 1;                                           // epilogue warps, over all products
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -180,14 +210,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(&acc_empty[b], 2 * kEpiWarps);
     }
     ptx::mbar_init(drain, 1);
+    *stored = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == 0 && lane == 0) {
-    ptx::prefetch_tensormap(&tm_phi);
-    ptx::prefetch_tensormap(&tm_plo);
-    ptx::prefetch_tensormap(&tm_qhi);
-    ptx::prefetch_tensormap(&tm_qlo);
-  }
+  if (warp == 0 && lane < 4)
+    for (int p = 0; p < kProducts; ++p) ptx::prefetch_tensormap(&it.map[p][lane]);
   ptx::cluster_sync();  // the peer's barriers exist before any remote arrive
   if (warp == 1) {
     ptx::tmem_alloc_pair(tmem_slot, P::TCOLS);
@@ -197,10 +224,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  ptx::griddep_wait();  // the operands come from the previous kernel
-  const int64_t total = a.tiles * a.batch;
-  const int64_t unit = blockIdx.x >> 1;
-  const int64_t units = gridDim.x >> 1;
+  const int unit = blockIdx.x >> 1;
+  const int units = gridDim.x >> 1;
+  const int products = 3 * it.steps;
 
   if (warp < 4) {
     ptx::regs_shrink<kRegsLow>();
@@ -210,32 +236,45 @@ __global__ void __launch_bounds__(kThreads, 1)
         int stage = 0;
         uint32_t phase = 0, issued = 0, last = 0;
         bool ok = true, skipped = false;
-        for (int64_t t = unit; t < total && ok; t += units) {
-          const int z = (int)(t / a.tiles);
-          int tm, tn;
-          tile_of<BN, SYM>(t - z * a.tiles, a, tm, tn);
-          const int i0 = tm * kTileRows + (int)rank * 128;
-          const int j0 = tn * BN + (int)rank * P::BROWS;
-          for (int kc = 0; kc < a.num_kc; ++kc) {
-            if (!ptx::mbar_wait_bounded(&empty[stage], phase ^ 1, a.status, a.timeout_ns)) { ok = false; break; }
-            if (a.debug_skip_first_load && !skipped && blockIdx.x == 0) {
-              skipped = true;  // test hook: this stage never fills, so its consumer times out
-            } else {
-              uint8_t* s = smem + stage * P::STAGE;
-              if (leader) ptx::mbar_arrive_expect_tx(&full[stage], 2 * P::STAGE);
-              const uint32_t fc = ptx::map_to_rank(&full[stage], 0);
-              ptx::tma_load_3d_pair(s, &tm_phi, kc * BK, i0, z, fc);
-              ptx::tma_load_3d_pair(s + P::A_BYTES, &tm_plo, kc * BK, i0, z, fc);
-              ptx::tma_load_3d_pair(s + 2 * P::A_BYTES, &tm_qhi, kc * BK, j0, z, fc);
-              ptx::tma_load_3d_pair(s + 2 * P::A_BYTES + P::B_BYTES, &tm_qlo, kc * BK, j0, z, fc);
-              if (leader) {
-                issued |= 1u << stage;
-                last = (last & ~(1u << stage)) | (phase << stage);
-              }
+        for (int p = 0; p < products && ok; ++p) {
+          const int pi = product_index(p, it.steps);
+          const CUtensorMap* map = it.map[pi];
+          const int tiles = it.gemm[pi].tiles, num_kc = it.gemm[pi].num_kc, out_kind = it.gemm[pi].out_kind;
+          const int tiles_m = it.gemm[pi].tiles_m, tiles_n = it.gemm[pi].tiles_n;
+          const int total = tiles * it.batch;
+          for (int t = unit; t < total && ok; t += units) {
+            const int z = t / tiles;
+            int tm, tn;
+            tile_of<BN>(t - z * tiles, out_kind, tiles_m, tiles_n, tm, tn);
+            const int i0 = tm * kTileRows + (int)rank * 128;
+            const int j0 = tn * BN + (int)rank * P::BROWS;
+            if (t == unit && p > 0) {
+              // The operands come from the other CTAs' epilogues: plain stores, read here by TMA.
+              ok = wait_arrived<false>(it.arrived, (unsigned)p * gridDim.x, it.status, it.timeout_ns);
+              if (!ok) break;
             }
-            if (++stage == P::STAGES) {
-              stage = 0;
-              phase ^= 1;
+            if (t == unit) ptx::fence_proxy_async();
+            for (int kc = 0; kc < num_kc; ++kc) {
+              if (!ptx::mbar_wait_bounded(&empty[stage], phase ^ 1, it.status, it.timeout_ns)) { ok = false; break; }
+              if (it.debug_skip_first_load && !skipped && blockIdx.x == 0) {
+                skipped = true;  // test hook: this stage never fills, so its consumer times out
+              } else {
+                uint8_t* s = smem + stage * P::STAGE;
+                if (leader) ptx::mbar_arrive_expect_tx(&full[stage], 2 * P::STAGE);
+                const uint32_t fc = ptx::map_to_rank(&full[stage], 0);
+                ptx::tma_load_3d_pair(s, map, kc * BK, i0, z, fc);
+                ptx::tma_load_3d_pair(s + P::A_BYTES, map + 1, kc * BK, i0, z, fc);
+                ptx::tma_load_3d_pair(s + 2 * P::A_BYTES, map + 2, kc * BK, j0, z, fc);
+                ptx::tma_load_3d_pair(s + 2 * P::A_BYTES + P::B_BYTES, map + 3, kc * BK, j0, z, fc);
+                if (leader) {
+                  issued |= 1u << stage;
+                  last = (last & ~(1u << stage)) | (phase << stage);
+                }
+              }
+              if (++stage == P::STAGES) {
+                stage = 0;
+                phase ^= 1;
+              }
             }
           }
         }
@@ -243,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // both CTAs' bytes, and the final cluster barrier holds the peer until then).
         if (!ok)
           for (int s = 0; s < P::STAGES; ++s)
-            if (issued >> s & 1u) ptx::mbar_wait_bounded(&full[s], (last >> s) & 1u, a.status, a.timeout_ns);
+            if (issued >> s & 1u) ptx::mbar_wait_bounded(&full[s], (last >> s) & 1u, it.status, it.timeout_ns);
       }
     } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issuer (the whole warp)
@@ -254,47 +293,51 @@ __global__ void __launch_bounds__(kThreads, 1)
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
-        // A unit of work is one run of a.run stages of a tile: each has an accumulator of its own.
-        const int runs = (a.num_kc + a.run - 1) / a.run;
-        for (int64_t t = unit; t < total && ok; t += units) {
-          for (int run = 0; run < runs && ok; ++run) {
-            if (!ptx::mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1, a.status, a.timeout_ns)) { ok = false; break; }
-            ptx::tc_fence_after();
-            const uint32_t d = tmem + (uint32_t)(acc * BN);
-            const int depth = min(a.run, a.num_kc - run * a.run);
-            for (int kc = 0; kc < depth; ++kc) {
-              if (!ptx::mbar_wait_bounded(&full[stage], phase, a.status, a.timeout_ns)) { ok = false; break; }
+        for (int p = 0; p < products && ok; ++p) {
+          const int pi = product_index(p, it.steps);
+          const int num_kc = it.gemm[pi].num_kc, total = it.gemm[pi].tiles * it.batch;
+          // A unit of work is one run of it.run stages of a tile: each has an accumulator of its own.
+          const int runs = (num_kc + it.run - 1) / it.run;
+          for (int t = unit; t < total && ok; t += units) {
+            for (int run = 0; run < runs && ok; ++run) {
+              if (!ptx::mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1, it.status, it.timeout_ns)) { ok = false; break; }
               ptx::tc_fence_after();
-              // Descriptors of the stage's four operands: the address field counts 16 bytes.
-              const uint64_t phi = base + (uint32_t)stage * (P::STAGE >> 4);
-              const uint64_t plo = phi + (P::A_BYTES >> 4);
-              const uint64_t qhi = phi + (2 * P::A_BYTES >> 4);
-              const uint64_t qlo = phi + ((2 * P::A_BYTES + P::B_BYTES) >> 4);
+              const uint32_t d = tmem + (uint32_t)(acc * BN);
+              const int depth = min(it.run, num_kc - run * it.run);
+              for (int kc = 0; kc < depth; ++kc) {
+                if (!ptx::mbar_wait_bounded(&full[stage], phase, it.status, it.timeout_ns)) { ok = false; break; }
+                ptx::tc_fence_after();
+                // Descriptors of the stage's four operands: the address field counts 16 bytes.
+                const uint64_t phi = base + (uint32_t)stage * (P::STAGE >> 4);
+                const uint64_t plo = phi + (P::A_BYTES >> 4);
+                const uint64_t qhi = phi + (2 * P::A_BYTES >> 4);
+                const uint64_t qlo = phi + ((2 * P::A_BYTES + P::B_BYTES) >> 4);
 #pragma unroll
-              for (int k = 0; k < BK / 16; ++k) {  // 16 fp16 are 32 bytes along the swizzled row
-                ptx::mma_f16_ss_pair(d, phi + 2 * k, qhi + 2 * k, idesc, (kc | k) != 0, elected);
-                ptx::mma_f16_ss_pair(d, phi + 2 * k, qlo + 2 * k, idesc, 1, elected);
-                ptx::mma_f16_ss_pair(d, plo + 2 * k, qhi + 2 * k, idesc, 1, elected);
+                for (int k = 0; k < BK / 16; ++k) {  // 16 fp16 are 32 bytes along the swizzled row
+                  ptx::mma_f16_ss_pair(d, phi + 2 * k, qhi + 2 * k, idesc, (kc | k) != 0, elected);
+                  ptx::mma_f16_ss_pair(d, phi + 2 * k, qlo + 2 * k, idesc, 1, elected);
+                  ptx::mma_f16_ss_pair(d, plo + 2 * k, qhi + 2 * k, idesc, 1, elected);
+                }
+                if (elected) ptx::mma_commit_pair(&empty[stage]);
+                __syncwarp();
+                if (++stage == P::STAGES) {
+                  stage = 0;
+                  phase ^= 1;
+                }
               }
-              if (elected) ptx::mma_commit_pair(&empty[stage]);
+              if (!ok) break;
+              if (elected) ptx::mma_commit_pair(&acc_full[acc]);
               __syncwarp();
-              if (++stage == P::STAGES) {
-                stage = 0;
-                phase ^= 1;
+              if (++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1;
               }
-            }
-            if (!ok) break;
-            if (elected) ptx::mma_commit_pair(&acc_full[acc]);
-            __syncwarp();
-            if (++acc == 2) {
-              acc = 0;
-              acc_phase ^= 1;
             }
           }
         }
         if (elected) ptx::mma_commit_pair(drain);  // every MMA issued so far finishes before TMEM is freed
         __syncwarp();
-        ptx::mbar_wait_bounded(drain, 0, a.status, a.timeout_ns);
+        ptx::mbar_wait_bounded(drain, 0, it.status, it.timeout_ns);
       }
     }
   } else {
@@ -305,135 +348,196 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t* turn = reinterpret_cast<uint32_t*>(smem + P::STAGES * P::STAGE + 256) + (warp - 4) * kTurnWords;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int64_t t = unit; t < total; t += units) {
-      const int z = (int)(t / a.tiles);
-      int tm, tn;
-      tile_of<BN, SYM>(t - z * a.tiles, a, tm, tn);
-      const int64_t i0 = (int64_t)tm * kTileRows + rank * 128 + q * 32;
-      const int64_t i = i0 + lane;
-      const StepScale sc = a.scale[(int64_t)z * a.scale_stride];
-      const float alpha = a.kind == 0 ? sc.gram : a.kind == 1 ? sc.square : sc.product;
-      const float beta = a.kind == 0 ? 0.f : a.kind == 1 ? sc.linear : sc.keep;
-      // All runs but the last are added up in registers; the last one's accumulator takes the total,
-      // so that the stores below go over it 32 columns at a time.
-      const int runs = (a.num_kc + a.run - 1) / a.run;
-      const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * (BN / 2));
-      float sum[BN / 2];
-      bool ok = true;
-      for (int run = 0; run < runs; ++run) {
-        if (!ptx::mbar_wait_bounded(&acc_full[acc], acc_phase, a.status, a.timeout_ns)) { ok = false; break; }
-        ptx::tc_fence_after();
-        if (runs == 1) break;
+    bool ok = true;
+    for (int p = 0; p < products && ok; ++p) {
+      const GemmArgs a = it.gemm[product_index(p, it.steps)];  // in registers: its index is not constant
+      const int total = a.tiles * it.batch;
+      const int runs = (a.num_kc + it.run - 1) / it.run;
+      const bool sym = a.out_kind == kSymmetric;
+      // The addend too comes from other CTAs, and a CTA counts itself in for this product only once
+      // the last one is complete.
+      if (p > 0) {
+        int in = 1;
+        if (lane == 0) in = wait_arrived<true>(it.arrived, (unsigned)p * gridDim.x, it.status, it.timeout_ns);
+        ok = __shfl_sync(0xffffffffu, in, 0) != 0;
+        if (!ok) break;
+      }
+      for (int t = unit; t < total; t += units) {
+        const int z = t / a.tiles;
+        int tm, tn;
+        tile_of<BN>(t - z * a.tiles, a.out_kind, a.tiles_m, a.tiles_n, tm, tn);
+        const int64_t i0 = (int64_t)tm * kTileRows + rank * 128 + q * 32;
+        const int64_t i = i0 + lane;
+        const StepScale sc = it.scale[(int64_t)z * it.steps + p / 3];
+        const float alpha = a.kind == 0 ? sc.gram : a.kind == 1 ? sc.square : sc.product;
+        const float beta = a.kind == 0 ? 0.f : a.kind == 1 ? sc.linear : sc.keep;
+        const int64_t col0 = (int64_t)tn * BN + h * (BN / 2);
+        const int sub = lane >> 2, part = (lane & 3) * 8;
+        // The addend of a block of 32 x 32, four lanes a row; a block's is fetched while the one before
+        // it is worked on, the first one's while the accumulator fills.  (Row pitches are multiples of
+        // 32, so a block's columns lie inside their row.)
+        uint4 add_hi[4], add_lo[4];
+        auto fetch = [&](int g) {
+          const int64_t j = col0 + g * 32;
+          if (a.add_hi == nullptr || j >= a.N || (sym && j > i0)) return;
+          const int64_t at = z * a.d_matrix + (i0 + sub) * a.ld_d + j + part;
 #pragma unroll
-        for (int c = 0; c < BN / 64; ++c) {
-          uint32_t v[32];
-          const uint32_t at = lanes + (uint32_t)(acc * BN + c * 32);
-          ptx::tmem_ld32(at, v);
-          ptx::tmem_wait_ld();
+          for (int k = 0; k < 4; ++k)
+            if (i0 + sub + 8 * k < a.M) {
+              add_hi[k] = *reinterpret_cast<const uint4*>(a.add_hi + at + 8 * k * a.ld_d);
+              add_lo[k] = *reinterpret_cast<const uint4*>(a.add_lo + at + 8 * k * a.ld_d);
+            }
+        };
+        if (runs == 1) fetch(0);
+        // All runs but the last are added up in registers; the last one's accumulator takes the
+        // total, so that the stores below go over it a few columns at a time.
+        const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * (BN / 2));
+        float sum[BN / 2];
+        for (int run = 0; run < runs; ++run) {
+          if (!ptx::mbar_wait_bounded(&acc_full[acc], acc_phase, it.status, it.timeout_ns)) { ok = false; break; }
+          ptx::tc_fence_after();
+          if (runs == 1) break;
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            sum[c * 32 + e] = run == 0 ? __uint_as_float(v[e]) : sum[c * 32 + e] + __uint_as_float(v[e]);
+          for (int c = 0; c < BN / 64; ++c) {
+            uint32_t v[32];
+            const uint32_t at = lanes + (uint32_t)(acc * BN + c * 32);
+            ptx::tmem_ld32(at, v);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              sum[c * 32 + e] = run == 0 ? __uint_as_float(v[e]) : sum[c * 32 + e] + __uint_as_float(v[e]);
+            if (run + 1 == runs) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(sum[c * 32 + e]);
+              ptx::tmem_st32(at, v);
+            }
+          }
           if (run + 1 == runs) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(sum[c * 32 + e]);
-            ptx::tmem_st32(at, v);
+            ptx::tmem_wait_st();
+            break;
+          }
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(&acc_empty[acc], 0));
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1;
           }
         }
-        if (run + 1 == runs) {
-          ptx::tmem_wait_st();
-          break;
+        if (!ok) break;
+        if (runs > 1) fetch(0);  // (not next to the partial sums: registers)
+        // Blocks of 32 x 32, in a loop that is not unrolled: instructions that run for the first time
+        // in a launch are fetched from L2, and took most of a small product's time when this was
+        // straight-line.  A block goes through shared memory, so that four lanes read or write 64
+        // bytes of a row: with a row a lane every access touched 32 lines.
+#pragma unroll 1
+        for (int g = 0; g < BN / 64; ++g) {
+          const int64_t j0 = col0 + g * 32;
+          // Below the diagonal, on it, or above it: the same for the whole warp, like the bounds.
+          const bool inside = j0 < a.N && i0 < a.M && !(sym && j0 > i0);
+          const int64_t d_at = z * a.d_matrix + (i0 + sub) * a.ld_d + j0 + part;
+          uint32_t v[32];
+          __syncwarp();  // the TMEM load is a whole warp's; the last block's reads of `turn` are done
+          ptx::tmem_ld32(lanes + (uint32_t)(acc * BN + g * 32), v);
+          ptx::tmem_wait_ld();
+          if (g == BN / 64 - 1) {  // the accumulator goes back before the last stores
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(&acc_empty[acc], 0));
+          }
+          if (!inside) continue;
+          // Word (row, column) of the block is at row * 32 + (column ^ row): rows, columns and the
+          // runs of eight below are all read and written without bank conflicts.
+#pragma unroll
+          for (int e = 0; e < 32; ++e) turn[lane * 32 + (e ^ lane)] = v[e];
+          __syncwarp();
+          const bool both = !sym || j0 < i0;  // a block on the diagonal is computed whole
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int r = sub + 8 * k;
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = alpha * __uint_as_float(turn[r * 32 + ((part + e) ^ r)]);
+            if (a.add_hi != nullptr) {
+              const __half2* hi = reinterpret_cast<const __half2*>(&add_hi[k]);
+              const __half2* lo = reinterpret_cast<const __half2*>(&add_lo[k]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 x = __half22float2(hi[e]), y = __half22float2(lo[e]);
+                f[2 * e] = fmaf(beta, x.x + y.x, f[2 * e]);
+                f[2 * e + 1] = fmaf(beta, x.y + y.y, f[2 * e + 1]);
+              }
+            }
+            uint32_t w[8];  // fp32, or hi in the low half and lo in the high half
+            if (a.out_kind == kFinal) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(f[e]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                __half hi, lo;
+                split_f16(f[e], hi, lo);
+                w[e] = (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
+              }
+              if (i0 + r < a.M) {
+                uint4 hi, lo;
+                unzip(w, hi, lo);
+                *reinterpret_cast<uint4*>(a.d_hi + d_at + 8 * k * a.ld_d) = hi;
+                *reinterpret_cast<uint4*>(a.d_lo + d_at + 8 * k * a.ld_d) = lo;
+              }
+            }
+            if (both) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) turn[r * 32 + ((part + e) ^ r)] = w[e];
+            }
+          }
+          if (g + 1 < BN / 64) fetch(g + 1);
+          if (!both) continue;
+          __syncwarp();
+          if (a.out_kind == kFinal) {
+            if (i < a.M) {
+              for (int e = 0; e < 32 && j0 + e < a.N; ++e)
+                store_as(a.out, z * a.out_matrix + (j0 + e) * a.ld_out + i, a.out_dtype, __uint_as_float(turn[lane * 32 + (e ^ lane)]));
+            }
+            continue;
+          }
+          // The other order: four lanes write a column's 32 rows.
+          __half* th = sym ? a.d_hi : a.t_hi;
+          __half* tl = sym ? a.d_lo : a.t_lo;
+          const int64_t ld = sym ? a.ld_d : a.ld_t;
+          const int64_t t_at = z * (sym ? a.d_matrix : a.t_matrix) + (j0 + sub) * ld + i0 + part;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int col = sub + 8 * k;
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = turn[(part + e) * 32 + (col ^ (part + e))];
+            if (j0 + col < a.N) {
+              uint4 hi, lo;
+              unzip(w, hi, lo);
+              *reinterpret_cast<uint4*>(th + t_at + 8 * k * ld) = hi;
+              *reinterpret_cast<uint4*>(tl + t_at + 8 * k * ld) = lo;
+            }
+          }
         }
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(&acc_empty[acc], 0));
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1;
         }
       }
       if (!ok) break;
-      // Eight columns at a time, in a loop that is not unrolled: instructions that run once in a launch
-      // are fetched from L2, and took most of a small product's time when this was straight-line.
-#pragma unroll 1
-      for (int g = 0; g < BN / 16; ++g) {
-        const int64_t j0 = (int64_t)tn * BN + h * (BN / 2) + g * 8;
-        uint32_t v[8];
-        __syncwarp();  // the TMEM load is a whole warp's
-        ptx::tmem_ld8(lanes + (uint32_t)(acc * BN + g * 8), v);
-        ptx::tmem_wait_ld();
-        if (g == BN / 16 - 1) {  // the accumulator goes back before the last stores
-          ptx::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(&acc_empty[acc], 0));
+      // This warp's part of the product is in memory, and the CTA's once all warps have said so (a
+      // count, not a barrier: a warp that gives up on a wait leaves the others to give up on theirs).
+      __syncwarp();
+      if (lane == 0) {
+        __threadfence_block();
+        if (atomicAdd(stored, 1u) == (unsigned)(p + 1) * kEpiWarps - 1) {
+          __threadfence();
+          asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(it.arrived) : "memory");
         }
-        // Blocks of 32 x 32, one row a lane: below the diagonal, on it, or above it.  These tests come
-        // out the same for the whole warp.
-        const int64_t block = j0 & ~(int64_t)31;
-        if (j0 >= a.N || i0 >= a.M || (SYM && block > i0)) continue;
-        float f[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = alpha * __uint_as_float(v[e]);
-        if (a.add_hi != nullptr && i < a.M) {
-          // Row pitches are multiples of 32, so eight columns lie inside their row.
-          const int64_t at = z * a.d_matrix + i * a.ld_d + j0;
-          const Pack<__half, 8> hi = *reinterpret_cast<const Pack<__half, 8>*>(a.add_hi + at);
-          const Pack<__half, 8> lo = *reinterpret_cast<const Pack<__half, 8>*>(a.add_lo + at);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = fmaf(beta, __half2float(hi.v[e]) + __half2float(lo.v[e]), f[e]);
-        }
-        if constexpr (OUT == Out::kFinal) {
-          if (i < a.M) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (j0 + e < a.N) store_as(a.out, z * a.out_matrix + (j0 + e) * a.ld_out + i, a.out_dtype, f[e]);
-          }
-        } else {
-          uint32_t both[8];  // hi in the low half, lo in the high half
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            __half hi, lo;
-            split_f16(f[e], hi, lo);
-            both[e] = (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
-          }
-          uint4 hi, lo;
-          if (i < a.M) {
-            unzip(both, hi, lo);
-            const int64_t at = z * a.d_matrix + i * a.ld_d + j0;
-            *reinterpret_cast<uint4*>(a.d_hi + at) = hi;
-            *reinterpret_cast<uint4*>(a.d_lo + at) = lo;
-          }
-          if (SYM && block == i0) continue;  // a block on the diagonal is computed whole
-          // The other order, turned around in shared memory 16 columns at a time: lane l then holds
-          // half of column l % 16.
-#pragma unroll
-          for (int e = 0; e < 8; ++e) turn[((g & 1) * 8 + e) * kTurnPitch + lane] = both[e];
-          if ((g & 1) == 0 && j0 + 8 < a.N) continue;
-          __syncwarp();
-          const int col = lane & 15, part = lane >> 4;
-          const int64_t j = (j0 & ~(int64_t)15) + col;
-          __half* th = (SYM ? a.d_hi : a.t_hi) + z * (SYM ? a.d_matrix : a.t_matrix);
-          __half* tl = (SYM ? a.d_lo : a.t_lo) + z * (SYM ? a.d_matrix : a.t_matrix);
-          const int64_t at = j * (SYM ? a.ld_d : a.ld_t) + i0 + part * 16;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            uint32_t w[8];
-            *reinterpret_cast<uint4*>(&w[0]) = *reinterpret_cast<const uint4*>(&turn[col * kTurnPitch + part * 16 + 8 * k]);
-            *reinterpret_cast<uint4*>(&w[4]) = *reinterpret_cast<const uint4*>(&turn[col * kTurnPitch + part * 16 + 8 * k + 4]);
-            unzip(w, hi, lo);
-            if (j < a.N) {
-              *reinterpret_cast<uint4*>(th + at + 8 * k) = hi;
-              *reinterpret_cast<uint4*>(tl + at + 8 * k) = lo;
-            }
-          }
-        }
-      }
-      if (++acc == 2) {
-        acc = 0;
-        acc_phase ^= 1;
       }
     }
   }
-  ptx::griddep_launch_dependents();
   ptx::tc_fence_before();
   __syncthreads();
   ptx::cluster_sync();  // neither CTA leaves before both are done with each other's memory
@@ -461,7 +565,7 @@ struct PrepArgs {
   __half* t_hi;            // the other order: [cols, ld_t]
   __half* t_lo;
   int64_t ld_g, ld_t, g_matrix, t_matrix;
-  int* status;
+  int* status;             // [0] status word, [1] arrivals of the products' CTAs
 };
 
 // Sums of squares in 64 bits: an update of any magnitude has a norm.  A warp takes pieces of
@@ -475,7 +579,10 @@ __global__ void __launch_bounds__(kNormThreads) ortho_norm_kernel(const PrepArgs
   ptx::griddep_launch_dependents();
   const int64_t z = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (z == 0 && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
+  if (z == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
+    a.status[0] = 0;
+    a.status[1] = 0;  // the arrival counter
+  }
   constexpr int piece = 32 * kNormPiece * VEC;
   const int64_t per_row = (a.cols + piece - 1) / piece, items = per_row * a.rows;
   const int64_t warps = (int64_t)a.parts * (kNormThreads / 32);
@@ -693,7 +800,7 @@ Layout layout_of(int64_t batch, int64_t rows, int64_t cols, int steps) {
   const size_t sq = sizeof(__half) * 2 * batch * L.r * L.ld_r;
   L.x = take(x);
   L.xt0 = take(xt);
-  L.xt1 = take(steps > 1 ? xt : 0);
+  L.xt1 = take(xt);
   L.a = take(sq);
   L.b = take(sq);
   L.end = off;
@@ -711,33 +818,24 @@ Split split_at(void* ws, size_t off, int64_t batch, int64_t rows, int64_t cols, 
   return s;
 }
 
-template <int BN, Out OUT>
-int64_t tiles_of(int64_t M, int64_t N) {
-  const int64_t m = ceil_div(M, kTileRows), n = ceil_div(N, BN);
-  if (OUT != Out::kSymmetric) return m * n;
+int64_t tiles_of(int64_t M, int64_t N, int bn, int out_kind) {
+  const int64_t m = ceil_div(M, kTileRows), n = ceil_div(N, bn);
+  if (out_kind != kSymmetric) return m * n;
   int64_t t = 0;
-  for (int64_t i = 0; i < m; ++i) t += std::min<int64_t>((kTileRows / BN) * (i + 1), n);
+  for (int64_t i = 0; i < m; ++i) t += std::min<int64_t>((kTileRows / bn) * (i + 1), n);
   return t;
 }
 
-// D = P Q^T: the launch of one product.
-template <int BN, Out OUT>
-cudaError_t launch_gemm(const Split& p, const Split& q, GemmArgs a, cudaStream_t stream) {
+// One product D = P Q^T of the iteration, apart from where D goes.
+struct Operands {
+  const Split* p;
+  const Split* q;
+};
+
+template <int BN>
+cudaError_t launch_iteration(IterArgs& it, const Operands* op, cudaStream_t stream) {
   using PL = Plan<BN>;
-  CUtensorMap m[4];
-  if (!make_tmap_f16(&m[0], p.hi, p.cols, p.rows, a.batch, p.ld, p.matrix, BK, 128) ||
-      !make_tmap_f16(&m[1], p.lo, p.cols, p.rows, a.batch, p.ld, p.matrix, BK, 128) ||
-      !make_tmap_f16(&m[2], q.hi, q.cols, q.rows, a.batch, q.ld, q.matrix, BK, PL::BROWS) ||
-      !make_tmap_f16(&m[3], q.lo, q.cols, q.rows, a.batch, q.ld, q.matrix, BK, PL::BROWS))
-    return cudaErrorInvalidValue;
-  a.M = p.rows;
-  a.N = q.rows;
-  a.num_kc = (int)ceil_div(p.cols, BK);
-  a.tiles_m = (int)ceil_div(a.M, kTileRows);
-  a.tiles_n = (int)ceil_div(a.N, BN);
-  a.tiles = tiles_of<BN, OUT>(a.M, a.N);
-  const int64_t total = a.tiles * a.batch;
-  auto k = ortho_gemm_kernel<BN, OUT>;
+  auto k = ortho_kernel<BN>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PL::SMEM);
   if (e != cudaSuccess) return e;
   // The register split must fit into what the block is launched with, or it would wait for ever.
@@ -746,25 +844,73 @@ cudaError_t launch_gemm(const Split& p, const Split& q, GemmArgs a, cudaStream_t
     return cudaFuncGetAttributes(&fa, k) == cudaSuccess ? fa.numRegs : 0;
   }();
   if (regs < kRegs) return cudaErrorInvalidConfiguration;
-  const unsigned grid = (unsigned)std::min<int64_t>(total, device_sm_count() / 2);
-  return launch_kernel_cluster(k, dim3(2 * grid), dim3(kThreads), PL::SMEM, 2, stream, m[0], m[1], m[2], m[3], a);
+  int64_t most = 0;
+  for (int p = 0; p < kProducts; ++p) {
+    GemmArgs& a = it.gemm[p];
+    const Split &l = *op[p].p, &r = *op[p].q;
+    if (!make_tmap_f16(&it.map[p][0], l.hi, l.cols, l.rows, it.batch, l.ld, l.matrix, BK, 128) ||
+        !make_tmap_f16(&it.map[p][1], l.lo, l.cols, l.rows, it.batch, l.ld, l.matrix, BK, 128) ||
+        !make_tmap_f16(&it.map[p][2], r.hi, r.cols, r.rows, it.batch, r.ld, r.matrix, BK, PL::BROWS) ||
+        !make_tmap_f16(&it.map[p][3], r.lo, r.cols, r.rows, it.batch, r.ld, r.matrix, BK, PL::BROWS))
+      return cudaErrorInvalidValue;
+    a.M = l.rows;
+    a.N = r.rows;
+    a.num_kc = (int)ceil_div(l.cols, BK);
+    a.tiles_m = (int)ceil_div(a.M, kTileRows);
+    a.tiles_n = (int)ceil_div(a.N, BN);
+    const int64_t tiles = tiles_of(a.M, a.N, BN, a.out_kind);
+    if (tiles * it.batch >= (int64_t(1) << 30)) return cudaErrorInvalidConfiguration;
+    a.tiles = (int)tiles;
+    most = std::max(most, tiles * it.batch);
+  }
+  // A cooperative launch: the CTAs wait for one another between products, so all must be resident.
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = PL::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeCooperative;
+  attr[1].val.cooperative = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)device_sm_count());
+  static int resident[64];  // clusters, by device
+  int dev = 0;
+  if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+  int clusters = dev < 64 ? resident[dev] : 0;
+  if (clusters == 0) {
+    if ((e = cudaOccupancyMaxActiveClusters(&clusters, k, &cfg)) != cudaSuccess) return e;
+    if (clusters < 1) return cudaErrorCooperativeLaunchTooLarge;
+    if (dev < 64) resident[dev] = clusters;
+  }
+  cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(most, clusters));
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, k, it);
 }
 
 // The tile width with the least estimated time.  A slice of 64 costs a pair the larger of its 12 MMAs
 // (6 BN cycles) and its operands' way into shared memory (64 bytes a cycle and CTA: 1024, 768 and 640
-// cycles for BN = 256, 128 and 64); a wave of tiles ends with an epilogue that nothing hides.
-template <Out OUT>
-cudaError_t launch_product(const Split& p, const Split& q, const GemmArgs& a, cudaStream_t stream) {
-  const int64_t pairs = device_sm_count() / 2, depth = ceil_div(p.cols, BK);
-  auto cost = [&](int64_t tiles, int64_t slice, int64_t tail) {
-    return ceil_div(tiles * a.batch, pairs) * depth * slice + tail;
-  };
-  const int64_t c256 = cost(tiles_of<256, OUT>(p.rows, q.rows), 1536, 8000);
-  const int64_t c128 = cost(tiles_of<128, OUT>(p.rows, q.rows), 768, 4000);
-  const int64_t c64 = cost(tiles_of<64, OUT>(p.rows, q.rows), 640, 2000);
-  if (c256 <= c128 && c256 <= c64) return launch_gemm<256, OUT>(p, q, a, stream);
-  if (c128 <= c64) return launch_gemm<128, OUT>(p, q, a, stream);
-  return launch_gemm<64, OUT>(p, q, a, stream);
+// cycles for BN = 256, 128 and 64); a product ends with an epilogue that nothing hides.
+int tile_width(const IterArgs& it, const Operands* op) {
+  const int64_t pairs = device_sm_count() / 2;
+  int best = 0;
+  int64_t least = 0;
+  for (const int bn : {256, 128, 64}) {
+    const int64_t slice = bn == 256 ? 1536 : bn == 128 ? 768 : 640;
+    int64_t cost = 0;
+    for (const int p : {kGram, kSquare, kProduct})
+      cost += ceil_div(tiles_of(op[p].p->rows, op[p].q->rows, bn, it.gemm[p].out_kind) * it.batch, pairs) *
+                  ceil_div(op[p].p->cols, BK) * slice + 32 * bn;
+    if (best == 0 || cost < least) {
+      best = bn;
+      least = cost;
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -782,8 +928,8 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
   int* status = ws_at<int>(o.workspace, L.status);
   StepScale* scale = ws_at<StepScale>(o.workspace, L.scale);
   const Split x = split_at(o.workspace, L.x, o.batch, L.r, L.c, L.ld_c);
-  Split xt = split_at(o.workspace, L.xt0, o.batch, L.c, L.r, L.ld_r);
-  Split xt_next = split_at(o.workspace, L.xt1, o.batch, L.c, L.r, L.ld_r);
+  const Split xt = split_at(o.workspace, L.xt0, o.batch, L.c, L.r, L.ld_r);
+  const Split xt_next = split_at(o.workspace, L.xt1, o.batch, L.c, L.r, L.ld_r);
   const Split ma = split_at(o.workspace, L.a, o.batch, L.r, L.r, L.ld_r);
   const Split mb = split_at(o.workspace, L.b, o.batch, L.r, L.r, L.ld_r);
 
@@ -833,61 +979,60 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
   if (e != cudaSuccess) return e;
   note_launches(2);
 
-  GemmArgs base{};
-  base.batch = (int)o.batch;
-  base.scale_stride = o.steps;
-  base.run = o.dtype == LM_F32 ? 4 : o.dtype == LM_F16 ? 16 : 32;
-  base.status = status;
-  base.timeout_ns = wc.timeout_ns;
-  base.debug_skip_first_load = wc.debug_skip_first_load;
-  for (int k = 0; k < o.steps; ++k) {
-    GemmArgs a = base;
-    a.scale = scale + k;
-    a.kind = 0;
-    a.d_hi = ma.hi;
-    a.d_lo = ma.lo;
-    a.ld_d = ma.ld;
-    a.d_matrix = ma.matrix;
-    if ((e = launch_product<Out::kSymmetric>(x, x, a, stream)) != cudaSuccess) return e;
-    a.kind = 1;
-    a.add_hi = ma.hi;
-    a.add_lo = ma.lo;
-    a.d_hi = mb.hi;
-    a.d_lo = mb.lo;
-    if ((e = launch_product<Out::kSymmetric>(ma, ma, a, stream)) != cudaSuccess) return e;
-    a = base;
-    a.scale = scale + k;
-    a.kind = 2;
-    if (k + 1 < o.steps) {
-      // X in place: each value is read by the thread that replaces it.
-      a.add_hi = x.hi;
-      a.add_lo = x.lo;
-      a.d_hi = x.hi;
-      a.d_lo = x.lo;
-      a.ld_d = x.ld;
-      a.d_matrix = x.matrix;
-      a.t_hi = xt_next.hi;
-      a.t_lo = xt_next.lo;
-      a.ld_t = xt_next.ld;
-      a.t_matrix = xt_next.matrix;
-      if ((e = launch_product<Out::kBoth>(mb, xt, a, stream)) != cudaSuccess) return e;
-      std::swap(xt, xt_next);
-    } else {
-      // The last product runs in the order that lets the lanes of a warp write the result's rows.
-      const Split& add = tall ? x : xt;
-      a.add_hi = add.hi;
-      a.add_lo = add.lo;
-      a.ld_d = add.ld;
-      a.d_matrix = add.matrix;
-      a.out = o.out;
-      a.ld_out = o.cols;
-      a.out_matrix = o.rows * o.cols;
-      a.out_dtype = o.dtype;
-      e = tall ? launch_product<Out::kFinal>(mb, xt, a, stream) : launch_product<Out::kFinal>(xt, mb, a, stream);
-      if (e != cudaSuccess) return e;
-    }
-    note_launches(3);
+  IterArgs it{};
+  it.scale = scale;
+  it.arrived = reinterpret_cast<unsigned*>(status + 1);
+  it.status = status;
+  it.timeout_ns = wc.timeout_ns;
+  it.steps = o.steps;
+  it.batch = (int)o.batch;
+  it.run = o.dtype == LM_F32 ? 4 : o.dtype == LM_F16 ? 16 : 32;
+  it.debug_skip_first_load = wc.debug_skip_first_load;
+  auto to = [](GemmArgs& a, int out_kind, int kind, const Split& d) {
+    a.out_kind = out_kind;
+    a.kind = kind;
+    a.d_hi = d.hi;
+    a.d_lo = d.lo;
+    a.ld_d = d.ld;
+    a.d_matrix = d.matrix;
+  };
+  auto add = [](GemmArgs& a, const Split& s) {
+    a.add_hi = s.hi;
+    a.add_lo = s.lo;
+  };
+  const Split xts[2] = {xt, xt_next};
+  Operands op[kProducts];
+  op[kGram] = {&x, &x};
+  to(it.gemm[kGram], kSymmetric, 0, ma);
+  op[kSquare] = {&ma, &ma};
+  to(it.gemm[kSquare], kSymmetric, 1, mb);
+  add(it.gemm[kSquare], ma);
+  for (int b = 0; b < 2; ++b) {
+    // X in place (each value is read by the thread that replaces it), X^T into the other buffer.
+    GemmArgs& a = it.gemm[kProduct + b];
+    op[kProduct + b] = {&mb, &xts[b]};
+    to(a, kBoth, 2, x);
+    add(a, x);
+    a.t_hi = xts[1 - b].hi;
+    a.t_lo = xts[1 - b].lo;
+    a.ld_t = xts[1 - b].ld;
+    a.t_matrix = xts[1 - b].matrix;
   }
+  // The last product runs in the order that lets the lanes of a warp write the result's rows.
+  const Split& last = xts[(o.steps - 1) & 1];
+  GemmArgs& f = it.gemm[kLast];
+  op[kLast] = tall ? Operands{&mb, &last} : Operands{&last, &mb};
+  to(f, kFinal, 2, tall ? x : last);
+  add(f, tall ? x : last);
+  f.out = o.out;
+  f.ld_out = o.cols;
+  f.out_matrix = o.rows * o.cols;
+  f.out_dtype = o.dtype;
+  const int bn = tile_width(it, op);
+  e = bn == 256 ? launch_iteration<256>(it, op, stream) : bn == 128 ? launch_iteration<128>(it, op, stream)
+                                                                    : launch_iteration<64>(it, op, stream);
+  if (e != cudaSuccess) return e;
+  note_launches(1);
   return cudaGetLastError();
 }
 
