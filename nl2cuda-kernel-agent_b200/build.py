@@ -1,7 +1,8 @@
-"""Build the sm_100a shared library of this package: lib/librbf_sm100.so.
+"""Build the sm_100a shared library of this package, lib/librbf_sm100.so, and the torch binding of
+its language-model entries, lib/lm_sm100_torch.so.
 
 One nvcc invocation per .cu (objects cached by mtime under _build/), then a single
-``nvcc -shared`` link.  The library exports only the C ABI of include/rbf_sm100.h.  Used by
+``nvcc -shared`` link.  The library exports only the C ABI of include/*.h.  Used by
 __graft_entry__.build(), by framework/loader.py (rebuild when a source is newer than the .so)
 and directly:  python nl2cuda-kernel-agent_b200/build.py [--verbose] [--ptxas-info]
 """
@@ -23,12 +24,59 @@ COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler",
           "-fvisibility=hidden", "-I", INCLUDE, "-I", CSRC]
 
 
+BINDING = "lm_sm100_torch"
+
+
 def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")))
 
 
 def lib_path(name="rbf_sm100"):
     return os.path.join(PKG, "lib", f"lib{name}.so")
+
+
+def binding_path():
+    """The torch binding of the language-model entries: a Python extension module."""
+    return os.path.join(PKG, "lib", f"{BINDING}.so")
+
+
+def binding_stale():
+    out = binding_path()
+    if not os.path.exists(out):
+        return True
+    srcs = glob.glob(os.path.join(CSRC, "binding", "*.cpp"))
+    srcs += glob.glob(os.path.join(INCLUDE, "*.h"))
+    return _newest(srcs + [__file__]) > os.path.getmtime(out)
+
+
+def build_binding(verbose=False):
+    """Compile csrc/binding/*.cpp against torch's headers and link lib/lm_sm100_torch.so to
+    lib/librbf_sm100.so beside it."""
+    import sysconfig
+
+    import torch
+    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    out = binding_path()
+    os.makedirs(os.path.dirname(out), exist_ok=True)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-fvisibility=hidden", f"-DTORCH_EXTENSION_NAME={BINDING}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-isystem", os.path.join(cuda, "include"),
+           "-isystem", sysconfig.get_paths()["include"],
+           *sorted(glob.glob(os.path.join(CSRC, "binding", "*.cpp"))), "-o", out + ".tmp",
+           "-L", os.path.dirname(out), "-l:librbf_sm100.so", "-Wl,-rpath,$ORIGIN", "-L", libs,
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
+           # The C++ runtime that torch uses, by name: where the compiler finds only the archive, the
+           # module would carry a second one, whose locale facets are not torch's.
+           "-l:libstdc++.so.6"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(out + ".tmp", out)
+    return out
 
 
 def headers():
@@ -84,4 +132,6 @@ if __name__ == "__main__":
     ap.add_argument("--force", action="store_true")
     a = ap.parse_args()
     print(build(verbose=a.verbose, ptxas_info=a.ptxas_info, force=a.force))
+    if a.force or binding_stale():
+        print(build_binding(verbose=a.verbose))
     sys.exit(0)

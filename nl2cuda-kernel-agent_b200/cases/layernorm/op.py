@@ -1,39 +1,16 @@
-"""The layer-norm candidate: autograd op over the sm_100a kernels.
+"""The layer-norm candidate: an autograd operator over the sm_100a kernels.
 
 ``layer_norm(x, weight, bias, eps)`` is the call for models; ``candidate(inputs, params)`` is the
 harness contract.  Gradients flow to x, weight and bias.
 """
-import torch
-from torch.autograd.function import once_differentiable
-
 from cases.layernorm import native
-
-
-class LayerNormFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = native.ln_forward(x, weight, bias, eps)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        given = weight if weight is not None else bias
-        ctx.wdtype = x.dtype if given is None else given.dtype
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        dx, dw, db = native.ln_backward(dy, x, weight, mean, rstd,
-                                        need=ctx.needs_input_grad[:3], wdtype=ctx.wdtype)
-        return dx, dw, db, None
+from cases.lm_binding import ext
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (CUDA tensor, float32,
     bfloat16 or float16); weight and bias [D], of x's type or float32, or None (1 and 0)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, weight, bias)):
-        return LayerNormFunction.apply(x, weight, bias, eps)
-    return native.ln_forward(x, weight, bias, eps, keep=False)[0]
+    return ext().layer_norm(x, weight, bias, eps)
 
 
 def candidate(inputs, params):

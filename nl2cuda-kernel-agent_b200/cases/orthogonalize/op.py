@@ -3,18 +3,14 @@
 ``orthogonalize(update, ...)`` is the call for optimisers; ``candidate(inputs, params)`` is the
 harness contract.  There is no gradient: an update is not differentiated.
 """
-import torch
-
 from cases.orthogonalize import config, native
 
 
 def orthogonalize(update, steps=config.STEPS, coefficients=config.COEFFICIENTS, eps=config.EPS):
     """``update`` [..., m, n] with all its singular values brought near 1 by ``steps``
     Newton-Schulz products; coefficients (a, b, c), or one of these for every step.  Same shape and
-    type (float32, bfloat16 or float16, CUDA); leading dimensions are a batch."""
-    if torch.is_grad_enabled() and update.requires_grad:
-        raise RuntimeError("orthogonalize has no gradient: pass a detached update, or call it under "
-                           "torch.no_grad()")
+    type (float32, bfloat16 or float16, CUDA); leading dimensions are a batch.  An update that
+    requires a gradient is refused outside torch.no_grad()."""
     return native.orthogonalize(update, steps, coefficients, eps)
 
 
@@ -25,5 +21,4 @@ def candidate(inputs, params):
 
 def forward_only(inputs, params):
     """Same: there is no autograd in this case."""
-    return native.orthogonalize(inputs["update"], params["steps"], params["coefficients"],
-                                params["eps"])
+    return candidate(inputs, params)

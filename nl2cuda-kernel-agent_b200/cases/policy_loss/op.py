@@ -1,34 +1,10 @@
-"""The clipped policy-loss candidate: autograd op over the sm_100a kernels.
+"""The clipped policy-loss candidate: an autograd operator over the sm_100a kernels.
 
 ``policy_loss(...)`` is the call for training programs; ``candidate(inputs, params)`` is the
 harness contract.  The gradient flows to the logits.
 """
-import torch
-from torch.autograd.function import once_differentiable
-
+from cases.lm_binding import ext
 from cases.policy_loss import native
-from cases.token_logprob.native import logprob_backward
-
-
-class PolicyLossFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, old_logprob, ref_logprob, advantage, clip_low, clip_high,
-                kl_coef, ignore_index):
-        loss, kl, stats, coef, norm = native.policy_forward(
-            logits, labels, old_logprob, ref_logprob, advantage, clip_low, clip_high, kl_coef,
-            ignore_index)
-        ctx.save_for_backward(logits, labels, stats, coef, norm)
-        ctx.ignore_index = ignore_index
-        ctx.mark_non_differentiable(kl)
-        return loss, kl
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _kl):
-        logits, labels, stats, coef, norm = ctx.saved_tensors
-        dx = logprob_backward(logits, labels, stats, coef, ctx.ignore_index, scale0=g,
-                              scale1=norm)
-        return (dx,) + (None,) * 8
 
 
 def policy_loss(logits, labels, old_logprob, ref_logprob, advantage, clip_low=0.2, clip_high=0.2,
@@ -38,8 +14,8 @@ def policy_loss(logits, labels, old_logprob, ref_logprob, advantage, clip_low=0.
 
     logits [B, T, V] (CUDA; float32, bfloat16 or float16), labels [B, T] int64, old_logprob and
     ref_logprob [B, T] float32, advantage [B] or [B, T] float32."""
-    return PolicyLossFunction.apply(logits, labels, old_logprob, ref_logprob, advantage,
-                                    clip_low, clip_high, kl_coef, ignore_index)
+    return ext().policy_loss(logits, labels, old_logprob, ref_logprob, advantage, clip_low,
+                             clip_high, kl_coef, ignore_index)
 
 
 def candidate(inputs, params):

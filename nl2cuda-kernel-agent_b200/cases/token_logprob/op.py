@@ -1,27 +1,10 @@
-"""The token log-probability candidate: autograd op over the sm_100a kernels.
+"""The token log-probability candidate: an autograd operator over the sm_100a kernels.
 
 ``token_logprob(logits, labels)`` is the call for models; ``candidate(inputs, params)`` is the
 harness contract.  The gradient flows to the logits.
 """
-import torch
-from torch.autograd.function import once_differentiable
-
+from cases.lm_binding import ext
 from cases.token_logprob import native
-
-
-class TokenLogprobFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, ignore_index):
-        lp, stats = native.logprob_forward(logits, labels, ignore_index)
-        ctx.save_for_backward(logits, labels, stats)
-        ctx.ignore_index = ignore_index
-        return lp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        logits, labels, stats = ctx.saved_tensors
-        return native.logprob_backward(logits, labels, stats, g, ctx.ignore_index), None, None
 
 
 def token_logprob(logits, labels, ignore_index=-100):
@@ -29,9 +12,7 @@ def token_logprob(logits, labels, ignore_index=-100):
 
     logits [..., V] (CUDA; float32, bfloat16 or float16), labels [...] int64.  A label outside
     [0, V) that is not ``ignore_index`` gives NaN."""
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return TokenLogprobFunction.apply(logits, labels, ignore_index)
-    return native.logprob_forward(logits, labels, ignore_index, keep=False)[0]
+    return ext().token_logprob(logits, labels, ignore_index)
 
 
 def candidate(inputs, params):

@@ -12,6 +12,7 @@ the build, but calling into the library without an sm_100 device returns an erro
 which the Python layer raises as RuntimeError.
 """
 import ctypes
+import importlib.util
 import os
 import shutil
 import sys
@@ -63,3 +64,24 @@ def load_kernel(name, sources=None, base_dir=None, extra_cuda_cflags=None, extra
         lib = ctypes.CDLL(path)
         _loaded[name] = lib
         return lib
+
+
+def load_torch_binding():
+    """Build (if stale) and import lib/lm_sm100_torch.so, the torch binding of the language-model
+    entries (csrc/binding): a Python extension module over lib/librbf_sm100.so."""
+    load_kernel("rbf_sm100")
+    with _lock:
+        if _build.BINDING in _loaded:
+            return _loaded[_build.BINDING]
+        path = _build.binding_path()
+        if _build.binding_stale():
+            if shutil.which(os.environ.get("CXX", "g++")) is not None:
+                _build.build_binding()
+            elif not os.path.exists(path):
+                raise RuntimeError(f"{path} is missing and there is no C++ compiler to build it")
+        import torch  # noqa: F401  (the module's symbols come from torch's libraries)
+        spec = importlib.util.spec_from_file_location(_build.BINDING, path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _loaded[_build.BINDING] = module
+        return module

@@ -313,10 +313,10 @@ def test_captured_and_replayed_on_new_data(which, cuda_device):
             out, stats = lp.logprob_forward(x, labels, IGNORE)
             return out, lp.logprob_backward(x, labels, stats, ref, IGNORE)
         if which == "preference":
-            loss, r, stats, c = pref.preference_forward(x, labels, ref, 0.1, 0.0, IGNORE)
-            return loss, r, lp.logprob_backward(x, labels, stats, c, IGNORE)
-        loss, kl, stats, c, n = pol.policy_forward(x, labels, old, ref, adv, 0.2, 0.2, 0.1, IGNORE)
-        return loss, kl, lp.logprob_backward(x, labels, stats, c, IGNORE, scale1=n)
+            loss, r, state = pref.preference_forward(x, labels, ref, 0.1, 0.0, IGNORE)
+            return loss, r, pref.preference_backward(x, labels, state, None, IGNORE)
+        loss, kl, state = pol.policy_forward(x, labels, old, ref, adv, 0.2, 0.2, 0.1, IGNORE)
+        return loss, kl, pol.policy_backward(x, labels, state, None, IGNORE)
 
     want = step(x, labels)
     graphs = []

@@ -9,6 +9,8 @@ import re
 import pytest
 import torch
 
+import lm_abi
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 OK, INVALID, MISALIGNED, WORKSPACE, UNSUPPORTED = 0, 1, 2, 3, 4
 A = 1 << 20  # an aligned address that is never touched: every refusal comes first
@@ -16,16 +18,14 @@ A = 1 << 20  # an aligned address that is never touched: every refusal comes fir
 
 @pytest.fixture(scope="module")
 def lib():
-    from cases import lm_binding
-    return lm_binding.lib()
+    return lm_abi.lib()
 
 
 def test_library_exports_the_header(lib):
     text = open(os.path.join(ROOT, "include", "lm_sm100.h")).read()
     names = re.findall(r"RBF_API\s+\w+\s+(\w+)\s*\(", text)
     assert len(names) >= 8
-    from cases import lm_binding
-    assert set(names) == set(lm_binding._SIGNATURES)
+    assert set(names) == set(lm_abi.SIGNATURES)
     assert all(hasattr(lib, n) for n in names)
 
 
