@@ -187,8 +187,6 @@ int lp_sm100_backward(const void* logits, int64_t batch_stride, int64_t t_stride
   if ((st = need(dlogits, rows * V, e, "dlogits"))) return st;
   if (scale0 != nullptr && (st = need(scale0, 1, 4, "scale0"))) return st;
   if (scale1 != nullptr && (st = need(scale1, 1, 4, "scale1"))) return st;
-  if (rows * logprob_backward_slices(V, dtype) >= kMaxRows)
-    return refuse(RBF_ERR_UNSUPPORTED, "rows * V too large for one launch");
   if ((st = check_device())) return st;
   LogitArgs a{};
   a.logits = logits;

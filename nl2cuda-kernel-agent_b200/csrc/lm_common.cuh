@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/lm_sm100.h"
 #include "rbf_common.cuh"
 #include "rbf_kernels.cuh"
@@ -40,6 +42,82 @@ template <typename T, int VEC>
 struct alignas(VEC * sizeof(T)) Pack {
   T v[VEC];
 };
+
+// ---- two fp32 values in one register pair: sm_100 adds and multiplies both in one instruction
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// Elements 2 k and 2 k + 1 of a pack, and back (one rounding each).
+template <typename T, int VEC>
+__device__ __forceinline__ F2 pair_of(const Pack<T, VEC>& p, int k) {
+  if constexpr (sizeof(T) == 4) {
+    return f2(p.v[2 * k], p.v[2 * k + 1]);
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const uint32_t w = reinterpret_cast<const uint32_t*>(&p)[k];
+    return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    const float2 x = __half22float2(reinterpret_cast<const __half2*>(&p)[k]);
+    return f2(x.x, x.y);
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void set_pair(Pack<T, VEC>& p, int k, F2 x) {
+  float a, b;
+  unpack(x, a, b);
+  if constexpr (sizeof(T) == 4) {
+    p.v[2 * k] = a;
+    p.v[2 * k + 1] = b;
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    reinterpret_cast<__nv_bfloat162*>(&p)[k] = __floats2bfloat162_rn(a, b);
+  } else {
+    reinterpret_cast<__half2*>(&p)[k] = __floats2half2_rn(a, b);
+  }
+}
+
+// The largest element of a pack (NaN is passed over), 16-bit types two at a time.
+template <typename T, int VEC>
+__device__ __forceinline__ float pack_max(const Pack<T, VEC>& p) {
+  if constexpr (sizeof(T) == 4) {
+    float m = p.v[0];
+#pragma unroll
+    for (int e = 1; e < VEC; ++e) m = fmaxf(m, p.v[e]);
+    return m;
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162* q = reinterpret_cast<const __nv_bfloat162*>(&p);
+    __nv_bfloat162 m = q[0];
+#pragma unroll
+    for (int e = 1; e < VEC / 2; ++e) m = __hmax2(m, q[e]);
+    return fmaxf(__low2float(m), __high2float(m));
+  } else {
+    const __half2* q = reinterpret_cast<const __half2*>(&p);
+    __half2 m = q[0];
+#pragma unroll
+    for (int e = 1; e < VEC / 2; ++e) m = __hmax2(m, q[e]);
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+}
 
 // Streaming read: data that this kernel reads once bypasses L1 (the operands that CTAs share,
 // such as a weight vector, keep it).

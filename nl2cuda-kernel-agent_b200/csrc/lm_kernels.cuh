@@ -44,7 +44,6 @@ struct LogitArgs {
   void* dlogits;
 };
 cudaError_t launch_logprob_forward(const LogitArgs& a, cudaStream_t stream);
-int64_t logprob_backward_slices(int64_t V, int dtype);
 cudaError_t launch_logprob_backward(const LogitArgs& a, cudaStream_t stream);
 
 struct LossArgs {

@@ -22,9 +22,10 @@ namespace lm {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kFwdThreads = 256;
-constexpr int kBwdThreads = 256;
-constexpr int kPacks = 4;        // 16-byte loads in flight per thread
+constexpr float kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e);
+constexpr int kFwdThreads = 256, kFwdCtas = 6;  // threads of a CTA, CTAs an SM holds at least
+constexpr int kBwdThreads = 256, kBwdCtas = 4;
+constexpr int kPacks = 4;                       // 16-byte loads in flight per thread
 constexpr int kMaxSplit = 8;     // CTAs (one cluster) of a forward row
 
 struct MaxSum {
@@ -33,13 +34,24 @@ struct MaxSum {
 
 __device__ __forceinline__ float exp_diff(float x, float m) { return exp2_approx((x - m) * kLog2e); }
 
+// For the sum: with what log2 e loses in fp32 (1.3e-8 of it), which makes every term of a given size
+// come out high alike, 1e-7 at x - m = -8: the rewards of long answers add that up.
+__device__ __forceinline__ float exp_diff_exact(float x, float m) {
+  const float d = x - m;
+  return exp2_approx(fmaf(d, kLog2e, d * kLog2eRest));
+}
+
+// For partial sums that move to a larger maximum: ex2.approx comes out low by some 2^-25 on average, and
+// a term passes through up to ten of these on its way, all in the same direction.  expf does not.
+__device__ __forceinline__ float rescale(float m, float to) { return expf(m - to); }
+
 // The maximum to subtract: any finite value while every term so far is exp(-inf).
 __device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
 
 __device__ __forceinline__ MaxSum merge(MaxSum a, MaxSum b) {
   const float m = fmaxf(a.m, b.m);
   const float ref = reference(m);
-  return {m, a.s * exp_diff(a.m, ref) + b.s * exp_diff(b.m, ref)};
+  return {m, a.s * rescale(a.m, ref) + b.s * rescale(b.m, ref)};
 }
 
 __device__ __forceinline__ MaxSum warp_merge(MaxSum v) {
@@ -55,9 +67,9 @@ __device__ __forceinline__ void accumulate(MaxSum& v, const float (&x)[N]) {
 #pragma unroll
   for (int e = 0; e < N; ++e) m = fmaxf(m, x[e]);
   const float ref = reference(m);
-  float s = v.s * exp_diff(v.m, ref);
+  float s = v.s * rescale(v.m, ref);
 #pragma unroll
-  for (int e = 0; e < N; ++e) s += exp_diff(x[e], ref);
+  for (int e = 0; e < N; ++e) s += exp_diff_exact(x[e], ref);
   v.m = m;
   v.s = s;
 }
@@ -76,11 +88,58 @@ __device__ __forceinline__ int64_t head_of(const T* p, int64_t n) {
   return h < n ? h : n;
 }
 
-// One row per CTA, or per cluster of `split` CTAs that share its elements: with few rows there
-// are more SMs than rows, and a row of 128 K elements read by one SM alone takes longer than the
-// rest of the pass.  The shares of a cluster meet in its first CTA's shared memory.
+// The elements of a row outside its whole packs: fewer than a pack at either end.
 template <typename T>
-__global__ void __launch_bounds__(kFwdThreads) logprob_forward_kernel(const LogitArgs a, int split) {
+__device__ __forceinline__ void accumulate_ends(MaxSum& v, const T* x, int64_t head, int64_t tail, int64_t V) {
+  if (threadIdx.x < head) {
+    const float f[1] = {to_f32(x[threadIdx.x])};
+    accumulate(v, f);
+  }
+  if (tail + threadIdx.x < V) {
+    const float f[1] = {to_f32(x[tail + threadIdx.x])};
+    accumulate(v, f);
+  }
+}
+
+template <typename T, int VEC, int N>
+__device__ __forceinline__ void accumulate_packs(MaxSum& v, const Pack<T, VEC> (&p)[N]) {
+  float m = v.m;
+#pragma unroll
+  for (int u = 0; u < N; ++u) m = fmaxf(m, pack_max(p[u]));
+  const float ref = reference(m);
+  const F2 shift = f2(-ref, -ref), hi = f2(kLog2e, kLog2e), lo = f2(kLog2eRest, kLog2eRest);
+  F2 s = f2(v.s * rescale(v.m, ref), 0.f);
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int k = 0; k < VEC / 2; ++k) {
+      const F2 d = add2(pair_of(p[u], k), shift);
+      float a, b;
+      unpack(fma2(d, hi, mul2(d, lo)), a, b);  // exp_diff_exact of both
+      s = add2(s, f2(exp2_approx(a), exp2_approx(b)));
+    }
+  float a, b;
+  unpack(s, a, b);
+  v.m = m;
+  v.s = a + b;
+}
+
+template <typename T>
+__device__ __forceinline__ void write_row(const LogitArgs& a, int64_t r, int64_t label, bool scored, const T* x, MaxSum t) {
+  float lp = 0.f;
+  if (scored) lp = label >= 0 && label < a.V ? (to_f32(x[label]) - t.m) - logf(t.s) : NAN;
+  a.logprob[r] = lp;
+  if (a.stats != nullptr) {
+    a.stats[2 * r] = t.m;
+    a.stats[2 * r + 1] = 1.f / t.s;
+  }
+}
+
+// One row per CTA; or a cluster of `split` CTAs per row: with few rows there are more SMs than rows, and
+// a row of 128 K elements read by one SM alone takes longer than the rest of the pass.  The shares
+// meet in the first CTA's shared memory.
+template <typename T>
+__global__ void __launch_bounds__(kFwdThreads, kFwdCtas) logprob_forward_kernel(const LogitArgs a, int split) {
   constexpr int VEC = 16 / sizeof(T);
   __shared__ MaxSum part[kMaxSplit][kFwdThreads / 32];
   if (split > 1) ptx::cluster_sync();  // every CTA of the cluster runs before one writes to another
@@ -101,31 +160,13 @@ __global__ void __launch_bounds__(kFwdThreads) logprob_forward_kernel(const Logi
       Pack<T, VEC> p[kPacks];
 #pragma unroll
       for (int u = 0; u < kPacks; ++u) p[u] = load_stream<T, VEC>(body + (i + u * kFwdThreads) * VEC);
-      float f[kPacks * VEC];
-#pragma unroll
-      for (int u = 0; u < kPacks; ++u)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) f[u * VEC + e] = to_f32(p[u].v[e]);
-      accumulate(v, f);
+      accumulate_packs(v, p);
     }
     for (; i < end; i += kFwdThreads) {
-      const Pack<T, VEC> p = load_stream<T, VEC>(body + i * VEC);
-      float f[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) f[e] = to_f32(p.v[e]);
-      accumulate(v, f);
+      const Pack<T, VEC> p[1] = {load_stream<T, VEC>(body + i * VEC)};
+      accumulate_packs(v, p);
     }
-    if (share == 0) {
-      const int64_t tail = head + packs * VEC;
-      if (threadIdx.x < head) {
-        const float f[1] = {to_f32(x[threadIdx.x])};
-        accumulate(v, f);
-      }
-      if (tail + threadIdx.x < a.V) {  // fewer than VEC elements
-        const float f[1] = {to_f32(x[tail + threadIdx.x])};
-        accumulate(v, f);
-      }
-    }
+    if (share == 0) accumulate_ends(v, x, head, head + packs * VEC, a.V);
     v = warp_merge(v);
   }
   if ((threadIdx.x & 31) == 0) {
@@ -145,27 +186,16 @@ __global__ void __launch_bounds__(kFwdThreads) logprob_forward_kernel(const Logi
   MaxSum t{-INFINITY, 0.f};
   for (int i = threadIdx.x; i < split * W; i += 32) t = merge(t, part[i / W][i % W]);
   t = warp_merge(t);
-  if (threadIdx.x == 0) {
-    float lp = 0.f;
-    if (scored) {
-      const bool valid = label >= 0 && label < a.V;
-      lp = valid ? (to_f32(x[label]) - t.m) - logf(t.s) : NAN;
-    }
-    a.logprob[r] = lp;
-    if (a.stats != nullptr) {
-      a.stats[2 * r] = t.m;
-      a.stats[2 * r + 1] = 1.f / t.s;
-    }
-  }
+  if (threadIdx.x == 0) write_row(a, r, label, scored, x, t);
 }
 
-// kPacks packs per thread and CTA, `slices` CTAs per row.  SAME: the row's logits and gradients
-// have the same offset from a 16-byte boundary, so both move in packs.
+// `slices` CTAs per row, each a share of its packs.  Registers for four CTAs an SM and no second set of
+// packs in flight: 98% of the copy rate at 16384 x 131072 bf16; a software pipeline over two packs in
+// the same registers was at 78%, one over single packs with six CTAs at 88%.
 template <typename T>
-__global__ void __launch_bounds__(kBwdThreads)
-    logprob_backward_kernel(const LogitArgs a, int slices) {
+__global__ void __launch_bounds__(kBwdThreads, kBwdCtas) logprob_backward_kernel(const LogitArgs a, int slices) {
   constexpr int VEC = 16 / sizeof(T);
-  constexpr int SPAN = kPacks * kBwdThreads;  // packs of one CTA
+  constexpr int STEP = kPacks * kBwdThreads;
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   // Last rows first: what the forward read last is still in L2.
@@ -173,61 +203,78 @@ __global__ void __launch_bounds__(kBwdThreads)
   const int64_t r = block / slices;
   const int64_t slice = block - r * slices;
   const int64_t label = a.labels[r];
-  const bool scored = label != a.ignore_index;
   const T* x = row_of<T>(a, r);
   T* dx = static_cast<T*>(a.dlogits) + r * a.V;
-  float c = 0.f, m = 0.f, neg = 0.f;
-  if (scored) {
-    c = a.coef[r];
-    if (a.scale0 != nullptr) c *= *a.scale0;
-    if (a.scale1 != nullptr) c *= *a.scale1;
-    m = a.stats[2 * r];
-    neg = -c * a.stats[2 * r + 1];
-  }
-  auto grad = [&](float v, int64_t j) {
-    const float g = neg * exp_diff(v, m);
-    return j == label ? c + g : g;
-  };
   const int64_t head = head_of(dx, a.V);
-  const bool same = head_of(x, a.V) == head;
   const int64_t packs = (a.V - head) / VEC;
   const int64_t tail = head + packs * VEC;
-  if (slice == 0) {
-    for (int64_t j = threadIdx.x; j < head; j += kBwdThreads)
-      dx[j] = from_f32<T>(scored ? grad(to_f32(x[j]), j) : 0.f);
-    for (int64_t j = tail + threadIdx.x; j < a.V; j += kBwdThreads)
-      dx[j] = from_f32<T>(scored ? grad(to_f32(x[j]), j) : 0.f);
+  const int64_t end = packs * (slice + 1) / slices;
+  int64_t i = packs * slice / slices + threadIdx.x;
+  if (label == a.ignore_index) {
+    Pack<T, VEC> zero;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) zero.v[e] = from_f32<T>(0.f);
+    for (; i < end; i += kBwdThreads) store_pack<T, VEC>(dx + head + i * VEC, zero);
+    if (slice == 0) {
+      if (threadIdx.x < head) dx[threadIdx.x] = from_f32<T>(0.f);
+      if (tail + threadIdx.x < a.V) dx[tail + threadIdx.x] = from_f32<T>(0.f);
+    }
+    return;
   }
-  const int64_t first = slice * SPAN + threadIdx.x;
+  const bool same = head_of(x, a.V) == head;  // both move in packs
   Pack<T, VEC> p[kPacks];
-  if (scored) {
+  auto fetch = [&]() {
 #pragma unroll
     for (int u = 0; u < kPacks; ++u) {
-      const int64_t i = first + u * kBwdThreads;
-      if (i < packs) {
-        if (same) {
-          p[u] = load_stream<T, VEC>(x + head + i * VEC);
-        } else {
+      const int64_t k = i + u * kBwdThreads;
+      if (k >= end) break;
+      const T* q = x + head + k * VEC;
+      if (same) {
+        p[u] = load_stream<T, VEC>(q);
+      } else {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) p[u].v[e] = x[head + i * VEC + e];
-        }
+        for (int e = 0; e < VEC; ++e) p[u].v[e] = q[e];
       }
     }
-  }
+  };
+  fetch();  // next to the row's scalars
+  float c = a.coef[r];
+  if (a.scale0 != nullptr) c *= *a.scale0;
+  if (a.scale1 != nullptr) c *= *a.scale1;
+  const float m = a.stats[2 * r];
+  const float neg = -c * a.stats[2 * r + 1];
+  auto grad = [&](float v, bool chosen) {
+    const float g = neg * exp_diff(v, m);
+    return chosen ? c + g : g;
+  };
+  const F2 shift = f2(-m, -m), log2e = f2(kLog2e, kLog2e), factor = f2(neg, neg);
+  while (i < end) {
 #pragma unroll
-  for (int u = 0; u < kPacks; ++u) {
-    const int64_t i = first + u * kBwdThreads;
-    if (i >= packs) break;
-    const int64_t j = head + i * VEC;
-    Pack<T, VEC> o;
+    for (int u = 0; u < kPacks; ++u) {
+      const int64_t k = i + u * kBwdThreads;
+      if (k >= end) break;
+      const int64_t j = head + k * VEC;
+      Pack<T, VEC> o;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<T>(scored ? neg * exp_diff(to_f32(p[u].v[e]), m) : 0.f);
-    if (scored && label >= j && label < j + VEC) {
+      for (int e = 0; e < VEC / 2; ++e) {
+        float x0, x1;
+        unpack(mul2(add2(pair_of(p[u], e), shift), log2e), x0, x1);
+        set_pair(o, e, mul2(f2(exp2_approx(x0), exp2_approx(x1)), factor));
+      }
+      if (label >= j && label < j + VEC) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (j + e == label) o.v[e] = from_f32<T>(grad(to_f32(p[u].v[e]), label));
+        for (int e = 0; e < VEC; ++e)
+          if (j + e == label) o.v[e] = from_f32<T>(grad(to_f32(p[u].v[e]), true));
+      }
+      store_pack<T, VEC>(dx + j, o);
     }
-    store_pack<T, VEC>(dx + j, o);
+    i += STEP;
+    fetch();
+  }
+  if (slice == 0) {
+    const int64_t j = threadIdx.x, k = tail + threadIdx.x;
+    if (j < head) dx[j] = from_f32<T>(grad(to_f32(x[j]), j == label));
+    if (k < a.V) dx[k] = from_f32<T>(grad(to_f32(x[k]), k == label));
   }
 }
 
@@ -383,30 +430,33 @@ cudaError_t by_type(int dtype, F f) {
 
 cudaError_t launch_logprob_forward(const LogitArgs& a, cudaStream_t stream) {
   if (a.rows == 0) return cudaSuccess;
-  // Enough CTAs for every SM to have two, as long as each keeps a few rounds of loads.
+  // With few rows, enough CTAs for every SM to have two, as long as each keeps a few rounds of loads.
   int split = 1;
   while (split < kMaxSplit && a.rows * split * 2 <= 2 * device_sm_count() &&
          a.V / (split * 2) >= 2 * kFwdThreads * 8)
     split *= 2;
-  const dim3 grid((unsigned)(a.rows * split));
   cudaError_t e = by_type(a.dtype, [&](auto t) {
-    auto k = logprob_forward_kernel<decltype(t)>;
-    if (split == 1) return launch_kernel(k, grid, dim3(kFwdThreads), 0, stream, a, 1);
-    return launch_kernel_cluster(k, grid, dim3(kFwdThreads), 0, split, stream, a, split);
+    using T = decltype(t);
+    const dim3 grid((unsigned)(a.rows * split)), block(kFwdThreads);
+    if (split > 1) return launch_kernel_cluster(logprob_forward_kernel<T>, grid, block, 0, split, stream, a, split);
+    return launch_kernel(logprob_forward_kernel<T>, grid, block, 0, stream, a, 1);
   });
   if (e != cudaSuccess) return e;
   note_launches(1);
   return cudaGetLastError();
 }
 
-// CTAs per row of the backward.
-int64_t logprob_backward_slices(int64_t V, int dtype) {
-  return ceil_div(V, (int64_t)kPacks * kBwdThreads * (16 / (int64_t)elem_bytes(dtype)));
+// CTAs per row of the backward: at least four steps each, and no more than give every SM 32 in all.
+int64_t logprob_backward_slices(int64_t rows, int64_t V, int dtype) {
+  const int64_t steps = ceil_div(V, (int64_t)kPacks * kBwdThreads * (16 / (int64_t)elem_bytes(dtype)));
+  const int64_t want = ceil_div(32 * (int64_t)device_sm_count(), rows > 0 ? rows : 1);
+  const int64_t most = steps / 4 > 1 ? steps / 4 : 1;
+  return want < 1 ? 1 : want < most ? want : most;
 }
 
 cudaError_t launch_logprob_backward(const LogitArgs& a, cudaStream_t stream) {
   if (a.rows == 0 || a.V == 0) return cudaSuccess;
-  const int64_t slices = logprob_backward_slices(a.V, a.dtype);
+  const int64_t slices = logprob_backward_slices(a.rows, a.V, a.dtype);
   cudaError_t e = by_type(a.dtype, [&](auto t) {
     return launch_kernel(logprob_backward_kernel<decltype(t)>, dim3((unsigned)(a.rows * slices)),
                          dim3(kBwdThreads), 0, stream, a, (int)slices);

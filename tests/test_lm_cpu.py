@@ -84,7 +84,7 @@ def test_logprob_refusals(lib):
     assert bwd(coef=A + 1) == MISALIGNED
     assert bwd(s0=A + 2) == MISALIGNED
     assert bwd(dx=None) == INVALID
-    assert bwd(rows=5 << 25, V=1 << 20) == UNSUPPORTED
+    assert bwd(rows=5 << 26) == UNSUPPORTED
 
 
 def test_loss_refusals(lib):
