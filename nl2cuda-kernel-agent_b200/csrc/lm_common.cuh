@@ -175,6 +175,15 @@ __device__ __forceinline__ void load_param(const void* p, int64_t i, int dtype, 
   }
 }
 
+// The same as pairs.
+template <int VEC>
+__device__ __forceinline__ void load_param(const void* p, int64_t i, int dtype, float absent, F2 (&out)[VEC / 2]) {
+  float t[VEC];
+  load_param<VEC>(p, i, dtype, absent, t);
+#pragma unroll
+  for (int e = 0; e < VEC / 2; ++e) out[e] = f2(t[2 * e], t[2 * e + 1]);
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

@@ -5,16 +5,15 @@
 //   dw = sum_rows dy * xh,   db = sum_rows dy
 //
 // Both passes are bound by HBM: the forward moves 2 elements and the backward 3 per value, at
-// some 10 flops each.  A row sits in the registers of a group of `W` warps, 16 values a lane, so
-// it is read once; the variance is a second pass over registers, not over memory, and has no
-// cancellation.  Groups walk over rows (a persistent grid) and load their next row before they
-// work on the present one, so that loads are in flight all the time.
+// some 10 flops each.  Every row is read once and held on chip; the variance is a second pass over
+// registers, not over memory, and has no cancellation.
 //
-// In the backward a lane keeps the sums of its 16 columns' dy * xh and dy in registers over all
+// In the backward a thread keeps the sums of its columns' dy * xh and dy in registers over all
 // its rows; each CTA writes one row of partial sums at its end and a second, short kernel adds
 // those in a fixed order.  No atomics: equal calls give equal bits.
 //
 // Statistics, sums and partial sums are fp32; every output is rounded once.
+#include <algorithm>
 #include <type_traits>
 
 #include "lm_common.cuh"
@@ -28,7 +27,7 @@ constexpr int kLaneElems = 16;                   // values of a row per lane
 constexpr int kWarpElems = 32 * kLaneElems;
 constexpr int64_t kMaxRegD = 32 * kWarpElems;    // longest row held in the registers of one CTA
 constexpr int kWideThreads = 1024;
-constexpr int kSumRows = 16;                     // partial rows a thread column of ln_sum adds at a time
+constexpr int kSumRows = 32;                     // partial rows that ln_sum adds side by side
 
 // Sum of (a, b) over the warps of a group.  red: two slots of 32 float2 for this group, used in
 // turn, so that one barrier per reduction is enough.
@@ -67,67 +66,393 @@ struct Row {
   }
 };
 
-// CTAs of `groups` groups of W warps; each group takes one row at a time.
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(1024) ln_forward_kernel(const LnArgs a, int W, int groups) {
+// A group of W warps takes a row, `groups` rows a CTA.  The row is read once, all its loads at a time,
+// and stays in registers as it came; mean, variance and result are three passes over those.
+template <typename T, int VEC, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS) ln_forward_kernel(const LnArgs a, int W, int groups) {
   __shared__ float2 red[32 * 2 * 8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = warp / W, w = warp - g * W;
   float2* slots = red + g * 64;
   int turn = 0;
   const int D = (int)a.D;
-  const int64_t step = (int64_t)gridDim.x * groups;
-  int64_t r = (int64_t)blockIdx.x * groups + g;
+  const int64_t r = (int64_t)blockIdx.x * groups + g;
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
-  const T* x = static_cast<const T*>(a.x);
-  T* y = static_cast<T*>(a.y);
-  Row<T, VEC, NV> next;
-  if (r < a.rows) next.load(x + r * a.x_stride, D, W, w, lane);
-  const float inv_d = 1.f / (float)a.D;
-  for (; r < a.rows; r += step) {
-    float v[NV * VEC];
+  if (r >= a.rows) return;
+  T* y = static_cast<T*>(a.y) + r * D;
+  Row<T, VEC, NV> x;
+  x.load(static_cast<const T*>(a.x) + r * a.x_stride, D, W, w, lane);
+  const float inv_d = 1.f / (float)D;
+  float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[i * VEC + e] = to_f32(next.p[i].v[e]);
-    if (r + step < a.rows) next.load(x + (r + step) * a.x_stride, D, W, w, lane);
-    float s = 0.f;
+    for (int e = 0; e < VEC; ++e) s += to_f32(x.p[i].v[e]);  // columns past D are 0
+  const float mean = group_sum(make_float2(s, 0.f), W, w, 1 + g, slots, turn).x * inv_d;
+  float q = 0.f;
 #pragma unroll
-    for (int k = 0; k < NV * VEC; ++k) s += v[k];
-    const float mean = group_sum(make_float2(s, 0.f), W, w, 1 + g, slots, turn).x * inv_d;
-    float q = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const bool in = ((i * W + w) * 32 + lane) * VEC < D;
+  for (int i = 0; i < NV; ++i) {
+    if (((i * W + w) * 32 + lane) * VEC < D) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float d = v[i * VEC + e] - mean;
-        if (in) q = fmaf(d, d, q);
-        v[i * VEC + e] = d;
+        const float d = to_f32(x.p[i].v[e]) - mean;
+        q = fmaf(d, d, q);
       }
     }
-    const float var = group_sum(make_float2(q, 0.f), W, w, 1 + g, slots, turn).x * inv_d;
-    const float rstd = 1.f / sqrtf(var + a.eps);
-    if (w == 0 && lane == 0 && a.mean != nullptr) {
-      a.mean[r] = mean;
-      a.rstd[r] = rstd;
-    }
+  }
+  const float var = group_sum(make_float2(q, 0.f), W, w, 1 + g, slots, turn).x * inv_d;
+  const float rstd = 1.f / sqrtf(var + a.eps);
+  if (w == 0 && lane == 0 && a.mean != nullptr) {
+    a.mean[r] = mean;
+    a.rstd[r] = rstd;
+  }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = ((i * W + w) * 32 + lane) * VEC;
-      if (c >= D) break;
+  for (int i = 0; i < NV; ++i) {
+    const int c = ((i * W + w) * 32 + lane) * VEC;
+    if (c < D) {
       float wv[VEC], bv[VEC];
       load_param<VEC>(a.weight, c, a.wdtype, 1.f, wv);
       load_param<VEC>(a.bias, c, a.wdtype, 0.f, bv);
       Pack<T, VEC> o;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<T>(fmaf(v[i * VEC + e] * rstd, wv[e], bv[e]));
-      store_pack<T, VEC>(y + r * a.D + c, o);
+      for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<T>(fmaf((to_f32(x.p[i].v[e]) - mean) * rstd, wv[e], bv[e]));
+      store_pack<T, VEC>(y + c, o);
     }
   }
 }
 
+// ---- rows of whole 16-byte packs, and enough of them: one CTA per SM
+// `TW` threads (a group) take ROWS rows at a time, each thread NV packs of a row.  A thread copies
+// what it will read itself into shared memory (cp.async), a ring of blocks ahead: 160 to 190 KB
+// an SM are on their way at any time, no registers wait for them, and no thread waits for another's
+// copy.  The rows of a block share each reduction and its barrier.  Arithmetic is on pairs: a value of
+// 16 bits has some 20 issue slots at the rate that HBM delivers them.
+constexpr int kRingThreads = 512;
+constexpr size_t kRingBytes = 196608;
+
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// OPS operands (x; or x and dy) of ROWS rows a block.
+template <typename T, int NV, int ROWS, int OPS>
+struct Ring {
+  static constexpr int VEC = 16 / sizeof(T);
+  static constexpr int kPieces = ROWS * NV * OPS;  // 16-byte pieces of a thread and block
+  static constexpr int kFit = (int)(kRingBytes / (kPieces * 16 * kRingThreads));
+  static constexpr int STAGES = kFit > 8 ? 8 : kFit;
+  static_assert(STAGES >= 3, "ring");
+  uint4* ring;  // [STAGES][kPieces][kRingThreads]
+  int TW, groups, g, in, D;
+  int64_t rows, per_block, blocks;
+  __device__ __forceinline__ Ring(uint4* smem, const LnArgs& a, int tw) : ring(smem), TW(tw), rows(a.rows) {
+    groups = kRingThreads / TW;
+    g = threadIdx.x / TW;
+    in = threadIdx.x - g * TW;
+    D = (int)a.D;
+    per_block = (int64_t)groups * ROWS;
+    blocks = (rows + per_block - 1) / per_block;
+  }
+  __device__ __forceinline__ int column(int i) const { return (i * TW + in) * VEC; }
+  __device__ __forceinline__ int64_t row(int64_t block, int k) const { return block * per_block + g * ROWS + k; }
+  __device__ __forceinline__ void issue(const T* const (&op)[OPS], const int64_t (&stride)[OPS], int64_t block, int stage) {
+    if (block < blocks) {
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) {
+        const int64_t r = row(block, k);
+        if (r < rows) {
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+            if (column(i) < D) {
+#pragma unroll
+              for (int o = 0; o < OPS; ++o)
+                copy_async16(ptx::smem_u32(ring + (stage * kPieces + (k * NV + i) * OPS + o) * kRingThreads + threadIdx.x),
+                             op[o] + r * stride[o] + column(i));
+            }
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // Piece (row k, pack i, operand o) of the block in `stage`; zeros outside the matrix.
+  __device__ __forceinline__ Pack<T, VEC> read(int64_t block, int stage, int k, int i, int o) const {
+    Pack<T, VEC> p;
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (row(block, k) < rows && column(i) < D) u = ring[(stage * kPieces + (k * NV + i) * OPS + o) * kRingThreads + threadIdx.x];
+    *reinterpret_cast<uint4*>(&p) = u;
+    return p;
+  }
+};
+
+// Sums of N values over a group's threads.  red: [2][warps of the CTA][N], used in turn.
+template <int N>
+__device__ __forceinline__ void ring_sum(float (&s)[N], int W, int g, float (*red)[kRingThreads / 32][N], int& turn) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int v = 0; v < N; ++v) s[v] = warp_sum(s[v]);
+  if (W == 1) return;
+  if (lane == 0) {
+#pragma unroll
+    for (int v = 0; v < N; ++v) red[turn][warp][v] = s[v];
+  }
+  named_sync(1 + g, W * 32);
+#pragma unroll
+  for (int v = 0; v < N; ++v) s[v] = warp_sum(lane < W ? red[turn][g * W + lane][v] : 0.f);
+  turn ^= 1;
+}
+
+__device__ __forceinline__ float total(F2 x) {
+  float a, b;
+  unpack(x, a, b);
+  return a + b;
+}
+
+template <typename T, int NV, int ROWS>
+__global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const LnArgs a, int TW) {
+  using R = Ring<T, NV, ROWS, 1>;
+  constexpr int VEC = R::VEC, H = VEC / 2;
+  extern __shared__ uint4 smem[];
+  __shared__ float red[2][kRingThreads / 32][ROWS];
+  R ring(smem, a, TW);
+  const int W = TW / 32;
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  const T* const op[1] = {static_cast<const T*>(a.x)};
+  const int64_t stride[1] = {a.x_stride};
+  const int64_t step = gridDim.x;
+  int64_t b = blockIdx.x;
+#pragma unroll
+  for (int s = 0; s < R::STAGES - 1; ++s) ring.issue(op, stride, b + s * step, s);
+  // Weight and bias of a thread's columns: in registers where they suffice, else read again (from L1).
+  constexpr bool KEEP = NV * VEC <= 8;
+  F2 wv[KEEP ? NV : 1][H], bv[KEEP ? NV : 1][H];
+  auto params = [&](int i) {
+    if (ring.column(i) < ring.D) {
+      load_param<VEC>(a.weight, ring.column(i), a.wdtype, 1.f, wv[KEEP ? i : 0]);
+      load_param<VEC>(a.bias, ring.column(i), a.wdtype, 0.f, bv[KEEP ? i : 0]);
+    }
+  };
+  if (KEEP) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) params(i);
+  }
+  const float inv_d = 1.f / (float)ring.D;
+  T* y = static_cast<T*>(a.y);
+  int stage = 0, turn = 0;
+  for (; b < ring.blocks; b += step) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(R::STAGES - 2) : "memory");
+    Pack<T, VEC> x[ROWS][NV];
+    float s[ROWS], q[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      F2 t = f2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        x[k][i] = ring.read(b, stage, k, i, 0);
+#pragma unroll
+        for (int e = 0; e < H; ++e) t = add2(t, pair_of(x[k][i], e));
+      }
+      s[k] = total(t);
+    }
+    ring.issue(op, stride, b + (R::STAGES - 1) * step, stage == 0 ? R::STAGES - 1 : stage - 1);
+    if (++stage == R::STAGES) stage = 0;
+    ring_sum(s, W, ring.g, red, turn);
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      s[k] *= inv_d;  // the mean
+      const F2 m = f2(-s[k], -s[k]);
+      F2 t = f2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (ring.column(i) < ring.D) {
+#pragma unroll
+          for (int e = 0; e < H; ++e) {
+            const F2 d = add2(pair_of(x[k][i], e), m);
+            t = fma2(d, d, t);
+          }
+        }
+      q[k] = total(t);
+    }
+    ring_sum(q, W, ring.g, red, turn);
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      q[k] = 1.f / sqrtf(q[k] * inv_d + a.eps);  // the reciprocal deviation
+      const int64_t r = ring.row(b, k);
+      if (ring.in == 0 && r < a.rows && a.mean != nullptr) {
+        a.mean[r] = s[k];
+        a.rstd[r] = q[k];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = ring.column(i);
+      if (c >= ring.D) break;
+      if (!KEEP) params(i);
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) {
+        const int64_t r = ring.row(b, k);
+        if (r >= a.rows) break;
+        const F2 m = f2(-s[k], -s[k]), rs = f2(q[k], q[k]);
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int e = 0; e < H; ++e)
+          set_pair(o, e, fma2(mul2(add2(pair_of(x[k][i], e), m), rs), wv[KEEP ? i : 0][e], bv[KEEP ? i : 0][e]));
+        store_pack<T, VEC>(y + r * ring.D + c, o);
+      }
+    }
+  }
+}
+
+template <typename T, int NV, int ROWS>
+__global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const LnArgs a, int TW) {
+  using R = Ring<T, NV, ROWS, 2>;
+  constexpr int VEC = R::VEC, H = VEC / 2;
+  extern __shared__ uint4 smem[];
+  __shared__ float red[2][kRingThreads / 32][2 * ROWS];
+  R ring(smem, a, TW);
+  const int W = TW / 32, D = ring.D;
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  const T* const op[2] = {static_cast<const T*>(a.x), static_cast<const T*>(a.dy)};
+  const int64_t stride[2] = {a.x_stride, a.dy_stride};
+  const int64_t step = gridDim.x;
+  int64_t b = blockIdx.x;
+#pragma unroll
+  for (int s = 0; s < R::STAGES - 1; ++s) ring.issue(op, stride, b + s * step, s);
+  constexpr bool KEEP = NV * VEC <= 8;
+  F2 wv[KEEP ? NV : 1][H], dw[NV][H], db[NV][H];
+  auto weight = [&](int i) {
+    if (ring.column(i) < D) {
+      load_param<VEC>(a.weight, ring.column(i), a.wdtype, 1.f, wv[KEEP ? i : 0]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < H; ++e) wv[KEEP ? i : 0][e] = f2(0.f, 0.f);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (KEEP) weight(i);
+#pragma unroll
+    for (int e = 0; e < H; ++e) dw[i][e] = db[i][e] = f2(0.f, 0.f);
+  }
+  float mean[ROWS], rstd[ROWS];
+  auto stats = [&](int64_t block) {
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int64_t r = ring.row(block, k);
+      const bool ok = block < ring.blocks && r < a.rows;
+      mean[k] = ok ? a.mean[r] : 0.f;
+      rstd[k] = ok ? a.rstd[r] : 0.f;
+    }
+  };
+  stats(b);
+  const float inv_d = 1.f / (float)D;
+  T* dx = static_cast<T*>(a.y);
+  int stage = 0, turn = 0;
+  for (; b < ring.blocks; b += step) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(R::STAGES - 2) : "memory");
+    Pack<T, VEC> x[ROWS][NV], dy[ROWS][NV];
+    float m[ROWS], rs[ROWS], s[2 * ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      rs[k] = rstd[k];
+      m[k] = mean[k];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        x[k][i] = ring.read(b, stage, k, i, 0);
+        dy[k][i] = ring.read(b, stage, k, i, 1);
+      }
+    }
+    ring.issue(op, stride, b + (R::STAGES - 1) * step, stage == 0 ? R::STAGES - 1 : stage - 1);
+    stats(b + step);
+    if (++stage == R::STAGES) stage = 0;
+    F2 t0[ROWS], t1[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) t0[k] = t1[k] = f2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (!KEEP) weight(i);
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) {
+        const F2 nm = f2(-m[k], -m[k]), rr = f2(rs[k], rs[k]);
+#pragma unroll
+        for (int e = 0; e < H; ++e) {
+          const F2 h = mul2(add2(pair_of(x[k][i], e), nm), rr);
+          const F2 d = pair_of(dy[k][i], e);  // 0 past D and past the last row
+          const F2 gw = mul2(d, wv[KEEP ? i : 0][e]);
+          t0[k] = add2(t0[k], gw);
+          t1[k] = fma2(gw, h, t1[k]);
+          dw[i][e] = fma2(d, h, dw[i][e]);
+          db[i][e] = add2(db[i][e], d);
+        }
+      }
+    }
+    if (a.y == nullptr) continue;
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      s[2 * k] = total(t0[k]);
+      s[2 * k + 1] = total(t1[k]);
+    }
+    ring_sum(s, W, ring.g, red, turn);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = ring.column(i);
+      if (c >= D) break;
+      if (!KEEP) weight(i);
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) {
+        const int64_t r = ring.row(b, k);
+        if (r >= a.rows) break;
+        const F2 nm = f2(-m[k], -m[k]), rr = f2(rs[k], rs[k]);
+        const F2 m1 = f2(-s[2 * k] * inv_d, -s[2 * k] * inv_d), m2 = f2(-s[2 * k + 1] * inv_d, -s[2 * k + 1] * inv_d);
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int e = 0; e < H; ++e) {
+          const F2 h = mul2(add2(pair_of(x[k][i], e), nm), rr);
+          const F2 gw = fma2(pair_of(dy[k][i], e), wv[KEEP ? i : 0][e], m1);
+          set_pair(o, e, mul2(fma2(h, m2, gw), rr));
+        }
+        store_pack<T, VEC>(dx + r * D + c, o);
+      }
+    }
+  }
+  if (a.part == nullptr) return;
+  // This CTA's column sums; groups add theirs up in shared memory (the ring's, whose copies are done).
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  F2* sums = reinterpret_cast<F2*>(smem);
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    auto& acc = which == 0 ? dw : db;
+    float* out = a.part + ((int64_t)which * gridDim.x + blockIdx.x) * D;
+    __syncthreads();
+    if (ring.g > 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = ring.column(i);
+        if (c >= D) break;
+#pragma unroll
+        for (int e = 0; e < H; ++e) sums[((ring.g - 1) * D + c) / 2 + e] = acc[i][e];
+      }
+    }
+    __syncthreads();
+    if (ring.g == 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = ring.column(i);
+        if (c >= D) break;
+#pragma unroll
+        for (int e = 0; e < H; ++e) {
+          F2 t = acc[i][e];
+          for (int k = 1; k < ring.groups; ++k) t = add2(t, sums[((k - 1) * D + c) / 2 + e]);
+          *reinterpret_cast<F2*>(out + c + 2 * e) = t;
+        }
+      }
+    }
+  }
+}
+
+// ---- backward, any rows
 template <typename T, int VEC, int NV, int THREADS>
 __global__ void __launch_bounds__(THREADS) ln_backward_kernel(const LnArgs a, int W, int groups) {
   extern __shared__ float sums[];  // groups > 1: [groups][D] column sums at the end
@@ -234,8 +559,8 @@ __global__ void __launch_bounds__(THREADS) ln_backward_kernel(const LnArgs a, in
   }
 }
 
-// dw[c] = sum_p part[0][p][c], db[c] = sum_p part[1][p][c]: 32 columns per CTA, 16 thread rows
-// that each add every 16th partial.
+// dw[c] = sum_p part[0][p][c], db[c] = sum_p part[1][p][c]: 32 columns per CTA, 32 thread rows
+// that each add every 32nd partial.
 __global__ void __launch_bounds__(32 * kSumRows) ln_sum_kernel(const LnArgs a, int parts) {
   __shared__ float s[kSumRows][33];
   ptx::griddep_wait();
@@ -378,10 +703,11 @@ struct Shape {
   int vec, nv, W, groups, threads;
 };
 
-// A row takes the fewest warps (a power of two) that hold it; short rows share a CTA of 8 warps.
-Shape shape_of(const LnArgs& a, bool backward) {
+// Backward of any rows: a row takes the fewest warps (a power of two) that hold it 16 values a lane;
+// short rows share a CTA of 8 warps.
+Shape backward_shape(const LnArgs& a, int vec) {
   Shape s;
-  s.vec = pack_elems(a, backward);
+  s.vec = vec;
   const int few = s.vec * 32 >= 256 ? s.vec : 4;  // values a lane when one warp can hold the row so
   const bool small = a.D <= 32 * few;
   s.nv = (small ? few : kLaneElems) / s.vec;
@@ -392,9 +718,25 @@ Shape shape_of(const LnArgs& a, bool backward) {
   return s;
 }
 
+// Forward: a row takes the fewest warps that hold it in up to 8 packs of 16 bytes (16 pairs, 32 single
+// values) a lane, so that few warps wait for one another; more of them while the rows alone do not fill the SMs.
+Shape forward_shape(const LnArgs& a) {
+  Shape s;
+  s.vec = pack_elems(a, false);
+  const int most = s.vec * (int)elem_bytes(a.dtype) == 16 ? 8 : s.vec == 2 ? 16 : 32;
+  const int64_t packs = ceil_div(a.D, 32 * s.vec);  // of a lane, with one warp
+  s.W = 1;
+  while (s.W * most < packs || (s.W < packs && s.W < 8 && a.rows * s.W < 8 * (int64_t)kSmCount)) s.W *= 2;
+  s.nv = 1;
+  while ((int64_t)s.nv * s.W < packs) s.nv *= 2;
+  s.groups = s.W < 4 ? 4 / s.W : 1;
+  s.threads = s.W * s.groups * 32;
+  return s;
+}
+
 // Calls f(T{}, vec, nv) with the instantiation of the shape.
 template <typename T, typename F>
-cudaError_t by_shape(const Shape& s, F f) {
+cudaError_t by_backward_shape(const Shape& s, F f) {
   constexpr int MAXV = 16 / sizeof(T);
   using std::integral_constant;
   if (s.vec == MAXV) {
@@ -411,6 +753,27 @@ cudaError_t by_shape(const Shape& s, F f) {
   return f(T{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
 }
 
+template <typename T, int VEC, int NV, typename F>
+cudaError_t by_forward_count(const Shape& s, F f) {
+  constexpr int most = VEC * sizeof(T) == 16 ? 8 : VEC == 2 ? 16 : 32;
+  if (s.nv <= NV) {
+    if (s.threads <= 256) return f(ln_forward_kernel<T, VEC, NV, 256>);
+    if constexpr (NV == most) return f(ln_forward_kernel<T, VEC, NV, 512>);  // only the longest rows
+  }
+  if constexpr (NV < most) return by_forward_count<T, VEC, NV * 2>(s, f);
+  return cudaErrorInvalidConfiguration;
+}
+
+template <typename T, typename F>
+cudaError_t by_forward_shape(const Shape& s, F f) {
+  constexpr int MAXV = 16 / sizeof(T);
+  if (s.vec == MAXV) return by_forward_count<T, MAXV, 1>(s, f);
+  if constexpr (sizeof(T) == 2) {
+    if (s.vec == 2) return by_forward_count<T, 2, 2>(s, f);
+  }
+  return by_forward_count<T, 1, 4>(s, f);
+}
+
 template <typename F>
 cudaError_t by_type(int dtype, F f) {
   if (dtype == LM_F32) return f(float{});
@@ -418,15 +781,59 @@ cudaError_t by_type(int dtype, F f) {
   return f(__half{});
 }
 
-// CTAs of the persistent backward grid, and so rows of partial sums: at most two per SM.
-int64_t reg_parts(int64_t rows, int64_t D) {
+// CTAs of the persistent backward grids, and so rows of partial sums, at most.
+int64_t reg_parts(int64_t rows) {
   const int64_t most = 2 * kSmCount;
   return rows < most ? (rows > 0 ? rows : 1) : most;
 }
 
+// Rows of whole 16-byte packs, up to 32 KB each, go through the ring: the fewest packs a thread.
+// The forward below so many values goes a row at a time: its CTAs then have a block or two each.
+constexpr int64_t kRingForwardMin = 2 * 1024 * 1024;
+bool ring_fits(const LnArgs& a, bool backward) {
+  const int64_t eb = (int64_t)elem_bytes(a.dtype);
+  return pack_elems(a, backward) * eb == 16 && a.D * eb <= 32768;
+}
+
+template <typename T>
+void ring_shape(const LnArgs& a, int* nv, int* TW) {
+  constexpr int VEC = 16 / sizeof(T);
+  *nv = 1;
+  while ((int64_t)*nv * VEC * kRingThreads < a.D) *nv *= 2;
+  *TW = 32;
+  while ((int64_t)*TW * *nv * VEC < a.D) *TW *= 2;
+}
+
+template <typename K>
+cudaError_t launch_ring(K k, const LnArgs& a, int TW, int rows, int* parts, cudaStream_t stream) {
+  const int64_t blocks = ceil_div(a.rows, (int64_t)(kRingThreads / TW) * rows);
+  *parts = (int)std::max<int64_t>(1, std::min<int64_t>(blocks, kSmCount));
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(k, dim3(*parts), dim3(kRingThreads), kRingBytes, stream, a, TW);
+}
+
+template <typename T>
+cudaError_t launch_ring_forward(const LnArgs& a, cudaStream_t stream) {
+  int nv, TW, parts;
+  ring_shape<T>(a, &nv, &TW);
+  if (nv == 1) return launch_ring(ln_ring_forward_kernel<T, 1, 4>, a, TW, 4, &parts, stream);
+  if (nv == 2) return launch_ring(ln_ring_forward_kernel<T, 2, 2>, a, TW, 2, &parts, stream);
+  return launch_ring(ln_ring_forward_kernel<T, 4, 1>, a, TW, 1, &parts, stream);
+}
+
+template <typename T>
+cudaError_t launch_ring_backward(const LnArgs& a, int* parts, cudaStream_t stream) {
+  int nv, TW;
+  ring_shape<T>(a, &nv, &TW);
+  if (nv == 1) return launch_ring(ln_ring_backward_kernel<T, 1, 2>, a, TW, 2, parts, stream);
+  if (nv == 2) return launch_ring(ln_ring_backward_kernel<T, 2, 2>, a, TW, 2, parts, stream);
+  return launch_ring(ln_ring_backward_kernel<T, 4, 1>, a, TW, 1, parts, stream);
+}
+
 }  // namespace
 
-int64_t ln_backward_parts(int64_t rows, int64_t D) { return reg_parts(rows, D); }
+int64_t ln_backward_parts(int64_t rows, int64_t D) { return reg_parts(rows); }
 
 cudaError_t launch_ln_forward(const LnArgs& a, cudaStream_t stream) {
   if (a.rows == 0 || a.D == 0) return cudaSuccess;
@@ -440,16 +847,14 @@ cudaError_t launch_ln_forward(const LnArgs& a, cudaStream_t stream) {
                    : (a.bias != nullptr ? ln_wide_forward_kernel<E, false, true> : ln_wide_forward_kernel<E, false, false>);
       return launch_kernel(k, dim3(grid), dim3(kWideThreads), 0, stream, a);
     });
+  } else if (ring_fits(a, false) && a.rows * a.D >= kRingForwardMin) {
+    e = by_type(a.dtype, [&](auto t) { return launch_ring_forward<decltype(t)>(a, stream); });
   } else {
-    const Shape s = shape_of(a, false);
+    const Shape s = forward_shape(a);
+    const unsigned grid = (unsigned)ceil_div(a.rows, s.groups);
     e = by_type(a.dtype, [&](auto t) {
-      return by_shape<decltype(t)>(s, [&](auto tt, auto vec, auto nv) {
-        auto k = ln_forward_kernel<decltype(tt), decltype(vec)::value, decltype(nv)::value>;
-        const int64_t ctas = ceil_div(a.rows, s.groups);
-        int per_sm = 1536 / s.threads;
-        if (per_sm < 1) per_sm = 1;
-        const int64_t most = (int64_t)per_sm * device_sm_count();
-        return launch_kernel(k, dim3((unsigned)(ctas < most ? ctas : most)), dim3(s.threads), 0, stream, a, s.W, s.groups);
+      return by_forward_shape<decltype(t)>(s, [&](auto k) {
+        return launch_kernel(k, dim3(grid), dim3(s.threads), 0, stream, a, s.W, s.groups);
       });
     });
   }
@@ -465,7 +870,7 @@ cudaError_t launch_ln_backward(const LnArgs& a, cudaStream_t stream) {
   if (a.rows == 0 && !sums) return cudaSuccess;
   LnArgs b = a;
   if (!sums) b.part = nullptr;
-  const int parts = (int)reg_parts(a.rows, a.D);
+  int parts = (int)reg_parts(a.rows);
   cudaError_t e = cudaSuccess;
   int launches = 0;
   if (a.D > kMaxRegD) {
@@ -484,10 +889,13 @@ cudaError_t launch_ln_backward(const LnArgs& a, cudaStream_t stream) {
       });
       ++launches;
     }
+  } else if (ring_fits(a, true)) {
+    e = by_type(a.dtype, [&](auto t) { return launch_ring_backward<decltype(t)>(b, &parts, stream); });
+    ++launches;
   } else {
-    const Shape s = shape_of(a, true);
+    const Shape s = backward_shape(a, pack_elems(a, true));
     e = by_type(a.dtype, [&](auto t) {
-      return by_shape<decltype(t)>(s, [&](auto tt, auto vec, auto nv) {
+      return by_backward_shape<decltype(t)>(s, [&](auto tt, auto vec, auto nv) {
         const size_t smem = s.groups > 1 && sums ? sizeof(float) * s.groups * a.D : 0;
         auto go = [&](auto k) {
           return launch_kernel(k, dim3(parts), dim3(s.threads), smem, stream, b, s.W, s.groups);
