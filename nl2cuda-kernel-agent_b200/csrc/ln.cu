@@ -135,70 +135,119 @@ __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// OPS operands (x; or x and dy) of ROWS rows a block.
+// OPS operands (x; or x and dy) of ROWS rows a block.  Pointers move from block to block: addresses made
+// anew from row and stride took more instructions than the arithmetic.
 template <typename T, int NV, int ROWS, int OPS>
 struct Ring {
   static constexpr int VEC = 16 / sizeof(T);
   static constexpr int kPieces = ROWS * NV * OPS;  // 16-byte pieces of a thread and block
   static constexpr int kFit = (int)(kRingBytes / (kPieces * 16 * kRingThreads));
   static constexpr int STAGES = kFit > 8 ? 8 : kFit;
+  static constexpr uint32_t kPiece = 16 * kRingThreads, kStage = kPieces * kPiece;
   static_assert(STAGES >= 3, "ring");
-  uint4* ring;  // [STAGES][kPieces][kRingThreads]
-  int TW, groups, g, in, D;
-  int64_t rows, per_block, blocks;
-  __device__ __forceinline__ Ring(uint4* smem, const LnArgs& a, int tw) : ring(smem), TW(tw), rows(a.rows) {
-    groups = kRingThreads / TW;
+  int g, in, D, pitch;      // pitch: elements between a thread's packs
+  unsigned columns;         // bit i: pack i lies inside the row
+  int64_t row, step;        // first row of this group's present block, rows from one block to the next
+  uint32_t base;            // this thread's slots
+  const T* next[OPS];       // this thread's first pack of the next block to copy
+  int64_t stride[OPS], hop[OPS];
+  int64_t next_row;
+  int in_stage, out_stage;
+
+  __device__ __forceinline__ Ring(void* smem, const LnArgs& a, int TW, const T* const (&op)[OPS], const int64_t (&st)[OPS]) {
+    const int groups = kRingThreads / TW;
     g = threadIdx.x / TW;
     in = threadIdx.x - g * TW;
     D = (int)a.D;
-    per_block = (int64_t)groups * ROWS;
-    blocks = (rows + per_block - 1) / per_block;
+    pitch = TW * VEC;
+    columns = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) columns |= (i * pitch + in * VEC < D ? 1u : 0u) << i;
+    step = (int64_t)gridDim.x * groups * ROWS;
+    row = next_row = ((int64_t)blockIdx.x * groups + g) * ROWS;
+    base = ptx::smem_u32(smem) + threadIdx.x * 16;
+#pragma unroll
+    for (int o = 0; o < OPS; ++o) {
+      stride[o] = st[o];
+      hop[o] = step * st[o];
+      next[o] = op[o] + row * st[o] + in * VEC;
+    }
+    in_stage = out_stage = 0;
   }
-  __device__ __forceinline__ int column(int i) const { return (i * TW + in) * VEC; }
-  __device__ __forceinline__ int64_t row(int64_t block, int k) const { return block * per_block + g * ROWS + k; }
-  __device__ __forceinline__ void issue(const T* const (&op)[OPS], const int64_t (&stride)[OPS], int64_t block, int stage) {
-    if (block < blocks) {
+  // How many of this group's ROWS rows from r on there are.
+  __device__ __forceinline__ int left(int64_t r, int64_t rows) const {
+    const int64_t n = rows - r;
+    return n >= ROWS ? ROWS : n > 0 ? (int)n : 0;
+  }
+  __device__ __forceinline__ void issue(int64_t rows) {
+    const int n = left(next_row, rows);
+    const uint32_t at = base + in_stage * kStage;
+#pragma unroll
+    for (int o = 0; o < OPS; ++o) {
+      const T* p = next[o];
 #pragma unroll
       for (int k = 0; k < ROWS; ++k) {
-        const int64_t r = row(block, k);
-        if (r < rows) {
+        if (k < n) {
 #pragma unroll
           for (int i = 0; i < NV; ++i)
-            if (column(i) < D) {
-#pragma unroll
-              for (int o = 0; o < OPS; ++o)
-                copy_async16(ptx::smem_u32(ring + (stage * kPieces + (k * NV + i) * OPS + o) * kRingThreads + threadIdx.x),
-                             op[o] + r * stride[o] + column(i));
-            }
+            if (columns >> i & 1u) copy_async16(at + ((k * NV + i) * OPS + o) * kPiece, p + i * pitch);
         }
+        p += stride[o];
       }
+      next[o] += hop[o];
     }
+    next_row += step;
+    if (++in_stage == STAGES) in_stage = 0;
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  // Piece (row k, pack i, operand o) of the block in `stage`; zeros outside the matrix.
-  __device__ __forceinline__ Pack<T, VEC> read(int64_t block, int stage, int k, int i, int o) const {
+  // Piece (row k, pack i, operand o) of the present block; zeros outside the matrix.
+  __device__ __forceinline__ Pack<T, VEC> read(int n, int k, int i, int o) const {
     Pack<T, VEC> p;
     uint4 u = make_uint4(0, 0, 0, 0);
-    if (row(block, k) < rows && column(i) < D) u = ring[(stage * kPieces + (k * NV + i) * OPS + o) * kRingThreads + threadIdx.x];
+    if (k < n && (columns >> i & 1u))
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                   : "r"(base + out_stage * kStage + ((k * NV + i) * OPS + o) * kPiece));
     *reinterpret_cast<uint4*>(&p) = u;
     return p;
   }
+  __device__ __forceinline__ void advance() {
+    row += step;
+    if (++out_stage == STAGES) out_stage = 0;
+  }
 };
 
-// Sums of N values over a group's threads.  red: [2][warps of the CTA][N], used in turn.
+// Sums of N values (a power of two) over a group's W warps.  In a warp each step hands half of the
+// values to the other half of the lanes, so that N values take N + 5 - log2 N exchanges in place of
+// 5 N.  red: [2][warps of the CTA][N], used in turn, so that one barrier is enough.
 template <int N>
 __device__ __forceinline__ void ring_sum(float (&s)[N], int W, int g, float (*red)[kRingThreads / 32][N], int& turn) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int v = 0;
 #pragma unroll
-  for (int v = 0; v < N; ++v) s[v] = warp_sum(s[v]);
-  if (W == 1) return;
-  if (lane == 0) {
+  for (int n = N / 2, o = 1; o < 32; n >>= 1, o <<= 1) {
+    if (n > 0) {
+      const bool up = lane & o;
+      v = 2 * v + (up ? 1 : 0);
 #pragma unroll
-    for (int v = 0; v < N; ++v) red[turn][warp][v] = s[v];
+      for (int i = 0; i < n; ++i) {
+        const float send = up ? s[i] : s[i + n], keep = up ? s[i + n] : s[i];
+        s[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+      }
+    } else {
+      s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+    }
   }
-  named_sync(1 + g, W * 32);
+  // This lane holds the warp's sum of value v.
+  if (lane < N) red[turn][warp][v] = s[0];
+  if (W == 1) __syncwarp();
+  else named_sync(1 + g, W * 32);
+  const float* r = red[turn][g * W + (lane & (W - 1))];
 #pragma unroll
-  for (int v = 0; v < N; ++v) s[v] = warp_sum(lane < W ? red[turn][g * W + lane][v] : 0.f);
+  for (int i = 0; i < N; ++i) s[i] = r[i];
+  for (int o = 1; o < W; o <<= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+  }
   turn ^= 1;
 }
 
@@ -207,6 +256,7 @@ __device__ __forceinline__ float total(F2 x) {
   unpack(x, a, b);
   return a + b;
 }
+__device__ __forceinline__ F2 twice(float x) { return f2(x, x); }
 
 template <typename T, int NV, int ROWS>
 __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const LnArgs a, int TW) {
@@ -214,23 +264,21 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const 
   constexpr int VEC = R::VEC, H = VEC / 2;
   extern __shared__ uint4 smem[];
   __shared__ float red[2][kRingThreads / 32][ROWS];
-  R ring(smem, a, TW);
-  const int W = TW / 32;
-  ptx::griddep_wait();
-  ptx::griddep_launch_dependents();
   const T* const op[1] = {static_cast<const T*>(a.x)};
   const int64_t stride[1] = {a.x_stride};
-  const int64_t step = gridDim.x;
-  int64_t b = blockIdx.x;
+  R ring(smem, a, TW, op, stride);
+  const int W = TW / 32, first = ring.in * VEC;
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
 #pragma unroll
-  for (int s = 0; s < R::STAGES - 1; ++s) ring.issue(op, stride, b + s * step, s);
+  for (int s = 0; s < R::STAGES - 1; ++s) ring.issue(a.rows);
   // Weight and bias of a thread's columns: in registers where they suffice, else read again (from L1).
   constexpr bool KEEP = NV * VEC <= 8;
   F2 wv[KEEP ? NV : 1][H], bv[KEEP ? NV : 1][H];
   auto params = [&](int i) {
-    if (ring.column(i) < ring.D) {
-      load_param<VEC>(a.weight, ring.column(i), a.wdtype, 1.f, wv[KEEP ? i : 0]);
-      load_param<VEC>(a.bias, ring.column(i), a.wdtype, 0.f, bv[KEEP ? i : 0]);
+    if (ring.columns >> i & 1u) {
+      load_param<VEC>(a.weight, i * ring.pitch + first, a.wdtype, 1.f, wv[KEEP ? i : 0]);
+      load_param<VEC>(a.bias, i * ring.pitch + first, a.wdtype, 0.f, bv[KEEP ? i : 0]);
     }
   };
   if (KEEP) {
@@ -238,37 +286,46 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const 
     for (int i = 0; i < NV; ++i) params(i);
   }
   const float inv_d = 1.f / (float)ring.D;
-  T* y = static_cast<T*>(a.y);
-  int stage = 0, turn = 0;
-  for (; b < ring.blocks; b += step) {
+  T* y = static_cast<T*>(a.y) + ring.row * ring.D + first;
+  const int64_t y_hop = ring.step * ring.D;
+  int turn = 0;
+  // Values as they came (16 bits), or converted once where a thread holds few enough of them.
+  constexpr bool WIDE = NV * ROWS * VEC <= 32;
+  for (; ring.row < a.rows; ring.advance(), y += y_hop) {
     asm volatile("cp.async.wait_group %0;" ::"n"(R::STAGES - 2) : "memory");
+    const int n = ring.left(ring.row, a.rows);
     Pack<T, VEC> x[ROWS][NV];
+    F2 xw[WIDE ? ROWS : 1][WIDE ? NV : 1][H] = {};
     float s[ROWS], q[ROWS];
+    auto value = [&](int k, int i, int e) { return WIDE ? xw[WIDE ? k : 0][WIDE ? i : 0][e] : pair_of(x[k][i], e); };
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-      F2 t = f2(0.f, 0.f);
+      F2 t = twice(0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        x[k][i] = ring.read(b, stage, k, i, 0);
+        x[k][i] = ring.read(n, k, i, 0);
 #pragma unroll
-        for (int e = 0; e < H; ++e) t = add2(t, pair_of(x[k][i], e));
+        for (int e = 0; e < H; ++e) {
+          if (WIDE) xw[WIDE ? k : 0][WIDE ? i : 0][e] = pair_of(x[k][i], e);
+          t = add2(t, value(k, i, e));
+        }
       }
       s[k] = total(t);
     }
-    ring.issue(op, stride, b + (R::STAGES - 1) * step, stage == 0 ? R::STAGES - 1 : stage - 1);
-    if (++stage == R::STAGES) stage = 0;
+    ring.issue(a.rows);
     ring_sum(s, W, ring.g, red, turn);
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
       s[k] *= inv_d;  // the mean
-      const F2 m = f2(-s[k], -s[k]);
-      F2 t = f2(0.f, 0.f);
+      const F2 m = twice(-s[k]);
+      F2 t = twice(0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (ring.column(i) < ring.D) {
+        if (ring.columns >> i & 1u) {
 #pragma unroll
           for (int e = 0; e < H; ++e) {
-            const F2 d = add2(pair_of(x[k][i], e), m);
+            const F2 d = add2(value(k, i, e), m);
+            if (WIDE) xw[WIDE ? k : 0][WIDE ? i : 0][e] = d;
             t = fma2(d, d, t);
           }
         }
@@ -278,27 +335,27 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const 
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
       q[k] = 1.f / sqrtf(q[k] * inv_d + a.eps);  // the reciprocal deviation
-      const int64_t r = ring.row(b, k);
-      if (ring.in == 0 && r < a.rows && a.mean != nullptr) {
-        a.mean[r] = s[k];
-        a.rstd[r] = q[k];
+      if (ring.in == 0 && k < n && a.mean != nullptr) {
+        a.mean[ring.row + k] = s[k];
+        a.rstd[ring.row + k] = q[k];
       }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = ring.column(i);
-      if (c >= ring.D) break;
+      if (!(ring.columns >> i & 1u)) break;
       if (!KEEP) params(i);
+      T* out = y + i * ring.pitch;
 #pragma unroll
       for (int k = 0; k < ROWS; ++k) {
-        const int64_t r = ring.row(b, k);
-        if (r >= a.rows) break;
-        const F2 m = f2(-s[k], -s[k]), rs = f2(q[k], q[k]);
+        const F2 m = twice(-s[k]), rs = twice(q[k]);
         Pack<T, VEC> o;
 #pragma unroll
-        for (int e = 0; e < H; ++e)
-          set_pair(o, e, fma2(mul2(add2(pair_of(x[k][i], e), m), rs), wv[KEEP ? i : 0][e], bv[KEEP ? i : 0][e]));
-        store_pack<T, VEC>(y + r * ring.D + c, o);
+        for (int e = 0; e < H; ++e) {
+          const F2 d = WIDE ? value(k, i, e) : add2(value(k, i, e), m);
+          set_pair(o, e, fma2(mul2(d, rs), wv[KEEP ? i : 0][e], bv[KEEP ? i : 0][e]));
+        }
+        if (k < n) store_pack<T, VEC>(out, o);
+        out += ring.D;
       }
     }
   }
@@ -310,75 +367,72 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
   constexpr int VEC = R::VEC, H = VEC / 2;
   extern __shared__ uint4 smem[];
   __shared__ float red[2][kRingThreads / 32][2 * ROWS];
-  R ring(smem, a, TW);
-  const int W = TW / 32, D = ring.D;
-  ptx::griddep_wait();
-  ptx::griddep_launch_dependents();
   const T* const op[2] = {static_cast<const T*>(a.x), static_cast<const T*>(a.dy)};
   const int64_t stride[2] = {a.x_stride, a.dy_stride};
-  const int64_t step = gridDim.x;
-  int64_t b = blockIdx.x;
+  R ring(smem, a, TW, op, stride);
+  const int W = TW / 32, D = ring.D, first = ring.in * VEC;
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
 #pragma unroll
-  for (int s = 0; s < R::STAGES - 1; ++s) ring.issue(op, stride, b + s * step, s);
+  for (int s = 0; s < R::STAGES - 1; ++s) ring.issue(a.rows);
   constexpr bool KEEP = NV * VEC <= 8;
   F2 wv[KEEP ? NV : 1][H], dw[NV][H], db[NV][H];
   auto weight = [&](int i) {
-    if (ring.column(i) < D) {
-      load_param<VEC>(a.weight, ring.column(i), a.wdtype, 1.f, wv[KEEP ? i : 0]);
+    if (ring.columns >> i & 1u) {
+      load_param<VEC>(a.weight, i * ring.pitch + first, a.wdtype, 1.f, wv[KEEP ? i : 0]);
     } else {
 #pragma unroll
-      for (int e = 0; e < H; ++e) wv[KEEP ? i : 0][e] = f2(0.f, 0.f);
+      for (int e = 0; e < H; ++e) wv[KEEP ? i : 0][e] = twice(0.f);
     }
   };
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     if (KEEP) weight(i);
 #pragma unroll
-    for (int e = 0; e < H; ++e) dw[i][e] = db[i][e] = f2(0.f, 0.f);
+    for (int e = 0; e < H; ++e) dw[i][e] = db[i][e] = twice(0.f);
   }
   float mean[ROWS], rstd[ROWS];
-  auto stats = [&](int64_t block) {
+  auto stats = [&](int64_t r) {
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-      const int64_t r = ring.row(block, k);
-      const bool ok = block < ring.blocks && r < a.rows;
-      mean[k] = ok ? a.mean[r] : 0.f;
-      rstd[k] = ok ? a.rstd[r] : 0.f;
+      mean[k] = r + k < a.rows ? a.mean[r + k] : 0.f;
+      rstd[k] = r + k < a.rows ? a.rstd[r + k] : 0.f;
     }
   };
-  stats(b);
+  stats(ring.row);
   const float inv_d = 1.f / (float)D;
-  T* dx = static_cast<T*>(a.y);
-  int stage = 0, turn = 0;
-  for (; b < ring.blocks; b += step) {
+  T* dx = static_cast<T*>(a.y) + ring.row * D + first;
+  const int64_t dx_hop = ring.step * D;
+  int turn = 0;
+  for (; ring.row < a.rows; ring.advance(), dx += dx_hop) {
     asm volatile("cp.async.wait_group %0;" ::"n"(R::STAGES - 2) : "memory");
+    const int n = ring.left(ring.row, a.rows);
     Pack<T, VEC> x[ROWS][NV], dy[ROWS][NV];
-    float m[ROWS], rs[ROWS], s[2 * ROWS];
+    float s[2 * ROWS];
+    F2 shift[ROWS], rs[ROWS];
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-      rs[k] = rstd[k];
-      m[k] = mean[k];
+      rs[k] = twice(rstd[k]);
+      shift[k] = twice(-mean[k]);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        x[k][i] = ring.read(b, stage, k, i, 0);
-        dy[k][i] = ring.read(b, stage, k, i, 1);
+        x[k][i] = ring.read(n, k, i, 0);
+        dy[k][i] = ring.read(n, k, i, 1);
       }
     }
-    ring.issue(op, stride, b + (R::STAGES - 1) * step, stage == 0 ? R::STAGES - 1 : stage - 1);
-    stats(b + step);
-    if (++stage == R::STAGES) stage = 0;
+    ring.issue(a.rows);
+    stats(ring.row + ring.step);
     F2 t0[ROWS], t1[ROWS];
 #pragma unroll
-    for (int k = 0; k < ROWS; ++k) t0[k] = t1[k] = f2(0.f, 0.f);
+    for (int k = 0; k < ROWS; ++k) t0[k] = t1[k] = twice(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (!KEEP) weight(i);
 #pragma unroll
-      for (int k = 0; k < ROWS; ++k) {
-        const F2 nm = f2(-m[k], -m[k]), rr = f2(rs[k], rs[k]);
+      for (int k = 0; k < ROWS; ++k)
 #pragma unroll
         for (int e = 0; e < H; ++e) {
-          const F2 h = mul2(add2(pair_of(x[k][i], e), nm), rr);
+          const F2 h = mul2(add2(pair_of(x[k][i], e), shift[k]), rs[k]);
           const F2 d = pair_of(dy[k][i], e);  // 0 past D and past the last row
           const F2 gw = mul2(d, wv[KEEP ? i : 0][e]);
           t0[k] = add2(t0[k], gw);
@@ -386,7 +440,6 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
           dw[i][e] = fma2(d, h, dw[i][e]);
           db[i][e] = add2(db[i][e], d);
         }
-      }
     }
     if (a.y == nullptr) continue;
 #pragma unroll
@@ -397,29 +450,28 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
     ring_sum(s, W, ring.g, red, turn);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = ring.column(i);
-      if (c >= D) break;
+      if (!(ring.columns >> i & 1u)) break;
       if (!KEEP) weight(i);
+      T* out = dx + i * ring.pitch;
 #pragma unroll
       for (int k = 0; k < ROWS; ++k) {
-        const int64_t r = ring.row(b, k);
-        if (r >= a.rows) break;
-        const F2 nm = f2(-m[k], -m[k]), rr = f2(rs[k], rs[k]);
-        const F2 m1 = f2(-s[2 * k] * inv_d, -s[2 * k] * inv_d), m2 = f2(-s[2 * k + 1] * inv_d, -s[2 * k + 1] * inv_d);
+        const F2 m1 = twice(-s[2 * k] * inv_d), m2 = twice(-s[2 * k + 1] * inv_d);
         Pack<T, VEC> o;
 #pragma unroll
         for (int e = 0; e < H; ++e) {
-          const F2 h = mul2(add2(pair_of(x[k][i], e), nm), rr);
+          const F2 h = mul2(add2(pair_of(x[k][i], e), shift[k]), rs[k]);
           const F2 gw = fma2(pair_of(dy[k][i], e), wv[KEEP ? i : 0][e], m1);
-          set_pair(o, e, mul2(fma2(h, m2, gw), rr));
+          set_pair(o, e, mul2(fma2(h, m2, gw), rs[k]));
         }
-        store_pack<T, VEC>(dx + r * D + c, o);
+        if (k < n) store_pack<T, VEC>(out, o);
+        out += D;
       }
     }
   }
   if (a.part == nullptr) return;
   // This CTA's column sums; groups add theirs up in shared memory (the ring's, whose copies are done).
   asm volatile("cp.async.wait_group 0;" ::: "memory");
+  const int groups = kRingThreads / TW;
   F2* sums = reinterpret_cast<F2*>(smem);
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
@@ -429,22 +481,21 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
     if (ring.g > 0) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = ring.column(i);
-        if (c >= D) break;
+        if (!(ring.columns >> i & 1u)) break;
 #pragma unroll
-        for (int e = 0; e < H; ++e) sums[((ring.g - 1) * D + c) / 2 + e] = acc[i][e];
+        for (int e = 0; e < H; ++e) sums[((ring.g - 1) * D + i * ring.pitch + first) / 2 + e] = acc[i][e];
       }
     }
     __syncthreads();
     if (ring.g == 0) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = ring.column(i);
-        if (c >= D) break;
+        if (!(ring.columns >> i & 1u)) break;
+        const int c = i * ring.pitch + first;
 #pragma unroll
         for (int e = 0; e < H; ++e) {
           F2 t = acc[i][e];
-          for (int k = 1; k < ring.groups; ++k) t = add2(t, sums[((k - 1) * D + c) / 2 + e]);
+          for (int k = 1; k < groups; ++k) t = add2(t, sums[((k - 1) * D + c) / 2 + e]);
           *reinterpret_cast<F2*>(out + c + 2 * e) = t;
         }
       }
@@ -795,10 +846,10 @@ bool ring_fits(const LnArgs& a, bool backward) {
   return pack_elems(a, backward) * eb == 16 && a.D * eb <= 32768;
 }
 
+// `nv` packs a thread or as many more as 512 threads need, and the threads of a row.
 template <typename T>
 void ring_shape(const LnArgs& a, int* nv, int* TW) {
   constexpr int VEC = 16 / sizeof(T);
-  *nv = 1;
   while ((int64_t)*nv * VEC * kRingThreads < a.D) *nv *= 2;
   *TW = 32;
   while ((int64_t)*TW * *nv * VEC < a.D) *TW *= 2;
@@ -813,21 +864,26 @@ cudaError_t launch_ring(K k, const LnArgs& a, int TW, int rows, int* parts, cuda
   return launch_kernel(k, dim3(*parts), dim3(kRingThreads), kRingBytes, stream, a, TW);
 }
 
+// Four rows a block, since each block costs two reductions and their barriers: 8192 x 4096 bf16 in 33 us
+// with two packs a thread and four rows, 54 us with one row, 38 us with one pack (and 512 threads that
+// wait for each other) and four rows.
 template <typename T>
 cudaError_t launch_ring_forward(const LnArgs& a, cudaStream_t stream) {
-  int nv, TW, parts;
+  int nv = a.D > 32 * (16 / (int64_t)sizeof(T)) ? 2 : 1, TW, parts;
   ring_shape<T>(a, &nv, &TW);
   if (nv == 1) return launch_ring(ln_ring_forward_kernel<T, 1, 4>, a, TW, 4, &parts, stream);
-  if (nv == 2) return launch_ring(ln_ring_forward_kernel<T, 2, 2>, a, TW, 2, &parts, stream);
-  return launch_ring(ln_ring_forward_kernel<T, 4, 1>, a, TW, 1, &parts, stream);
+  if (nv == 2) return launch_ring(ln_ring_forward_kernel<T, 2, 4>, a, TW, 4, &parts, stream);
+  return launch_ring(ln_ring_forward_kernel<T, 4, 2>, a, TW, 2, &parts, stream);
 }
 
+// One pack a thread and two rows: 48 us at that size; one row took 57 us, and two packs or four rows
+// do not fit the registers next to the column sums (70 us and more).
 template <typename T>
 cudaError_t launch_ring_backward(const LnArgs& a, int* parts, cudaStream_t stream) {
-  int nv, TW;
+  int nv = 1, TW;
   ring_shape<T>(a, &nv, &TW);
   if (nv == 1) return launch_ring(ln_ring_backward_kernel<T, 1, 2>, a, TW, 2, parts, stream);
-  if (nv == 2) return launch_ring(ln_ring_backward_kernel<T, 2, 2>, a, TW, 2, parts, stream);
+  if (nv == 2) return launch_ring(ln_ring_backward_kernel<T, 2, 1>, a, TW, 1, parts, stream);
   return launch_ring(ln_ring_backward_kernel<T, 4, 1>, a, TW, 1, parts, stream);
 }
 
