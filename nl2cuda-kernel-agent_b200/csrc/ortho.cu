@@ -23,8 +23,9 @@
 // The tensor core truncates each addition to its fp32 accumulator, so a long sum of one sign comes out
 // low by half a unit per MMA: 1.8e-5 of the result at a depth of 2601.  So an accumulator takes a
 // run of slices only, and the epilogue warps add these partial sums in registers, rounded to nearest.
-// A run is 256 deep for fp32 results (error 4.8e-6 there, the fp32 library product's is 3.3e-6), 1024
-// for fp16 and 2048 for bf16, whose own rounding is far larger: short runs cost up to 9% of the time.
+// The products with lo, two thirds of the MMAs but 2^-11 of the sum, go to an accumulator of their own
+// where there is room for one.  A run is 256 deep for fp32 results, 1024 for fp16 and 2048 for bf16, whose
+// own rounding is far larger: short runs cost up to 9% of the time.
 //
 // Kernel: one launch runs the whole iteration (cooperative, one CTA per SM).  A product's tiles are
 // shared out over the CTA pairs; each CTA counts itself in when its part is stored, and the loads of
@@ -60,57 +61,56 @@ static_assert(kRegsLow + 2 * kRegsHigh <= 3 * kRegs && kThreads == 384, "registe
 constexpr size_t kSmemMax = 232448;
 constexpr int kTurnWords = 32 * 32;             // an epilogue warp's block in shared memory
 
-// Scale factors of one step of one matrix (see scale_table).
-struct StepScale {
-  float gram;             // A      from the accumulator of X X^T
-  float square, linear;   // B      from the accumulator of A^2, and from A
-  float product, keep;    // X_next from the accumulator of B X, and from X
-};
-
 enum { kSymmetric = 0, kBoth = 1, kFinal = 2 };
 
-// One product D = P Q^T of every matrix of the batch.
-struct GemmArgs {
-  int64_t M, N;             // D [M, N] per matrix
-  int tiles;                // of one matrix
-  int tiles_m, tiles_n;
-  int num_kc;               // slices of the depth
-  int out_kind;             // kSymmetric, kBoth, kFinal
-  int kind;                 // of the scales: 0 gram, 1 square, 2 product
-  int out_dtype;
-  // D = alpha * accumulator + beta * (add_hi + add_lo), alpha and beta from the scale table
-  const __half* add_hi;     // row-major [M, ld_d] (NULL: no addend)
-  const __half* add_lo;
-  __half* d_hi;             // row-major [M, ld_d]
-  __half* d_lo;
-  __half* t_hi;             // transposed [N, ld_t]; pitches are multiples of 32
-  __half* t_lo;
-  int64_t ld_d, ld_t, d_matrix, t_matrix;  // strides of rows and of matrices, in elements
-  void* out;                // kFinal: out[col * ld_out + row], type out_dtype
-  int64_t ld_out, out_matrix;
+// The matrices of an iteration, and the products D = P Q^T it is made of.  A group of steps is
+//   A = X X^T,  Q = a + b A + c A^2                                     kGram, kSquare
+//   and for every further step of the group, with P the last polynomial (P = Q at first):
+//     T = A P,  A = T P                     (the next X X^T)            kTimes, kAgain
+//     P = a + b A + c A^2,  Q = P Q                                     kSquare, kChain
+//   X = Q X                                                             kApply
+// For fp32 results every step is a group, Q leaves the identity out (Q = b A + c A^2) and X = a X + Q X:
+// in the full polynomial the terms of Q X cancel, whose rounding is 3 times the fp32 library product's
+// error, and 1 / 50 of what rounding the result to 16 bits takes.
+enum { mX, mXT0, mXT1, mA, mT, mP, mQ0, mQ1, kMatrices };
+enum { kGram, kSquare, kTimes, kAgain, kChain, kApply };
+constexpr int kMaxSteps = 32;
+constexpr int kMaxOps = 4 * kMaxSteps;  // 11 products for a group of three steps, 3 for a single one
+constexpr int kNone = kMatrices;        // no addend
+
+// hi and lo of one matrix per batch entry, row-major.
+struct Split {
+  __half* hi;
+  __half* lo;
+  int64_t rows, cols, ld, matrix;  // strides of rows (a multiple of 32) and of matrices, in elements
 };
 
-// The whole iteration: for each step gram, square and one of the two products (X^T alternates
-// between two buffers), the last step's being `final`.
-enum { kGram = 0, kSquare = 1, kProduct = 2, kLast = 4, kProducts = 5 };
+struct Op {
+  uint8_t kind, p, q, d, t, add;  // matrices: the operands, where D and its transpose go, what is added
+  uint8_t out_kind;
+  int tiles;                      // of one matrix of the batch
+};
+
+// Factors of one product of one batch entry: D = acc * (accumulator) + add * addend + diagonal * I.
+struct Scale {
+  float acc, add, diagonal;
+};
+
 struct IterArgs {
-  CUtensorMap map[kProducts][4];  // P hi, P lo, Q hi, Q lo
-  GemmArgs gemm[kProducts];
-  const StepScale* scale;         // [batch][steps]
+  CUtensorMap as_p[kMatrices][2], as_q[kMatrices][2];  // hi, lo; boxes of a CTA's rows of either operand
+  Split mat[kMatrices];
+  Op op[kMaxOps];
+  int ops, batch;
+  int run;                        // slices that share a TMEM accumulator
+  int out_dtype;
+  void* out;                      // of the last product: out[column * ld_out + row]
+  int64_t ld_out, out_matrix;
+  const Scale* scale;             // [batch][ops]
   unsigned* arrived;              // CTAs that have finished a product, counted over all products
   int* status;
   unsigned long long timeout_ns;
-  int steps, batch;
-  int run;                        // slices that share a TMEM accumulator
   int debug_skip_first_load;
 };
-static_assert(sizeof(IterArgs) <= 4096, "kernel parameters");
-
-__device__ __forceinline__ int product_index(int p, int steps) {
-  const int step = p / 3, w = p - 3 * step;
-  if (w < 2) return w;
-  return step + 1 == steps ? kLast : kProduct + (step & 1);
-}
 
 // Wait (bounded) until `want` CTAs have arrived; what they wrote before is visible after it.
 // `pause`: between polls, where nothing hangs on the first moment.
@@ -178,7 +178,10 @@ struct Plan {
   static constexpr size_t FIXED = 1024 + 256 + sizeof(uint32_t) * kEpiWarps * kTurnWords;
   static constexpr int STAGES = (int)((kSmemMax - FIXED) / STAGE);
   static constexpr size_t SMEM = FIXED + (size_t)STAGES * STAGE;
-  static constexpr uint32_t TCOLS = 2 * BN;
+  // Two accumulators of ACC columns, one for the MMAs and one for the epilogue.  Where TMEM holds it (512
+  // columns), the hi x lo products have a part of their own (column BN on): see the truncation above.
+  static constexpr bool APART = BN <= 128;
+  static constexpr uint32_t ACC = APART ? 2 * BN : BN, TCOLS = 2 * ACC;
   static_assert(STAGES >= 2 && SMEM <= kSmemMax, "stages");
 };
 
@@ -213,8 +216,12 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
     *stored = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == 0 && lane < 4)
-    for (int p = 0; p < kProducts; ++p) ptx::prefetch_tensormap(&it.map[p][lane]);
+  if (warp == 0 && lane < kMatrices) {
+    for (int h = 0; h < 2; ++h) {
+      ptx::prefetch_tensormap(&it.as_p[lane][h]);
+      ptx::prefetch_tensormap(&it.as_q[lane][h]);
+    }
+  }
   ptx::cluster_sync();  // the peer's barriers exist before any remote arrive
   if (warp == 1) {
     ptx::tmem_alloc_pair(tmem_slot, P::TCOLS);
@@ -226,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
   const uint32_t tmem = *tmem_slot;
   const int unit = blockIdx.x >> 1;
   const int units = gridDim.x >> 1;
-  const int products = 3 * it.steps;
+  const int products = it.ops;
 
   if (warp < 4) {
     ptx::regs_shrink<kRegsLow>();
@@ -237,11 +244,12 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
         uint32_t phase = 0, issued = 0, last = 0;
         bool ok = true, skipped = false;
         for (int p = 0; p < products && ok; ++p) {
-          const int pi = product_index(p, it.steps);
-          const CUtensorMap* map = it.map[pi];
-          const int tiles = it.gemm[pi].tiles, num_kc = it.gemm[pi].num_kc, out_kind = it.gemm[pi].out_kind;
-          const int tiles_m = it.gemm[pi].tiles_m, tiles_n = it.gemm[pi].tiles_n;
-          const int total = tiles * it.batch;
+          const Op op = it.op[p];
+          const CUtensorMap *mp = it.as_p[op.p], *mq = it.as_q[op.q];
+          const int tiles = op.tiles, out_kind = op.out_kind, total = tiles * it.batch;
+          const int num_kc = (int)((it.mat[op.p].cols + BK - 1) / BK);
+          const int tiles_m = (int)((it.mat[op.p].rows + kTileRows - 1) / kTileRows);
+          const int tiles_n = (int)((it.mat[op.q].rows + BN - 1) / BN);
           for (int t = unit; t < total && ok; t += units) {
             const int z = t / tiles;
             int tm, tn;
@@ -262,10 +270,10 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
                 uint8_t* s = smem + stage * P::STAGE;
                 if (leader) ptx::mbar_arrive_expect_tx(&full[stage], 2 * P::STAGE);
                 const uint32_t fc = ptx::map_to_rank(&full[stage], 0);
-                ptx::tma_load_3d_pair(s, map, kc * BK, i0, z, fc);
-                ptx::tma_load_3d_pair(s + P::A_BYTES, map + 1, kc * BK, i0, z, fc);
-                ptx::tma_load_3d_pair(s + 2 * P::A_BYTES, map + 2, kc * BK, j0, z, fc);
-                ptx::tma_load_3d_pair(s + 2 * P::A_BYTES + P::B_BYTES, map + 3, kc * BK, j0, z, fc);
+                ptx::tma_load_3d_pair(s, mp, kc * BK, i0, z, fc);
+                ptx::tma_load_3d_pair(s + P::A_BYTES, mp + 1, kc * BK, i0, z, fc);
+                ptx::tma_load_3d_pair(s + 2 * P::A_BYTES, mq, kc * BK, j0, z, fc);
+                ptx::tma_load_3d_pair(s + 2 * P::A_BYTES + P::B_BYTES, mq + 1, kc * BK, j0, z, fc);
                 if (leader) {
                   issued |= 1u << stage;
                   last = (last & ~(1u << stage)) | (phase << stage);
@@ -294,15 +302,15 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
         for (int p = 0; p < products && ok; ++p) {
-          const int pi = product_index(p, it.steps);
-          const int num_kc = it.gemm[pi].num_kc, total = it.gemm[pi].tiles * it.batch;
+          const Op op = it.op[p];
+          const int num_kc = (int)((it.mat[op.p].cols + BK - 1) / BK), total = op.tiles * it.batch;
           // A unit of work is one run of it.run stages of a tile: each has an accumulator of its own.
           const int runs = (num_kc + it.run - 1) / it.run;
           for (int t = unit; t < total && ok; t += units) {
             for (int run = 0; run < runs && ok; ++run) {
               if (!ptx::mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1, it.status, it.timeout_ns)) { ok = false; break; }
               ptx::tc_fence_after();
-              const uint32_t d = tmem + (uint32_t)(acc * BN);
+              const uint32_t d = tmem + (uint32_t)acc * P::ACC;
               const int depth = min(it.run, num_kc - run * it.run);
               for (int kc = 0; kc < depth; ++kc) {
                 if (!ptx::mbar_wait_bounded(&full[stage], phase, it.status, it.timeout_ns)) { ok = false; break; }
@@ -315,8 +323,8 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
 #pragma unroll
                 for (int k = 0; k < BK / 16; ++k) {  // 16 fp16 are 32 bytes along the swizzled row
                   ptx::mma_f16_ss_pair(d, phi + 2 * k, qhi + 2 * k, idesc, (kc | k) != 0, elected);
-                  ptx::mma_f16_ss_pair(d, phi + 2 * k, qlo + 2 * k, idesc, 1, elected);
-                  ptx::mma_f16_ss_pair(d, plo + 2 * k, qhi + 2 * k, idesc, 1, elected);
+                  ptx::mma_f16_ss_pair(P::APART ? d + BN : d, phi + 2 * k, qlo + 2 * k, idesc, !P::APART || (kc | k) != 0, elected);
+                  ptx::mma_f16_ss_pair(P::APART ? d + BN : d, plo + 2 * k, qhi + 2 * k, idesc, 1, elected);
                 }
                 if (elected) ptx::mma_commit_pair(&empty[stage]);
                 __syncwarp();
@@ -350,10 +358,15 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
     uint32_t acc_phase = 0;
     bool ok = true;
     for (int p = 0; p < products && ok; ++p) {
-      const GemmArgs a = it.gemm[product_index(p, it.steps)];  // in registers: its index is not constant
-      const int total = a.tiles * it.batch;
-      const int runs = (a.num_kc + it.run - 1) / it.run;
-      const bool sym = a.out_kind == kSymmetric;
+      const Op op = it.op[p];
+      const int64_t M = it.mat[op.p].rows, N = it.mat[op.q].rows;
+      const int num_kc = (int)((it.mat[op.p].cols + BK - 1) / BK);
+      const int tiles_m = (int)((M + kTileRows - 1) / kTileRows), tiles_n = (int)((N + BN - 1) / BN);
+      const int total = op.tiles * it.batch;
+      const int runs = (num_kc + it.run - 1) / it.run;
+      const bool sym = op.out_kind == kSymmetric;
+      const bool adds = op.add != kNone;
+      const Split d = it.mat[op.d], dt = it.mat[op.t], add = it.mat[adds ? op.add : mA];
       // The addend too comes from other CTAs, and a CTA counts itself in for this product only once
       // the last one is complete.
       if (p > 0) {
@@ -363,14 +376,12 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
         if (!ok) break;
       }
       for (int t = unit; t < total; t += units) {
-        const int z = t / a.tiles;
+        const int z = t / op.tiles;
         int tm, tn;
-        tile_of<BN>(t - z * a.tiles, a.out_kind, a.tiles_m, a.tiles_n, tm, tn);
+        tile_of<BN>(t - z * op.tiles, op.out_kind, tiles_m, tiles_n, tm, tn);
         const int64_t i0 = (int64_t)tm * kTileRows + rank * 128 + q * 32;
         const int64_t i = i0 + lane;
-        const StepScale sc = it.scale[(int64_t)z * it.steps + p / 3];
-        const float alpha = a.kind == 0 ? sc.gram : a.kind == 1 ? sc.square : sc.product;
-        const float beta = a.kind == 0 ? 0.f : a.kind == 1 ? sc.linear : sc.keep;
+        const Scale sc = it.scale[(int64_t)z * it.ops + p];
         const int64_t col0 = (int64_t)tn * BN + h * (BN / 2);
         const int sub = lane >> 2, part = (lane & 3) * 8;
         // The addend of a block of 32 x 32, four lanes a row; a block's is fetched while the one before
@@ -379,13 +390,13 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
         uint4 add_hi[4], add_lo[4];
         auto fetch = [&](int g) {
           const int64_t j = col0 + g * 32;
-          if (a.add_hi == nullptr || j >= a.N || (sym && j > i0)) return;
-          const int64_t at = z * a.d_matrix + (i0 + sub) * a.ld_d + j + part;
+          if (!adds || j >= N || (sym && j > i0)) return;
+          const int64_t at = z * add.matrix + (i0 + sub) * add.ld + j + part;
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (i0 + sub + 8 * k < a.M) {
-              add_hi[k] = *reinterpret_cast<const uint4*>(a.add_hi + at + 8 * k * a.ld_d);
-              add_lo[k] = *reinterpret_cast<const uint4*>(a.add_lo + at + 8 * k * a.ld_d);
+            if (i0 + sub + 8 * k < M) {
+              add_hi[k] = *reinterpret_cast<const uint4*>(add.hi + at + 8 * k * add.ld);
+              add_lo[k] = *reinterpret_cast<const uint4*>(add.lo + at + 8 * k * add.ld);
             }
         };
         if (runs == 1) fetch(0);
@@ -400,12 +411,18 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
 #pragma unroll
           for (int c = 0; c < BN / 64; ++c) {
             uint32_t v[32];
-            const uint32_t at = lanes + (uint32_t)(acc * BN + c * 32);
+            const uint32_t at = lanes + (uint32_t)acc * P::ACC + c * 32;
             ptx::tmem_ld32(at, v);
             ptx::tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               sum[c * 32 + e] = run == 0 ? __uint_as_float(v[e]) : sum[c * 32 + e] + __uint_as_float(v[e]);
+            if (P::APART) {
+              ptx::tmem_ld32(at + BN, v);
+              ptx::tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) sum[c * 32 + e] += __uint_as_float(v[e]);
+            }
             if (run + 1 == runs) {
 #pragma unroll
               for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(sum[c * 32 + e]);
@@ -434,12 +451,19 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
         for (int g = 0; g < BN / 64; ++g) {
           const int64_t j0 = col0 + g * 32;
           // Below the diagonal, on it, or above it: the same for the whole warp, like the bounds.
-          const bool inside = j0 < a.N && i0 < a.M && !(sym && j0 > i0);
-          const int64_t d_at = z * a.d_matrix + (i0 + sub) * a.ld_d + j0 + part;
+          const bool inside = j0 < N && i0 < M && !(sym && j0 > i0);
+          const int64_t d_at = z * d.matrix + (i0 + sub) * d.ld + j0 + part;
           uint32_t v[32];
           __syncwarp();  // the TMEM load is a whole warp's; the last block's reads of `turn` are done
-          ptx::tmem_ld32(lanes + (uint32_t)(acc * BN + g * 32), v);
+          ptx::tmem_ld32(lanes + (uint32_t)acc * P::ACC + g * 32, v);
           ptx::tmem_wait_ld();
+          if (P::APART && runs == 1) {
+            uint32_t x[32];
+            ptx::tmem_ld32(lanes + (uint32_t)acc * P::ACC + BN + g * 32, x);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + __uint_as_float(x[e]));
+          }
           if (g == BN / 64 - 1) {  // the accumulator goes back before the last stores
             ptx::tc_fence_before();
             __syncwarp();
@@ -457,19 +481,24 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
             const int r = sub + 8 * k;
             float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = alpha * __uint_as_float(turn[r * 32 + ((part + e) ^ r)]);
-            if (a.add_hi != nullptr) {
+            for (int e = 0; e < 8; ++e) f[e] = sc.acc * __uint_as_float(turn[r * 32 + ((part + e) ^ r)]);
+            if (adds) {
               const __half2* hi = reinterpret_cast<const __half2*>(&add_hi[k]);
               const __half2* lo = reinterpret_cast<const __half2*>(&add_lo[k]);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float2 x = __half22float2(hi[e]), y = __half22float2(lo[e]);
-                f[2 * e] = fmaf(beta, x.x + y.x, f[2 * e]);
-                f[2 * e + 1] = fmaf(beta, x.y + y.y, f[2 * e + 1]);
+                f[2 * e] = fmaf(sc.add, x.x + y.x, f[2 * e]);
+                f[2 * e + 1] = fmaf(sc.add, x.y + y.y, f[2 * e + 1]);
+              }
+              if (sym && j0 == i0) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (part + e == r) f[e] += sc.diagonal;
               }
             }
             uint32_t w[8];  // fp32, or hi in the low half and lo in the high half
-            if (a.out_kind == kFinal) {
+            if (op.out_kind == kFinal) {
 #pragma unroll
               for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(f[e]);
             } else {
@@ -479,11 +508,11 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
                 split_f16(f[e], hi, lo);
                 w[e] = (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
               }
-              if (i0 + r < a.M) {
+              if (i0 + r < M) {
                 uint4 hi, lo;
                 unzip(w, hi, lo);
-                *reinterpret_cast<uint4*>(a.d_hi + d_at + 8 * k * a.ld_d) = hi;
-                *reinterpret_cast<uint4*>(a.d_lo + d_at + 8 * k * a.ld_d) = lo;
+                *reinterpret_cast<uint4*>(d.hi + d_at + 8 * k * d.ld) = hi;
+                *reinterpret_cast<uint4*>(d.lo + d_at + 8 * k * d.ld) = lo;
               }
             }
             if (both) {
@@ -494,29 +523,26 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
           if (g + 1 < BN / 64) fetch(g + 1);
           if (!both) continue;
           __syncwarp();
-          if (a.out_kind == kFinal) {
-            if (i < a.M) {
-              for (int e = 0; e < 32 && j0 + e < a.N; ++e)
-                store_as(a.out, z * a.out_matrix + (j0 + e) * a.ld_out + i, a.out_dtype, __uint_as_float(turn[lane * 32 + (e ^ lane)]));
+          if (op.out_kind == kFinal) {
+            if (i < M) {
+              for (int e = 0; e < 32 && j0 + e < N; ++e)
+                store_as(it.out, z * it.out_matrix + (j0 + e) * it.ld_out + i, it.out_dtype, __uint_as_float(turn[lane * 32 + (e ^ lane)]));
             }
             continue;
           }
           // The other order: four lanes write a column's 32 rows.
-          __half* th = sym ? a.d_hi : a.t_hi;
-          __half* tl = sym ? a.d_lo : a.t_lo;
-          const int64_t ld = sym ? a.ld_d : a.ld_t;
-          const int64_t t_at = z * (sym ? a.d_matrix : a.t_matrix) + (j0 + sub) * ld + i0 + part;
+          const int64_t t_at = z * dt.matrix + (j0 + sub) * dt.ld + i0 + part;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int col = sub + 8 * k;
             uint32_t w[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = turn[(part + e) * 32 + (col ^ (part + e))];
-            if (j0 + col < a.N) {
+            if (j0 + col < N) {
               uint4 hi, lo;
               unzip(w, hi, lo);
-              *reinterpret_cast<uint4*>(th + t_at + 8 * k * ld) = hi;
-              *reinterpret_cast<uint4*>(tl + t_at + 8 * k * ld) = lo;
+              *reinterpret_cast<uint4*>(dt.hi + t_at + 8 * k * dt.ld) = hi;
+              *reinterpret_cast<uint4*>(dt.lo + t_at + 8 * k * dt.ld) = lo;
             }
           }
         }
@@ -549,17 +575,18 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
 
 // ---- the norm, the scales and the first X ---------------------------------------------------
 
-constexpr int kMaxSteps = 32;
 constexpr int kNormThreads = 256;
 
 struct PrepArgs {
   const void* g;
   int64_t rows, cols, row_stride, matrix_stride;  // of G; its rows are contiguous
-  int dtype, tall, parts, steps;
+  int parts, ops;
+  int whole;               // Q with the identity
   float eps;
   float coef[kMaxSteps][3];
+  uint8_t kind[kMaxOps];   // of the iteration's products
   double* part;            // [batch][parts] sums of squares
-  StepScale* scale;        // [batch][steps]
+  Scale* scale;            // [batch][ops]
   __half* g_hi;            // G's order: [rows, ld_g]
   __half* g_lo;
   __half* t_hi;            // the other order: [cols, ld_t]
@@ -628,16 +655,24 @@ __device__ double pow2_scale(double bound) {
   return ldexp(1.0, 15 - e);
 }
 
-__device__ double max_on(double top, double c1, double c3, double c5) {
-  // max of |c1 s + c3 s^3 + c5 s^5| over [0, top]: at the end, or where c1 + 3 c3 u + 5 c5 u^2 = 0, u = s^2
-  auto p = [&](double s) { return fabs(s * (c1 + s * s * (c3 + s * s * c5))); };
-  double m = p(top);
-  auto at = [&](double u) {
-    if (u > 0.0 && u < top * top) m = fmax(m, p(sqrt(u)));
+// max |f| over [0, top] of f = s^k (c0 + c1 u + c2 u^2): at the ends, or where f' = 0, a quadratic in u.
+// With u = s (k = 0 or 1) or u = s^2 (k = 1, `odd`: the polynomial of a step).
+__device__ double max_on(double top, int k, bool odd, double c0, double c1, double c2) {
+  auto f = [&](double s) {
+    const double u = odd ? s * s : s;
+    return fabs((k == 1 ? s : 1.0) * (c0 + u * (c1 + u * c2)));
   };
-  const double A = 5.0 * c5, B = 3.0 * c3, disc = B * B - 4.0 * A * c1;
+  double m = fmax(f(0.0), f(top));
+  const double last = odd ? top * top : top;
+  auto at = [&](double u) {
+    if (u > 0.0 && u < last) m = fmax(m, f(odd ? sqrt(u) : u));
+  };
+  // f' is proportional to A u^2 + B u + C.
+  const double A = k == 0 ? 0.0 : odd ? 5.0 * c2 : 3.0 * c2, B = k == 0 ? 2.0 * c2 : odd ? 3.0 * c1 : 2.0 * c1;
+  const double C = k == 0 ? c1 : c0;
+  const double disc = B * B - 4.0 * A * C;
   if (A == 0.0) {
-    if (B != 0.0) at(-c1 / B);
+    if (B != 0.0) at(-C / B);
   } else if (disc >= 0.0) {
     at((-B + sqrt(disc)) / (2.0 * A));
     at((-B - sqrt(disc)) / (2.0 * A));
@@ -649,30 +684,68 @@ constexpr double kSlack = 1.0 + 1e-3;  // on the bounds, for rounding along the 
 
 __device__ double first_scale(double rho) { return pow2_scale(rho * kSlack); }
 
-// The scales of every step of one matrix; rho is |X_0|_F.
-__device__ void scale_table(double rho, const PrepArgs& a, StepScale* out) {
-  double bound = rho * kSlack;
-  double sx = first_scale(rho);
-  for (int k = 0; k < a.steps; ++k) {
-    const double ca = a.coef[k][0], cb = a.coef[k][1], cc = a.coef[k][2];
-    const double u = bound * bound;
-    const double sa = pow2_scale(u);
-    // |b u + c u^2| over [0, bound^2]
-    double mb = fabs(u * (cb + cc * u));
-    if (cc != 0.0) {
-      const double peak = -cb / (2.0 * cc);
-      if (peak > 0.0 && peak < u) mb = fmax(mb, fabs(peak * (cb + cc * peak)));
+// The factors of every product for one matrix; rho is |X_0|_F.  x bounds |X|_2; A, T, P and Q are
+// polynomials in the eigenvalues of X X^T, whose bounds follow; sx ... sq are the matrices' scales.
+__device__ void scale_table(double rho, const PrepArgs& a, Scale* out) {
+  double x = rho * kSlack, u = 0.0, q = 0.0, next = 0.0;
+  double sx = first_scale(rho), sa = 1.0, st = 1.0, sp = 1.0, sq = 1.0;
+  int step = 0;
+  bool chained = false;  // Q is the last polynomial itself
+  for (int i = 0; i < a.ops; ++i) {
+    const double c0 = a.coef[step][0], c1 = a.coef[step][1], c2 = a.coef[step][2];
+    double acc = 0.0, add = 0.0, diagonal = 0.0;
+    switch (a.kind[i]) {
+      case kGram:
+        u = x * x;
+        sa = pow2_scale(u);
+        acc = sa / (sx * sx);
+        chained = false;
+        break;
+      case kSquare: {
+        const double p = max_on(u, 0, false, a.whole ? c0 : 0.0, c1, c2) * kSlack;
+        sp = pow2_scale(p);
+        acc = c2 * sp / (sa * sa);
+        add = c1 * sp / sa;
+        diagonal = a.whole ? c0 * sp : 0.0;
+        next = max_on(x, 1, true, c0, c1, c2) * kSlack;
+        if (!chained) {
+          q = p;
+          sq = sp;
+        } else {
+          q *= p;
+        }
+        break;
+      }
+      case kTimes:
+        st = pow2_scale(max_on(u, 1, false, c0, c1, c2) * kSlack);
+        acc = st / (sa * sp);
+        break;
+      case kAgain: {
+        x = next;
+        u = x * x;
+        const double to = pow2_scale(u);
+        acc = to / (st * sp);
+        sa = to;
+        chained = true;
+        ++step;
+        break;
+      }
+      case kChain: {
+        const double to = pow2_scale(q * kSlack);
+        acc = to / (sp * sq);
+        sq = to;
+        break;
+      }
+      default: {  // kApply
+        x = next;
+        const double to = i + 1 == a.ops ? 1.0 : pow2_scale(x);
+        acc = to / (sq * sx);
+        add = c0 * to / sx;  // unless Q is whole
+        sx = to;
+        ++step;
+      }
     }
-    const double sb = pow2_scale(mb * kSlack);
-    const double next = max_on(bound, ca, cb, cc) * kSlack;
-    const double sn = k + 1 == a.steps ? 1.0 : pow2_scale(next);
-    out[k].gram = (float)(sa / (sx * sx));
-    out[k].square = (float)(cc * sb / (sa * sa));
-    out[k].linear = (float)(cb * sb / sa);
-    out[k].product = (float)(sn / (sb * sx));
-    out[k].keep = (float)(ca * sn / sx);
-    bound = next;
-    sx = sn;
+    out[i] = {(float)acc, (float)add, (float)diagonal};
   }
 }
 
@@ -717,7 +790,7 @@ __global__ void __launch_bounds__(256) ortho_split_kernel(const PrepArgs a) {
       const bool first = blockIdx.x == 0 && blockIdx.y == 0;
       const double rho = den > 0.0 ? norm / den : 0.0;
       s_factor = first_scale(rho) / den;
-      if (first) scale_table(rho, a, a.scale + z * a.steps);
+      if (first) scale_table(rho, a, a.scale + z * a.ops);
     }
   }
   __syncthreads();
@@ -764,26 +837,74 @@ __global__ void __launch_bounds__(256) ortho_split_kernel(const PrepArgs a) {
 
 // ---- host side ----------------------------------------------------------------------------
 
-// One matrix kept as hi and lo in both halves of a buffer.
-struct Split {
-  __half* hi;
-  __half* lo;
-  int64_t rows, cols, ld, matrix;
-};
+// Steps that form a group.  Carrying A over (two products of r^3) in place of going through X
+// (r^2 c + 2 r^2 c of products) saves (1.5 c / r - 1.5) r^3 a step, so long rows are grouped: up to three
+// steps, which leaves the error where it was (an error of A grows by a^2 a step; four steps and more
+// let it show: 8 times for an update with a few strong directions).  4096 x 8192 bf16: 5.3 -> 3.9 ms.
+int group_size(int64_t r, int64_t c, bool whole, const float* coef, int step, int steps) {
+  if (!whole || 4 * c < 5 * r) return 1;
+  const int left = steps - step, groups = (left + 2) / 3;
+  int n = (left + groups - 1) / groups;
+  double growth = 1.0;
+  for (int k = 0; k + 1 < n; ++k) {
+    growth *= (double)coef[3 * (step + k)] * coef[3 * (step + k)];
+    if (growth > 200.0) return k + 1;
+  }
+  return n;
+}
+
+// The products of an iteration.
+int list_ops(int64_t r, int64_t c, bool tall, bool whole, const float* coef, int steps, Op* op) {
+  int n = 0, xt = mXT0;
+  auto put = [&](int kind, int p, int q, int d, int t, int out_kind, int add = kNone) {
+    op[n++] = Op{(uint8_t)kind, (uint8_t)p, (uint8_t)q, (uint8_t)d, (uint8_t)t, (uint8_t)add, (uint8_t)out_kind, 0};
+  };
+  for (int step = 0; step < steps;) {
+    const int size = group_size(r, c, whole, coef, step, steps);
+    int last = mQ0, q = mQ0;  // the last polynomial, and the product of the group's
+    put(kGram, mX, mX, mA, mA, kSymmetric);
+    put(kSquare, mA, mA, mQ0, mQ0, kSymmetric, mA);
+    for (int k = 1; k < size; ++k) {
+      put(kTimes, mA, last, mT, mT, kSymmetric);
+      put(kAgain, mT, last, mA, mA, kSymmetric);
+      put(kSquare, mA, mA, mP, mP, kSymmetric, mA);
+      const int to = q == mQ0 ? mQ1 : mQ0;
+      put(kChain, mP, q, to, to, kSymmetric);
+      last = mP;
+      q = to;
+    }
+    step += size;
+    if (step < steps) {
+      const int to = xt == mXT0 ? mXT1 : mXT0;
+      put(kApply, q, xt, mX, to, kBoth, whole ? kNone : mX);  // X in place: a thread reads what it replaces
+      xt = to;
+    } else if (tall) {
+      // The last product runs in the order that lets the lanes of a warp write the result's rows.
+      put(kApply, q, xt, mX, mX, kFinal, whole ? kNone : mX);
+    } else {
+      put(kApply, xt, q, mX, mX, kFinal, whole ? kNone : xt);
+    }
+  }
+  return n;
+}
 
 struct Layout {
-  int64_t r, c;                 // X is r x c, r <= c
+  int64_t r, c;  // X is r x c, r <= c
   int64_t ld_c, ld_r;
-  size_t status, part, scale, x, xt0, xt1, a, b, end;
-  int parts;
+  size_t status, part, scale, mat[kMatrices], end;
+  int parts, ops;
+  Op op[kMaxOps];
 };
 
-Layout layout_of(int64_t batch, int64_t rows, int64_t cols, int steps) {
+// The offsets do not depend on the element type or the coefficients (NULL: any), only the products do.
+Layout layout_of(int64_t batch, int64_t rows, int64_t cols, int dtype, const float* coef, int steps) {
   Layout L;
   L.r = std::min(rows, cols);
   L.c = std::max(rows, cols);
   L.ld_c = round_up(L.c, 32);
   L.ld_r = round_up(L.r, 32);
+  static const float ones[3 * kMaxSteps] = {};
+  L.ops = list_ops(L.r, L.c, rows > cols, dtype != LM_F32, coef != nullptr ? coef : ones, steps, L.op);
   // About 8 K values for each CTA of the norm, and no more CTAs than give each SM four.
   const int64_t want = std::min<int64_t>(ceil_div(rows * cols, 8192), ceil_div(4 * kSmCount, batch > 0 ? batch : 1));
   L.parts = (int)std::max<int64_t>(1, want);
@@ -795,27 +916,16 @@ Layout layout_of(int64_t batch, int64_t rows, int64_t cols, int steps) {
   };
   L.status = take(64);
   L.part = take(sizeof(double) * batch * L.parts);
-  L.scale = take(sizeof(StepScale) * batch * steps);
+  L.scale = take(sizeof(Scale) * batch * kMaxOps);
   const size_t x = sizeof(__half) * 2 * batch * L.r * L.ld_c, xt = sizeof(__half) * 2 * batch * L.c * L.ld_r;
   const size_t sq = sizeof(__half) * 2 * batch * L.r * L.ld_r;
-  L.x = take(x);
-  L.xt0 = take(xt);
-  L.xt1 = take(xt);
-  L.a = take(sq);
-  L.b = take(sq);
+  const bool grouped = 4 * L.c >= 5 * L.r && steps > 1;
+  for (int m = 0; m < kMatrices; ++m) {
+    const bool used = m <= mA || m == mQ0 || grouped;  // the others belong to groups of steps
+    L.mat[m] = !used ? L.mat[mA] : take(m == mX ? x : m <= mXT1 ? xt : sq);
+  }
   L.end = off;
   return L;
-}
-
-Split split_at(void* ws, size_t off, int64_t batch, int64_t rows, int64_t cols, int64_t ld) {
-  Split s;
-  s.hi = ws_at<__half>(ws, off);
-  s.lo = s.hi + batch * rows * ld;
-  s.rows = rows;
-  s.cols = cols;
-  s.ld = ld;
-  s.matrix = rows * ld;
-  return s;
 }
 
 int64_t tiles_of(int64_t M, int64_t N, int bn, int out_kind) {
@@ -826,14 +936,8 @@ int64_t tiles_of(int64_t M, int64_t N, int bn, int out_kind) {
   return t;
 }
 
-// One product D = P Q^T of the iteration, apart from where D goes.
-struct Operands {
-  const Split* p;
-  const Split* q;
-};
-
 template <int BN>
-cudaError_t launch_iteration(IterArgs& it, const Operands* op, cudaStream_t stream) {
+cudaError_t launch_iteration(IterArgs& it, cudaStream_t stream) {
   using PL = Plan<BN>;
   auto k = ortho_kernel<BN>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PL::SMEM);
@@ -844,23 +948,21 @@ cudaError_t launch_iteration(IterArgs& it, const Operands* op, cudaStream_t stre
     return cudaFuncGetAttributes(&fa, k) == cudaSuccess ? fa.numRegs : 0;
   }();
   if (regs < kRegs) return cudaErrorInvalidConfiguration;
+  for (int m = 0; m < kMatrices; ++m) {
+    const Split& s = it.mat[m];
+    for (int h = 0; h < 2; ++h) {
+      const __half* base = h == 0 ? s.hi : s.lo;
+      if (!make_tmap_f16(&it.as_p[m][h], base, s.cols, s.rows, it.batch, s.ld, s.matrix, BK, 128) ||
+          !make_tmap_f16(&it.as_q[m][h], base, s.cols, s.rows, it.batch, s.ld, s.matrix, BK, PL::BROWS))
+        return cudaErrorInvalidValue;
+    }
+  }
   int64_t most = 0;
-  for (int p = 0; p < kProducts; ++p) {
-    GemmArgs& a = it.gemm[p];
-    const Split &l = *op[p].p, &r = *op[p].q;
-    if (!make_tmap_f16(&it.map[p][0], l.hi, l.cols, l.rows, it.batch, l.ld, l.matrix, BK, 128) ||
-        !make_tmap_f16(&it.map[p][1], l.lo, l.cols, l.rows, it.batch, l.ld, l.matrix, BK, 128) ||
-        !make_tmap_f16(&it.map[p][2], r.hi, r.cols, r.rows, it.batch, r.ld, r.matrix, BK, PL::BROWS) ||
-        !make_tmap_f16(&it.map[p][3], r.lo, r.cols, r.rows, it.batch, r.ld, r.matrix, BK, PL::BROWS))
-      return cudaErrorInvalidValue;
-    a.M = l.rows;
-    a.N = r.rows;
-    a.num_kc = (int)ceil_div(l.cols, BK);
-    a.tiles_m = (int)ceil_div(a.M, kTileRows);
-    a.tiles_n = (int)ceil_div(a.N, BN);
-    const int64_t tiles = tiles_of(a.M, a.N, BN, a.out_kind);
+  for (int i = 0; i < it.ops; ++i) {
+    Op& op = it.op[i];
+    const int64_t tiles = tiles_of(it.mat[op.p].rows, it.mat[op.q].rows, BN, op.out_kind);
     if (tiles * it.batch >= (int64_t(1) << 30)) return cudaErrorInvalidConfiguration;
-    a.tiles = (int)tiles;
+    op.tiles = (int)tiles;
     most = std::max(most, tiles * it.batch);
   }
   // A cooperative launch: the CTAs wait for one another between products, so all must be resident.
@@ -892,19 +994,23 @@ cudaError_t launch_iteration(IterArgs& it, const Operands* op, cudaStream_t stre
   return cudaLaunchKernelEx(&cfg, k, it);
 }
 
-// The tile width with the least estimated time.  A slice of 64 costs a pair the larger of its 12 MMAs
-// (6 BN cycles) and its operands' way into shared memory (64 bytes a cycle and CTA: 1024, 768 and 640
-// cycles for BN = 256, 128 and 64); a product ends with an epilogue that nothing hides.
-int tile_width(const IterArgs& it, const Operands* op) {
+// The tile width with the least estimated time, in cycles.  A slice of 64 costs a pair the larger of its
+// 12 MMAs (6 BN cycles) and its operands' way into shared memory (64 bytes a cycle and CTA: 1024, 768 and
+// 640 for BN = 256, 128 and 64; 850 for 128 with every SM at it).  A product ends with the epilogue of a
+// tile, which nothing hides: 150 BN.  Measured for 64, 128 and 256: four of 256 x 256: 134, 207 and 374
+// us; 2048 x 4096: 960, 835 and 1110; 4096 x 8192 (not grouped): 7.1, 5.6 and 5.3 ms.
+int tile_width(const IterArgs& it) {
   const int64_t pairs = device_sm_count() / 2;
   int best = 0;
   int64_t least = 0;
   for (const int bn : {256, 128, 64}) {
-    const int64_t slice = bn == 256 ? 1536 : bn == 128 ? 768 : 640;
+    const int64_t slice = bn == 256 ? 1536 : bn == 128 ? 850 : 640;
     int64_t cost = 0;
-    for (const int p : {kGram, kSquare, kProduct})
-      cost += ceil_div(tiles_of(op[p].p->rows, op[p].q->rows, bn, it.gemm[p].out_kind) * it.batch, pairs) *
-                  ceil_div(op[p].p->cols, BK) * slice + 32 * bn;
+    for (int i = 0; i < it.ops; ++i) {
+      const Split &p = it.mat[it.op[i].p], &q = it.mat[it.op[i].q];
+      cost += ceil_div(tiles_of(p.rows, q.rows, bn, it.op[i].out_kind) * it.batch, pairs) * ceil_div(p.cols, BK) * slice +
+              150 * bn;
+    }
     if (best == 0 || cost < least) {
       best = bn;
       least = cost;
@@ -916,22 +1022,26 @@ int tile_width(const IterArgs& it, const Operands* op) {
 }  // namespace
 
 size_t ortho_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int steps) {
-  return layout_of(batch, rows, cols, steps).end;
+  return layout_of(batch, rows, cols, LM_F32, nullptr, steps).end;
 }
 
 int ortho_max_steps() { return kMaxSteps; }
 
 cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaStream_t stream) {
   if (o.batch == 0 || o.rows == 0 || o.cols == 0) return cudaSuccess;
-  const Layout L = layout_of(o.batch, o.rows, o.cols, o.steps);
+  const Layout L = layout_of(o.batch, o.rows, o.cols, o.dtype, o.coefficients, o.steps);
   const bool tall = o.rows > o.cols;
   int* status = ws_at<int>(o.workspace, L.status);
-  StepScale* scale = ws_at<StepScale>(o.workspace, L.scale);
-  const Split x = split_at(o.workspace, L.x, o.batch, L.r, L.c, L.ld_c);
-  const Split xt = split_at(o.workspace, L.xt0, o.batch, L.c, L.r, L.ld_r);
-  const Split xt_next = split_at(o.workspace, L.xt1, o.batch, L.c, L.r, L.ld_r);
-  const Split ma = split_at(o.workspace, L.a, o.batch, L.r, L.r, L.ld_r);
-  const Split mb = split_at(o.workspace, L.b, o.batch, L.r, L.r, L.ld_r);
+  IterArgs it{};
+  for (int m = 0; m < kMatrices; ++m) {
+    Split& s = it.mat[m];
+    s.rows = m == mXT0 || m == mXT1 ? L.c : L.r;
+    s.cols = m == mX ? L.c : L.r;
+    s.ld = m == mX ? L.ld_c : L.ld_r;
+    s.matrix = s.rows * s.ld;
+    s.hi = ws_at<__half>(o.workspace, L.mat[m]);
+    s.lo = s.hi + o.batch * s.matrix;
+  }
 
   PrepArgs p{};
   p.g = o.update;
@@ -939,17 +1049,17 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
   p.cols = o.cols;
   p.row_stride = o.row_stride;
   p.matrix_stride = o.matrix_stride;
-  p.dtype = o.dtype;
-  p.tall = tall;
   p.parts = L.parts;
-  p.steps = o.steps;
+  p.ops = L.ops;
+  p.whole = o.dtype != LM_F32;
   p.eps = o.eps;
   for (int k = 0; k < o.steps; ++k)
     for (int e = 0; e < 3; ++e) p.coef[k][e] = o.coefficients[3 * k + e];
+  for (int i = 0; i < L.ops; ++i) p.kind[i] = L.op[i].kind;
   p.part = ws_at<double>(o.workspace, L.part);
-  p.scale = scale;
-  const Split& g = tall ? xt : x;
-  const Split& t = tall ? x : xt;
+  p.scale = ws_at<Scale>(o.workspace, L.scale);
+  const Split& g = it.mat[tall ? mXT0 : mX];
+  const Split& t = it.mat[tall ? mX : mXT0];
   p.g_hi = g.hi;
   p.g_lo = g.lo;
   p.ld_g = g.ld;
@@ -969,70 +1079,32 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
   const bool packs = (o.cols * es) % 16 == 0 && (o.row_stride * es) % 16 == 0 &&
                      (o.batch == 1 || (o.matrix_stride * es) % 16 == 0) &&
                      reinterpret_cast<uintptr_t>(o.update) % 16 == 0;
-  auto by_pack = [&](auto t) {
-    using T = decltype(t);
+  auto by_pack = [&](auto x) {
+    using T = decltype(x);
     constexpr int V = 16 / sizeof(T);
     return packs ? prep(ortho_norm_kernel<T, V>, ortho_split_kernel<T, V>)
                  : prep(ortho_norm_kernel<T, 1>, ortho_split_kernel<T, 1>);
   };
   cudaError_t e = o.dtype == LM_F32 ? by_pack(float{}) : o.dtype == LM_BF16 ? by_pack(__nv_bfloat16{}) : by_pack(__half{});
   if (e != cudaSuccess) return e;
-  note_launches(2);
 
-  IterArgs it{};
-  it.scale = scale;
+  it.ops = L.ops;
+  std::copy(L.op, L.op + L.ops, it.op);
+  it.batch = (int)o.batch;
+  it.run = o.dtype == LM_F32 ? 4 : o.dtype == LM_F16 ? 16 : 32;
+  it.out = o.out;
+  it.ld_out = o.cols;
+  it.out_matrix = o.rows * o.cols;
+  it.out_dtype = o.dtype;
+  it.scale = p.scale;
   it.arrived = reinterpret_cast<unsigned*>(status + 1);
   it.status = status;
   it.timeout_ns = wc.timeout_ns;
-  it.steps = o.steps;
-  it.batch = (int)o.batch;
-  it.run = o.dtype == LM_F32 ? 4 : o.dtype == LM_F16 ? 16 : 32;
   it.debug_skip_first_load = wc.debug_skip_first_load;
-  auto to = [](GemmArgs& a, int out_kind, int kind, const Split& d) {
-    a.out_kind = out_kind;
-    a.kind = kind;
-    a.d_hi = d.hi;
-    a.d_lo = d.lo;
-    a.ld_d = d.ld;
-    a.d_matrix = d.matrix;
-  };
-  auto add = [](GemmArgs& a, const Split& s) {
-    a.add_hi = s.hi;
-    a.add_lo = s.lo;
-  };
-  const Split xts[2] = {xt, xt_next};
-  Operands op[kProducts];
-  op[kGram] = {&x, &x};
-  to(it.gemm[kGram], kSymmetric, 0, ma);
-  op[kSquare] = {&ma, &ma};
-  to(it.gemm[kSquare], kSymmetric, 1, mb);
-  add(it.gemm[kSquare], ma);
-  for (int b = 0; b < 2; ++b) {
-    // X in place (each value is read by the thread that replaces it), X^T into the other buffer.
-    GemmArgs& a = it.gemm[kProduct + b];
-    op[kProduct + b] = {&mb, &xts[b]};
-    to(a, kBoth, 2, x);
-    add(a, x);
-    a.t_hi = xts[1 - b].hi;
-    a.t_lo = xts[1 - b].lo;
-    a.ld_t = xts[1 - b].ld;
-    a.t_matrix = xts[1 - b].matrix;
-  }
-  // The last product runs in the order that lets the lanes of a warp write the result's rows.
-  const Split& last = xts[(o.steps - 1) & 1];
-  GemmArgs& f = it.gemm[kLast];
-  op[kLast] = tall ? Operands{&mb, &last} : Operands{&last, &mb};
-  to(f, kFinal, 2, tall ? x : last);
-  add(f, tall ? x : last);
-  f.out = o.out;
-  f.ld_out = o.cols;
-  f.out_matrix = o.rows * o.cols;
-  f.out_dtype = o.dtype;
-  const int bn = tile_width(it, op);
-  e = bn == 256 ? launch_iteration<256>(it, op, stream) : bn == 128 ? launch_iteration<128>(it, op, stream)
-                                                                    : launch_iteration<64>(it, op, stream);
+  const int bn = tile_width(it);
+  e = bn == 256 ? launch_iteration<256>(it, stream) : bn == 128 ? launch_iteration<128>(it, stream) : launch_iteration<64>(it, stream);
   if (e != cudaSuccess) return e;
-  note_launches(1);
+  note_launches(3);
   return cudaGetLastError();
 }
 
