@@ -1,13 +1,15 @@
 // ortho.cu -- orthogonalisation of an update by Newton-Schulz products, on the tensor cores.
 //
 //   X_0 = G / (|G|_F + eps)          (transposed where G has more rows than columns: X is r x c,
-//   A = X X^T,  B = b A + c A^2       r <= c)
-//   X <- a X + B X                    `steps` times, with (a, b, c) of each step
+//   A = X X^T                         r <= c)
+//   X <- (a + b A + c A^2) X          `steps` times, with (a, b, c) of each step
 //
-// All three products run as D = P Q^T with both operands K-major, on tcgen05.mma kind::f16: A takes
-// X twice, A^2 takes A twice (A is symmetric), and B X takes B and X^T, so every step keeps X in
-// both orders.  A and B are symmetric: only tiles that touch the lower triangle are computed, and
-// each block of 32 x 32 below the diagonal is stored at (i, j) and turned around at (j, i).  Flops of a step: r^2 c + r^3 + 2 r^2 c.
+// All products run as D = P Q^T with both operands K-major, on tcgen05.mma kind::f16: A takes X twice,
+// A^2 takes A twice (A is symmetric), and the last takes the polynomial and X^T, so X is kept in both
+// orders.  Polynomials of A are symmetric: only tiles that touch the lower triangle are computed, and
+// each block of 32 x 32 below the diagonal is stored at (i, j) and turned around at (j, i).  Flops of a
+// step: r^2 c + r^3 + 2 r^2 c.  With long rows several steps form a group that goes through X once (the
+// enums below).
 //
 // Precision: 3 x fp16.  An operand v is kept as v * 2^k = hi + lo, hi = fp16(v 2^k) and
 // lo = fp16(v 2^k - hi), and P Q^T = hi hi^T + hi lo^T + lo hi^T in fp32: 22 bits of each operand,
@@ -24,15 +26,16 @@
 // low by half a unit per MMA: 1.8e-5 of the result at a depth of 2601.  So an accumulator takes a
 // run of slices only, and the epilogue warps add these partial sums in registers, rounded to nearest.
 // The products with lo, two thirds of the MMAs but 2^-11 of the sum, go to an accumulator of their own
-// where there is room for one.  A run is 256 deep for fp32 results, 1024 for fp16 and 2048 for bf16, whose
-// own rounding is far larger: short runs cost up to 9% of the time.
+// where there is room for one.  2601 x 1001 fp32, runs 128, 192 and 256 deep: error 2.9e-6, 4.0e-6 and
+// 5.1e-6 (the fp32 library products': 3.3e-6) in 472, 410 and 364 us; 192 is taken.  fp16 and bf16
+// results, whose own rounding is far larger, take 1024 and 2048.
 //
 // Kernel: one launch runs the whole iteration (cooperative, one CTA per SM).  A product's tiles are
 // shared out over the CTA pairs; each CTA counts itself in when its part is stored, and the loads of
-// the next product wait until all have.  Against a launch for each product, which the next one's
-// start had to follow, (11 us from one to the next) this takes 8 us for a batch of four of 256 x 256.  Warp 0 loads operand slices by TMA (64 deep, 128-byte swizzle, hi and lo of
-// both operands) into a ring of stages; warp 1 issues 3 x 4 MMAs per stage into one of
-// two TMEM accumulators; warps 4..11 read the other one, apply the epilogue and store.  All
+// the next product wait until all have.  A launch for each product took 11 us from one to the next on a
+// batch of four of 256 x 256; this takes 8.  Warp 0 loads operand slices by TMA (64 deep, 128-byte
+// swizzle, hi and lo of both operands) into a ring of stages; warp 1 issues 3 x 4 MMAs per stage into one
+// of the TMEM accumulators; warps 4..11 read the others, apply the epilogue and store.  All
 // on CTA pairs (cta_group::2), tiles of 256 x 256, 128 or 64: a CTA of the pair loads its 128 rows of P
 // and half of the tile's rows of Q, for 256 x 256 two thirds of what a single CTA's 128 x 256 tile
 // takes.  That counts: an SM takes in about 64 bytes a cycle, so narrower tiles wait for their
@@ -178,10 +181,11 @@ struct Plan {
   static constexpr size_t FIXED = 1024 + 256 + sizeof(uint32_t) * kEpiWarps * kTurnWords;
   static constexpr int STAGES = (int)((kSmemMax - FIXED) / STAGE);
   static constexpr size_t SMEM = FIXED + (size_t)STAGES * STAGE;
-  // Two accumulators of ACC columns, one for the MMAs and one for the epilogue.  Where TMEM holds it (512
-  // columns), the hi x lo products have a part of their own (column BN on): see the truncation above.
+  // NACC accumulators of ACC columns, so that the MMAs go on while the epilogue reads.  Where TMEM (512
+  // columns) holds it, the hi x lo products have a part of their own (column BN on): see the truncation above.
   static constexpr bool APART = BN <= 128;
-  static constexpr uint32_t ACC = APART ? 2 * BN : BN, TCOLS = 2 * ACC;
+  static constexpr uint32_t ACC = APART ? 2 * BN : BN, TCOLS = 512;
+  static constexpr int NACC = TCOLS / ACC;
   static_assert(STAGES >= 2 && SMEM <= kSmemMax, "stages");
 };
 
@@ -193,9 +197,9 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
                                              ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + P::STAGES * P::STAGE);  // [STAGES] TMA -> MMA
   uint64_t* empty = full + P::STAGES;                                         // [STAGES] MMA -> TMA
-  uint64_t* acc_full = empty + P::STAGES;                                     // [2] MMA -> epilogue
-  uint64_t* acc_empty = acc_full + 2;                                         // [2] epilogue -> MMA
-  uint64_t* drain = acc_empty + 2;                                            // MMA teardown
+  uint64_t* acc_full = empty + P::STAGES;                                     // [NACC] MMA -> epilogue
+  uint64_t* acc_empty = acc_full + P::NACC;                                   // [NACC] epilogue -> MMA
+  uint64_t* drain = acc_empty + P::NACC;                                            // MMA teardown
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   unsigned* stored = tmem_slot + 1;                                           // epilogue warps, over all products
 
@@ -208,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
       ptx::mbar_init(&full[s], 1);
       ptx::mbar_init(&empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < P::NACC; ++b) {
       ptx::mbar_init(&acc_full[b], 1);
       ptx::mbar_init(&acc_empty[b], 2 * kEpiWarps);
     }
@@ -336,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
               if (!ok) break;
               if (elected) ptx::mma_commit_pair(&acc_full[acc]);
               __syncwarp();
-              if (++acc == 2) {
+              if (++acc == P::NACC) {
                 acc = 0;
                 acc_phase ^= 1;
               }
@@ -413,16 +417,18 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
             uint32_t v[32];
             const uint32_t at = lanes + (uint32_t)acc * P::ACC + c * 32;
             ptx::tmem_ld32(at, v);
-            ptx::tmem_wait_ld();
+            if constexpr (P::APART) {
+              uint32_t x[32];
+              ptx::tmem_ld32(at + BN, x);
+              ptx::tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + __uint_as_float(x[e]));
+            } else {
+              ptx::tmem_wait_ld();
+            }
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               sum[c * 32 + e] = run == 0 ? __uint_as_float(v[e]) : sum[c * 32 + e] + __uint_as_float(v[e]);
-            if (P::APART) {
-              ptx::tmem_ld32(at + BN, v);
-              ptx::tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) sum[c * 32 + e] += __uint_as_float(v[e]);
-            }
             if (run + 1 == runs) {
 #pragma unroll
               for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(sum[c * 32 + e]);
@@ -436,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
           ptx::tc_fence_before();
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(&acc_empty[acc], 0));
-          if (++acc == 2) {
+          if (++acc == P::NACC) {
             acc = 0;
             acc_phase ^= 1;
           }
@@ -456,13 +462,14 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
           uint32_t v[32];
           __syncwarp();  // the TMEM load is a whole warp's; the last block's reads of `turn` are done
           ptx::tmem_ld32(lanes + (uint32_t)acc * P::ACC + g * 32, v);
-          ptx::tmem_wait_ld();
           if (P::APART && runs == 1) {
             uint32_t x[32];
             ptx::tmem_ld32(lanes + (uint32_t)acc * P::ACC + BN + g * 32, x);
             ptx::tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + __uint_as_float(x[e]));
+          } else {
+            ptx::tmem_wait_ld();
           }
           if (g == BN / 64 - 1) {  // the accumulator goes back before the last stores
             ptx::tc_fence_before();
@@ -546,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
             }
           }
         }
-        if (++acc == 2) {
+        if (++acc == P::NACC) {
           acc = 0;
           acc_phase ^= 1;
         }
@@ -1091,7 +1098,7 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
   it.ops = L.ops;
   std::copy(L.op, L.op + L.ops, it.op);
   it.batch = (int)o.batch;
-  it.run = o.dtype == LM_F32 ? 4 : o.dtype == LM_F16 ? 16 : 32;
+  it.run = o.dtype == LM_F32 ? 3 : o.dtype == LM_F16 ? 16 : 32;
   it.out = o.out;
   it.ld_out = o.cols;
   it.out_matrix = o.rows * o.cols;

@@ -151,6 +151,11 @@ def format_raw(recs):
 CAPTURE_KERNELS = {
     "rbf": ("rbf_fwd_tc_kernel", "rbf_bwd_tc_kernel"),
     "cosine_sim": ("rbf_fwd_tc_kernel", "rbf_bwd_tc_kernel"),
+    "layernorm": ("ln_ring_forward_kernel", "ln_ring_backward_kernel"),
+    "token_logprob": ("logprob_forward_kernel", "logprob_backward_kernel"),
+    "preference_loss": ("logprob_forward_kernel", "logprob_backward_kernel"),
+    "policy_loss": ("logprob_forward_kernel", "logprob_backward_kernel"),
+    "orthogonalize": ("ortho_kernel",),
 }
 
 
@@ -191,6 +196,8 @@ def profile_candidate(case_name, impl=None, mode="both", iters=20, seed=0):
     from torch.profiler import ProfilerActivity, profile
     from framework.protocol import dtype_of
     case = _load_case(case_name)
+    if not case.grad_inputs:
+        mode = "forward"  # nothing to differentiate
     fn = _load_impl(impl) if impl else _load_impl(f"cases.{case_name}.op:candidate")
     dev = torch.device("cuda")
     inputs = case.make_inputs(seed, dtype_of(case.dtype), dev, requires_grad=mode != "forward")
