@@ -225,3 +225,37 @@ def test_verify_all_passes(cuda_device):
     from framework.verify import verify_all
     ok, report = verify_all(CASE, candidate, device="cuda")
     assert ok, report
+
+
+@pytest.mark.parametrize("D", [40, 1000, 1023, 4096, 9000, 20000])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_single_gradient(D, which, cuda_device):
+    """Only one of x, weight and bias requires a gradient: it equals the one among all three."""
+    from cases.layernorm.op import layer_norm
+    x, w, b, dy = inputs(37, D, torch.bfloat16, torch.float32, D + which)
+    every = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    layer_norm(*every, EPS).backward(dy)
+    one = [t.clone().requires_grad_(k == which) for k, t in enumerate((x, w, b))]
+    layer_norm(*one, EPS).backward(dy)
+    for k in range(3):
+        assert (one[k].grad is not None) == (k == which)
+    assert torch.equal(one[which].grad, every[which].grad)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """2^31 values and more: the last rows, and the column sums of rows beyond the boundary."""
+    from cases.layernorm import native
+    rows, D = (1 << 31) // 4096 + 700, 4096
+    x = torch.zeros(rows, D, dtype=torch.bfloat16, device="cuda")
+    dy = torch.zeros_like(x)
+    tail, w, b, up = inputs(600, D, torch.bfloat16, torch.bfloat16, 3)
+    x[-600:], dy[-600:] = tail, up
+    y, stats = native.ln_forward(x, w, b, EPS)
+    ys, ss = native.ln_forward(tail, w, b, EPS)
+    assert torch.equal(y[-600:], ys) and torch.equal(y[0], b) and torch.equal(y[-601], b)
+    dx, dw, db = native.ln_backward(dy, x, w, stats)
+    dxs, dws, dbs = native.ln_backward(up, tail, w, ss)
+    assert torch.equal(dx[-600:], dxs) and not dx[:-600].any()
+    # The other rows add zeros, in another grouping of the sums: a few fp32 roundings, then one.
+    for p, q in ((dw, dws), (db, dbs)):
+        assert float((p.float() - q.float()).abs().max()) <= 2.0 ** -7 * float(q.abs().max())

@@ -6,6 +6,11 @@ by up to 2^-21 of the product of its row's and column's norms (fp32 accumulation
 The noise goes through the same iteration, so the bound follows an update's own conditioning.  The
 kernel's errors are of this kind and size but not the same draw: a factor 4 for the whole (2-norm)
 and 40 for a single entry against the noise's root mean square.
+
+Results of 16 bits are summed in longer runs (1024 deep for fp16, 2048 for bf16) in an accumulator that
+truncates: each of the up to 3 MMAs for 16 terms takes up to one unit, 2^-23 of the accumulator, half of
+it on average.  The accumulator is at most the product of the norms, so a product of depth K carries up to
+3 min(K, run) / 16 * 2^-24 of that: 1.7e-5 at K = 1500 in bf16, 1/200 of its rounding.
 """
 import math
 
@@ -23,6 +28,7 @@ NOISE = 2.0 ** -21
 
 def iterate(g, steps, coef, eps, noise=None):
     """The iteration in fp64; ``noise``: a generator for the perturbed copy."""
+    run = {torch.float32: 0, torch.float16: 1024, torch.bfloat16: 2048}.get(g.dtype, 0)
     coef = [coef] * steps if not isinstance(coef[0], (tuple, list)) else coef
     x = g.double()
     tall = x.size(-2) > x.size(-1)
@@ -39,7 +45,8 @@ def iterate(g, steps, coef, eps, noise=None):
         out = rough(p) @ rough(q)
         if noise is not None:
             size = p.norm(dim=-1, keepdim=True) * q.norm(dim=-2, keepdim=True)
-            out = out + NOISE * size * (2 * torch.rand(out.shape, device=out.device,
+            sums = max(NOISE, 3 * min(p.size(-1), run) / 16 * 2.0 ** -24)
+            out = out + sums * size * (2 * torch.rand(out.shape, device=out.device,
                                                        dtype=out.dtype, generator=noise) - 1)
         return out
 
@@ -67,8 +74,12 @@ def check(g, steps=5, coef=COEF, eps=EPS, got=None):
     assert got.shape == g.shape and got.dtype == g.dtype and got.is_contiguous()
     want = iterate(g, steps, coef, eps)
     noisy = iterate(g, steps, coef, eps, torch.Generator(device="cuda").manual_seed(1))
-    err = got.double() - want
+    # What lies beyond the type's range rounds to infinity.
+    big = want.abs() > torch.finfo(g.dtype).max * (1 + 2 * half_ulp(g.dtype))
+    assert torch.equal(got.double()[big], want[big].sign() * math.inf)
+    err = torch.where(big, 0.0, got.double() - want)
     off = noisy - want
+    want = torch.where(big, 0.0, want)
     ulp = half_ulp(g.dtype)
     dims = (-2, -1)
     tiny = 2.0 ** -24 if g.dtype == torch.float16 else 0.0
@@ -236,3 +247,17 @@ def test_verify_all_passes(cuda_device):
     from framework.verify import verify_all
     ok, report = verify_all(CASE, candidate, device="cuda")
     assert ok and "[backward] none" in report, report
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(40, 400), (129, 1300), (1500, 300), (3, 70, 500)])
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 8])
+def test_groups_of_steps(shape, steps, dtype, cuda_device):
+    """Long rows: 16-bit types take several steps through X at once, of every group size, with
+    coefficients that change from step to step and with some that forbid a group."""
+    g = update(shape, dtype, sum(shape) + steps)
+    check(g, steps)
+    schedule = [(3.4445, -4.775, 2.0315), (3.0, -3.2, 1.2), (2.5, -2.0, 0.6), (1.875, -1.25, 0.375)]
+    check(g, steps, [schedule[k % 4] for k in range(steps)])
+    # a^2 = 225 is past what a group may carry: these two steps (15 times, then back) stand alone.
+    check(g, steps, ([(15.0, 0.0, 0.0), (1 / 15, 0.0, 0.0)] + [(1.875, -1.25, 0.375)] * steps)[:steps])

@@ -106,6 +106,7 @@ def test_masked_and_extreme_logits(dtype, cuda_device):
     lp = token_logprob(leaf, labels, IGNORE)
     lp.backward(torch.ones_like(lp))
     assert_within("logprob", lp, want, 200 * U32 * (1 + want.abs().nan_to_num(0, 0, 0)))
+    lp = lp.detach()
     assert float(lp[2]) == 0.0 and float(lp[5]) == -math.inf
     assert torch.isnan(lp[[3, 6, 7]]).all()
     for r in (0, 1, 2, 4, 8):
@@ -341,3 +342,92 @@ def test_verify_all_passes(name, cuda_device):
     op = importlib.import_module(f"cases.{name}.op")
     ok, report = verify_all(case, op.candidate, device="cuda")
     assert ok, report
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_unscored_positions_are_not_read(dtype, cuda_device):
+    """NaN and infinities in the logits, scores and advantages of unscored positions change nothing."""
+    from cases.policy_loss.op import policy_loss
+    from cases.preference_loss.op import preference_loss
+    x, labels, g = inputs(4, 9, 700, dtype, 6)
+    scored = labels != IGNORE
+    ref, old, adv = (torch.randn(4, 9, device="cuda", generator=g) for _ in range(3))
+
+    def run(x, ref, old, adv):
+        leaf = x.clone().requires_grad_(True)
+        a = preference_loss(leaf, labels, ref)
+        b = policy_loss(leaf, labels, old, ref, adv, kl_coef=0.1)
+        (a[0] + b[0]).backward()
+        return a[0], a[1], b[0], b[1], leaf.grad
+
+    want = run(x, ref, old, adv)
+    bad = x.clone()
+    bad[~scored] = math.nan
+    spoil = [torch.where(scored, t, v) for t, v in ((ref, math.nan), (old, math.inf), (adv, math.nan))]
+    for p, q in zip(want, run(bad, *spoil)):
+        assert torch.equal(p, q)
+
+
+def test_empty_batches(cuda_device):
+    from cases.policy_loss.op import policy_loss
+    from cases.preference_loss.op import preference_loss
+    from cases.token_logprob.op import token_logprob
+    for B, T in ((2, 0), (0, 5)):
+        x = torch.randn(B, T, 30, device="cuda", requires_grad=True)
+        lab = torch.zeros(B, T, dtype=torch.int64, device="cuda")
+        z = torch.zeros(B, T, device="cuda")
+        assert token_logprob(x, lab).shape == (B, T)
+        loss, reward = preference_loss(x, lab, z)
+        assert reward.shape == (B,)
+        assert (abs(float(loss.detach()) - math.log(2)) < 1e-6) if B else torch.isnan(loss)
+        loss.backward()
+        assert x.grad.shape == x.shape
+        loss, kl = policy_loss(x, lab, z, z, torch.ones(B, device="cuda"))
+        assert float(loss.detach()) == 0.0 and float(kl) == 0.0
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """A view whose rows lie 2^31 elements and more behind its start."""
+    from cases.token_logprob import native
+    V = 70000
+    rows = (1 << 31) // V + 40
+    base = torch.zeros(rows, V, dtype=torch.bfloat16, device="cuda")
+    x, labels, g = inputs(1, 30, V, torch.bfloat16, 2, scored=0.8)
+    base[-30:] = x[0]
+    lab = torch.full((rows,), IGNORE, device="cuda")
+    lab[-30:] = labels[0]
+    lab[0] = 17
+    lp, stats = native.logprob_forward(base, lab, IGNORE)
+    small, sstats = native.logprob_forward(x[0], labels[0], IGNORE)
+    assert_within("logprob", lp[-30:], small, 200 * U32 * (1 + small.abs()))
+    assert abs(float(lp[0]) + math.log(V)) < 1e-5
+    up = torch.ones_like(lp)
+    dx = native.logprob_backward(base, lab, stats, up, IGNORE)
+    want = native.logprob_backward(x[0], labels[0], sstats, up[-30:], IGNORE)
+    # Equal up to the sums' grouping: two roundings to bf16 apart at most.
+    assert_within("dlogits", dx[-30:], want, 2.01 * rounded(want, torch.bfloat16) + 1e-9)
+    assert not dx[1:-30].any() and dx[0].any()
+
+
+def test_other_streams(cuda_device):
+    from cases.policy_loss.op import policy_loss
+    x, labels, g = inputs(4, 50, 2001, torch.bfloat16, 4)
+    z = torch.full((4, 50), -3.0, device="cuda")
+    adv = torch.randn(4, device="cuda", generator=g)
+
+    def run():
+        leaf = x.clone().requires_grad_(True)
+        loss, kl = policy_loss(leaf, labels, z, z, adv, kl_coef=0.1)
+        loss.backward()
+        return loss.detach(), kl, leaf.grad
+
+    want = run()
+    outs = []
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append(run())
+    torch.cuda.synchronize()
+    for o in outs:
+        assert all(torch.equal(p, q) for p, q in zip(o, want))
