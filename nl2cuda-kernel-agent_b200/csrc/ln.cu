@@ -744,9 +744,8 @@ int pack_elems(const LnArgs& a, bool backward) {
     return a.D % vec == 0 && ok(a.x, a.x_stride, eb) && ok(a.y, a.D, eb) && okw(a.weight) &&
            (backward ? ok(a.dy, a.dy_stride, eb) : okw(a.bias));
   };
-  const int64_t most = 16 / eb;
-  if (fits(most)) return (int)most;
-  if (eb == 2 && fits(2)) return 2;
+  for (int64_t vec = 16 / eb; vec > 1; vec /= 2)
+    if (fits(vec)) return (int)vec;
   return 1;
 }
 
@@ -769,12 +768,15 @@ Shape backward_shape(const LnArgs& a, int vec) {
   return s;
 }
 
+// Packs that a lane of the forward holds at most: 64 bytes of single values, 128 of wider ones.
+constexpr int most_packs(int vec, int elem_bytes) { return vec == 1 ? 32 : vec * elem_bytes == 4 ? 16 : 128 / (vec * elem_bytes); }
+
 // Forward: a row takes the fewest warps that hold it in up to 8 packs of 16 bytes (16 pairs, 32 single
 // values) a lane, so that few warps wait for one another; more of them while the rows alone do not fill the SMs.
 Shape forward_shape(const LnArgs& a) {
   Shape s;
   s.vec = pack_elems(a, false);
-  const int most = s.vec * (int)elem_bytes(a.dtype) == 16 ? 8 : s.vec == 2 ? 16 : 32;
+  const int most = most_packs(s.vec, (int)elem_bytes(a.dtype));
   const int64_t packs = ceil_div(a.D, 32 * s.vec);  // of a lane, with one warp
   s.W = 1;
   while (s.W * most < packs || (s.W < packs && s.W < 8 && a.rows * s.W < 8 * (int64_t)kSmCount)) s.W *= 2;
@@ -794,10 +796,14 @@ cudaError_t by_backward_shape(const Shape& s, F f) {
     if (s.nv * s.vec == kLaneElems) return f(T{}, integral_constant<int, MAXV>{}, integral_constant<int, kLaneElems / MAXV>{});
     return f(T{}, integral_constant<int, MAXV>{}, integral_constant<int, 1>{});
   }
-  if constexpr (sizeof(T) == 2) {
-    if (s.vec == 2) {
-      if (s.nv * s.vec == kLaneElems) return f(T{}, integral_constant<int, 2>{}, integral_constant<int, kLaneElems / 2>{});
-      return f(T{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
+  if (s.vec == 2) {
+    if (s.nv * s.vec == kLaneElems) return f(T{}, integral_constant<int, 2>{}, integral_constant<int, kLaneElems / 2>{});
+    return f(T{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
+  }
+  if constexpr (MAXV == 8) {
+    if (s.vec == 4) {
+      if (s.nv * s.vec == kLaneElems) return f(T{}, integral_constant<int, 4>{}, integral_constant<int, kLaneElems / 4>{});
+      return f(T{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
     }
   }
   if (s.nv == kLaneElems) return f(T{}, integral_constant<int, 1>{}, integral_constant<int, kLaneElems>{});
@@ -806,7 +812,7 @@ cudaError_t by_backward_shape(const Shape& s, F f) {
 
 template <typename T, int VEC, int NV, typename F>
 cudaError_t by_forward_count(const Shape& s, F f) {
-  constexpr int most = VEC * sizeof(T) == 16 ? 8 : VEC == 2 ? 16 : 32;
+  constexpr int most = most_packs(VEC, sizeof(T));
   if (s.nv <= NV) {
     if (s.threads <= 256) return f(ln_forward_kernel<T, VEC, NV, 256>);
     if constexpr (NV == most) return f(ln_forward_kernel<T, VEC, NV, 512>);  // only the longest rows
@@ -819,8 +825,9 @@ template <typename T, typename F>
 cudaError_t by_forward_shape(const Shape& s, F f) {
   constexpr int MAXV = 16 / sizeof(T);
   if (s.vec == MAXV) return by_forward_count<T, MAXV, 1>(s, f);
-  if constexpr (sizeof(T) == 2) {
-    if (s.vec == 2) return by_forward_count<T, 2, 2>(s, f);
+  if (s.vec == 2) return by_forward_count<T, 2, 2>(s, f);
+  if constexpr (MAXV == 8) {
+    if (s.vec == 4) return by_forward_count<T, 4, 1>(s, f);
   }
   return by_forward_count<T, 1, 4>(s, f);
 }
