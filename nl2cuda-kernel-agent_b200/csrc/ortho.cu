@@ -844,14 +844,13 @@ __global__ void __launch_bounds__(256) ortho_split_kernel(const PrepArgs a) {
 
 // ---- host side ----------------------------------------------------------------------------
 
-// Steps that form a group.  Carrying A over (two products of r^3) in place of going through X
-// (r^2 c + 2 r^2 c of products) saves (1.5 c / r - 1.5) r^3 a step, so long rows are grouped: up to three
-// steps, which leaves the error where it was (an error of A grows by a^2 a step; four steps and more
-// let it show: 8 times for an update with a few strong directions).  4096 x 8192 bf16: 5.3 -> 3.9 ms.
-int group_size(int64_t r, int64_t c, bool whole, const float* coef, int step, int steps) {
-  if (!whole || 4 * c < 5 * r) return 1;
+// Steps that a group may hold.  Carrying A over (two products of r^3 in place of going through X: r^2 c + 2
+// r^2 c) saves (1.5 c / r - 1.5) r^3 a step, at one product more.  Up to three steps, which leaves the
+// error where it was: an error of A grows by a^2 a step; four steps and more let it show (8 times, for an
+// update with a few strong directions).  4096 x 8192 bf16: 5.3 -> 3.9 ms.
+int group_size(const float* coef, int step, int steps) {
   const int left = steps - step, groups = (left + 2) / 3;
-  int n = (left + groups - 1) / groups;
+  const int n = (left + groups - 1) / groups;
   double growth = 1.0;
   for (int k = 0; k + 1 < n; ++k) {
     growth *= (double)coef[3 * (step + k)] * coef[3 * (step + k)];
@@ -861,13 +860,13 @@ int group_size(int64_t r, int64_t c, bool whole, const float* coef, int step, in
 }
 
 // The products of an iteration.
-int list_ops(int64_t r, int64_t c, bool tall, bool whole, const float* coef, int steps, Op* op) {
+int list_ops(bool tall, bool whole, bool grouped, const float* coef, int steps, Op* op) {
   int n = 0, xt = mXT0;
   auto put = [&](int kind, int p, int q, int d, int t, int out_kind, int add = kNone) {
     op[n++] = Op{(uint8_t)kind, (uint8_t)p, (uint8_t)q, (uint8_t)d, (uint8_t)t, (uint8_t)add, (uint8_t)out_kind, 0};
   };
   for (int step = 0; step < steps;) {
-    const int size = group_size(r, c, whole, coef, step, steps);
+    const int size = grouped ? group_size(coef, step, steps) : 1;
     int last = mQ0, q = mQ0;  // the last polynomial, and the product of the group's
     put(kGram, mX, mX, mA, mA, kSymmetric);
     put(kSquare, mA, mA, mQ0, mQ0, kSymmetric, mA);
@@ -899,19 +898,17 @@ struct Layout {
   int64_t r, c;  // X is r x c, r <= c
   int64_t ld_c, ld_r;
   size_t status, part, scale, mat[kMatrices], end;
-  int parts, ops;
-  Op op[kMaxOps];
+  int parts;
+  bool may_group;
 };
 
-// The offsets do not depend on the element type or the coefficients (NULL: any), only the products do.
-Layout layout_of(int64_t batch, int64_t rows, int64_t cols, int dtype, const float* coef, int steps) {
+Layout layout_of(int64_t batch, int64_t rows, int64_t cols, int steps) {
   Layout L;
   L.r = std::min(rows, cols);
   L.c = std::max(rows, cols);
   L.ld_c = round_up(L.c, 32);
   L.ld_r = round_up(L.r, 32);
-  static const float ones[3 * kMaxSteps] = {};
-  L.ops = list_ops(L.r, L.c, rows > cols, dtype != LM_F32, coef != nullptr ? coef : ones, steps, L.op);
+  L.may_group = 4 * L.c >= 5 * L.r && steps > 1;
   // About 8 K values for each CTA of the norm, and no more CTAs than give each SM four.
   const int64_t want = std::min<int64_t>(ceil_div(rows * cols, 8192), ceil_div(4 * kSmCount, batch > 0 ? batch : 1));
   L.parts = (int)std::max<int64_t>(1, want);
@@ -926,9 +923,8 @@ Layout layout_of(int64_t batch, int64_t rows, int64_t cols, int dtype, const flo
   L.scale = take(sizeof(Scale) * batch * kMaxOps);
   const size_t x = sizeof(__half) * 2 * batch * L.r * L.ld_c, xt = sizeof(__half) * 2 * batch * L.c * L.ld_r;
   const size_t sq = sizeof(__half) * 2 * batch * L.r * L.ld_r;
-  const bool grouped = 4 * L.c >= 5 * L.r && steps > 1;
   for (int m = 0; m < kMatrices; ++m) {
-    const bool used = m <= mA || m == mQ0 || grouped;  // the others belong to groups of steps
+    const bool used = m <= mA || m == mQ0 || L.may_group;  // the others belong to groups of steps
     L.mat[m] = !used ? L.mat[mA] : take(m == mX ? x : m <= mXT1 ? xt : sq);
   }
   L.end = off;
@@ -1001,26 +997,37 @@ cudaError_t launch_iteration(IterArgs& it, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, k, it);
 }
 
-// The tile width with the least estimated time, in cycles.  A slice of 64 costs a pair the larger of its
-// 12 MMAs (6 BN cycles) and its operands' way into shared memory (64 bytes a cycle and CTA: 1024, 768 and
-// 640 for BN = 256, 128 and 64; 850 for 128 with every SM at it).  A product ends with the epilogue of a
-// tile, which nothing hides: 150 BN.  Measured for 64, 128 and 256: four of 256 x 256: 134, 207 and 374
-// us; 2048 x 4096: 960, 835 and 1110; 4096 x 8192 (not grouped): 7.1, 5.6 and 5.3 ms.
-int tile_width(const IterArgs& it) {
-  const int64_t pairs = device_sm_count() / 2;
+// Estimated time of the products with tiles of width bn, in cycles.  A slice of 64 costs a pair the larger
+// of its 12 MMAs (6 bn cycles) and its operands' way into shared memory (64 bytes a cycle and CTA: 1024, 768
+// and 640 for bn = 256, 128 and 64; 850 for 128 with every SM at it).  A product ends with what nothing
+// hides, the epilogue of a tile and the wait for the other CTAs: 6000 + 130 bn.  Measured for 64, 128
+// and 256: four of 256 x 256: 134, 207 and 374 us; 2048 x 4096: 960, 835 and 1110; 4096 x 8192 (not
+// grouped): 7.1, 5.6 and 5.3 ms.
+int64_t estimate(const IterArgs& it, const Op* op, int ops, int bn) {
+  const int64_t pairs = device_sm_count() / 2, slice = bn == 256 ? 1536 : bn == 128 ? 850 : 640;
+  int64_t cost = 0;
+  for (int i = 0; i < ops; ++i) {
+    const Split &p = it.mat[op[i].p], &q = it.mat[op[i].q];
+    cost += ceil_div(tiles_of(p.rows, q.rows, bn, op[i].out_kind) * it.batch, pairs) * ceil_div(p.cols, BK) * slice + 6000 + 130 * bn;
+  }
+  return cost;
+}
+
+// The products and the tile width with the least estimated time.
+int plan(IterArgs& it, bool tall, bool whole, bool may_group, const float* coef, int steps) {
+  Op op[kMaxOps];
   int best = 0;
   int64_t least = 0;
-  for (const int bn : {256, 128, 64}) {
-    const int64_t slice = bn == 256 ? 1536 : bn == 128 ? 850 : 640;
-    int64_t cost = 0;
-    for (int i = 0; i < it.ops; ++i) {
-      const Split &p = it.mat[it.op[i].p], &q = it.mat[it.op[i].q];
-      cost += ceil_div(tiles_of(p.rows, q.rows, bn, it.op[i].out_kind) * it.batch, pairs) * ceil_div(p.cols, BK) * slice +
-              150 * bn;
-    }
-    if (best == 0 || cost < least) {
-      best = bn;
-      least = cost;
+  for (int grouped = 0; grouped <= (whole && may_group ? 1 : 0); ++grouped) {
+    const int ops = list_ops(tall, whole, grouped != 0, coef, steps, op);
+    for (const int bn : {256, 128, 64}) {
+      const int64_t cost = estimate(it, op, ops, bn);
+      if (best == 0 || cost < least) {
+        best = bn;
+        least = cost;
+        it.ops = ops;
+        std::copy(op, op + ops, it.op);
+      }
     }
   }
   return best;
@@ -1029,14 +1036,14 @@ int tile_width(const IterArgs& it) {
 }  // namespace
 
 size_t ortho_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int steps) {
-  return layout_of(batch, rows, cols, LM_F32, nullptr, steps).end;
+  return layout_of(batch, rows, cols, steps).end;
 }
 
 int ortho_max_steps() { return kMaxSteps; }
 
 cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaStream_t stream) {
   if (o.batch == 0 || o.rows == 0 || o.cols == 0) return cudaSuccess;
-  const Layout L = layout_of(o.batch, o.rows, o.cols, o.dtype, o.coefficients, o.steps);
+  const Layout L = layout_of(o.batch, o.rows, o.cols, o.steps);
   const bool tall = o.rows > o.cols;
   int* status = ws_at<int>(o.workspace, L.status);
   IterArgs it{};
@@ -1049,6 +1056,9 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
     s.hi = ws_at<__half>(o.workspace, L.mat[m]);
     s.lo = s.hi + o.batch * s.matrix;
   }
+  const bool whole = o.dtype != LM_F32;
+  it.batch = (int)o.batch;
+  const int bn = plan(it, tall, whole, L.may_group, o.coefficients, o.steps);
 
   PrepArgs p{};
   p.g = o.update;
@@ -1057,12 +1067,12 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
   p.row_stride = o.row_stride;
   p.matrix_stride = o.matrix_stride;
   p.parts = L.parts;
-  p.ops = L.ops;
-  p.whole = o.dtype != LM_F32;
+  p.ops = it.ops;
+  p.whole = whole;
   p.eps = o.eps;
   for (int k = 0; k < o.steps; ++k)
     for (int e = 0; e < 3; ++e) p.coef[k][e] = o.coefficients[3 * k + e];
-  for (int i = 0; i < L.ops; ++i) p.kind[i] = L.op[i].kind;
+  for (int i = 0; i < it.ops; ++i) p.kind[i] = it.op[i].kind;
   p.part = ws_at<double>(o.workspace, L.part);
   p.scale = ws_at<Scale>(o.workspace, L.scale);
   const Split& g = it.mat[tall ? mXT0 : mX];
@@ -1095,9 +1105,6 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
   cudaError_t e = o.dtype == LM_F32 ? by_pack(float{}) : o.dtype == LM_BF16 ? by_pack(__nv_bfloat16{}) : by_pack(__half{});
   if (e != cudaSuccess) return e;
 
-  it.ops = L.ops;
-  std::copy(L.op, L.op + L.ops, it.op);
-  it.batch = (int)o.batch;
   it.run = o.dtype == LM_F32 ? 3 : o.dtype == LM_F16 ? 16 : 32;
   it.out = o.out;
   it.ld_out = o.cols;
@@ -1108,7 +1115,6 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
   it.status = status;
   it.timeout_ns = wc.timeout_ns;
   it.debug_skip_first_load = wc.debug_skip_first_load;
-  const int bn = tile_width(it);
   e = bn == 256 ? launch_iteration<256>(it, stream) : bn == 128 ? launch_iteration<128>(it, stream) : launch_iteration<64>(it, stream);
   if (e != cudaSuccess) return e;
   note_launches(3);
