@@ -51,11 +51,12 @@ RBF_API int ln_sm100_backward(const void* dy, int64_t dy_stride, const void* x, 
  * elements: T positions of each sequence.  labels [rows] int64: a vocabulary index, or
  * ignore_index for a row that is not scored (its logits are not read).
  *   logprob[r] = x[label] - log sum_j exp(x[j])     (0 for a row that is not scored)
+ * rest [rows] receives what fp32 drops of logprob, for the losses (NULL: not kept).
  * stats [rows, 2] fp32 receives the row's maximum and 1 / sum_j exp(x[j] - maximum) (NULL: not
  * kept).  A label that is neither ignore_index nor in [0, V) gives NaN. */
 RBF_API int lp_sm100_forward(const void* logits, int64_t batch_stride, int64_t t_stride,
-                             const int64_t* labels, float* logprob, float* stats, int64_t rows,
-                             int64_t T, int64_t V, int64_t ignore_index, int dtype,
+                             const int64_t* labels, float* logprob, float* rest, float* stats,
+                             int64_t rows, int64_t T, int64_t V, int64_t ignore_index, int dtype,
                              rbf_stream_t stream);
 
 /* dlogits[r, j] = c_r * ((j == label_r) - exp(x[j] - max_r) * inv_r),
@@ -69,7 +70,8 @@ RBF_API int lp_sm100_backward(const void* logits, int64_t batch_stride, int64_t 
                               rbf_stream_t stream);
 
 /* ---- losses on log-probabilities [B, T] ----------------------------------------------------
- * Sums over tokens and over the batch are taken in 64 bits in a fixed order. */
+ * Sums over tokens and over the batch are taken in 64 bits in a fixed order.  The log-probabilities
+ * are logprob + rest, as lp_sm100_forward leaves them (rest may be NULL: 0). */
 
 /* Bytes of the workspace of either loss. */
 RBF_API size_t loss_sm100_workspace_bytes(int64_t B, int64_t T);
@@ -79,8 +81,8 @@ RBF_API size_t loss_sm100_workspace_bytes(int64_t B, int64_t T);
  *   z_p = reward_p - reward_{B/2+p}
  *   loss = mean_p [ -(1 - s) log sigmoid(z_p) - s log sigmoid(-z_p) ],   s = label_smoothing
  * reward [B], loss [1]; coef [B, T] receives d loss / d logprob for lp_sm100_backward. */
-RBF_API int pref_sm100_loss(const float* logprob, const float* ref_logprob, const int64_t* labels,
-                            float* loss, float* reward, float* coef, int64_t B, int64_t T,
+RBF_API int pref_sm100_loss(const float* logprob, const float* rest, const float* ref_logprob,
+                            const int64_t* labels, float* loss, float* reward, float* coef, int64_t B, int64_t T,
                             float beta, float label_smoothing, int64_t ignore_index,
                             void* workspace, size_t workspace_bytes, rbf_stream_t stream);
 
@@ -90,7 +92,7 @@ RBF_API int pref_sm100_loss(const float* logprob, const float* ref_logprob, cons
  * A = advantage[b] ([B], per_token = 0) or advantage[b, t] ([B, T], per_token = 1).
  * loss [1] and kl [1] (the mean of kl); coef [B, T] receives count * d loss / d logprob and norm
  * [1] receives 1 / count (pass it to lp_sm100_backward as a scale). */
-RBF_API int policy_sm100_loss(const float* logprob, const float* old_logprob,
+RBF_API int policy_sm100_loss(const float* logprob, const float* rest, const float* old_logprob,
                               const float* ref_logprob, const float* advantage, int per_token,
                               const int64_t* labels, float* loss, float* kl, float* coef,
                               float* norm, int64_t B, int64_t T, float clip_low, float clip_high,

@@ -213,8 +213,8 @@ Logits check_logits(const Tensor& logits, const Tensor& labels) {
   return l;
 }
 
-void logprob_forward(const Logits& l, float* logprob, float* stats, int64_t ignore_index) {
-  check(lp_sm100_forward(ptr(l.x), l.batch_stride, l.t_stride, iptr(l.labels), logprob, stats, l.rows, l.T, l.V,
+void logprob_forward(const Logits& l, float* logprob, float* rest, float* stats, int64_t ignore_index) {
+  check(lp_sm100_forward(ptr(l.x), l.batch_stride, l.t_stride, iptr(l.labels), logprob, rest, stats, l.rows, l.T, l.V,
                          ignore_index, l.dtype, stream_of(l.x)),
         "lp_sm100_forward");
 }
@@ -236,7 +236,7 @@ std::pair<Tensor, Tensor> token_logprob_forward(const Tensor& logits, const Tens
   const c10::cuda::CUDAGuard guard(logits.device());
   Tensor lp = fp32(labels.sizes(), logits);
   Tensor stats = keep ? fp32({l.rows, 2}, logits) : Tensor();
-  logprob_forward(l, fptr(lp), fptr(stats), ignore_index);
+  logprob_forward(l, fptr(lp), nullptr, fptr(stats), ignore_index);
   return {lp, stats};
 }
 
@@ -280,17 +280,19 @@ Tensor constant(const Tensor& t, at::IntArrayRef shape, const char* name, const 
   return t.contiguous();
 }
 
-// What a loss keeps for its backward, in one allocation of 4 rows + 1 floats: the log-probabilities,
-// the coefficients d loss / d logprob, the rows' statistics and a common factor.
+// What a loss keeps for its backward, in one allocation: a common factor, the log-probabilities (and what
+// fp32 drops of them), the coefficients d loss / d logprob, and the rows' statistics.
 struct LossState {
   Tensor all;
-  float *logprob, *coef, *stats, *norm;
+  float *norm, *stats, *logprob, *rest, *coef;
+  static int64_t size(int64_t rows) { return 4 + 5 * rows; }
   explicit LossState(const Tensor& state) : all(state) {
-    const int64_t n = (state.numel() - 4) / 4;
+    const int64_t n = (state.numel() - 4) / 5;
     norm = fptr(state);
-    logprob = norm + 4;
-    coef = logprob + n;
-    stats = coef + n;  // pairs: 8-byte aligned for every n, since 4 + 2 n is even
+    stats = norm + 4;  // pairs, 8-byte aligned
+    logprob = stats + 2 * n;
+    rest = logprob + n;
+    coef = rest + n;
   }
 };
 
@@ -306,12 +308,12 @@ LossOut preference_forward(const Tensor& logits, const Tensor& labels, const Ten
   const Tensor ref = constant(ref_logprob, labels.sizes(), "ref_logprob", labels);
   const c10::cuda::CUDAGuard guard(logits.device());
   const int64_t B = logits.size(0), T = logits.size(1);
-  LossOut o{fp32({}, logits), fp32({B}, logits), fp32({4 * l.rows + 4}, logits)};
+  LossOut o{fp32({}, logits), fp32({B}, logits), fp32({LossState::size(l.rows)}, logits)};
   const LossState s(o.state);
   const size_t bytes = loss_sm100_workspace_bytes(B, T);
   const Tensor ws = workspace(bytes, logits);
-  logprob_forward(l, s.logprob, s.stats, ignore_index);
-  check(pref_sm100_loss(s.logprob, fptr(ref), iptr(l.labels), fptr(o.loss), fptr(o.second), s.coef, B, T, (float)beta,
+  logprob_forward(l, s.logprob, s.rest, s.stats, ignore_index);
+  check(pref_sm100_loss(s.logprob, s.rest, fptr(ref), iptr(l.labels), fptr(o.loss), fptr(o.second), s.coef, B, T, (float)beta,
                         (float)smoothing, ignore_index, ptr(ws), bytes, stream_of(logits)),
         "pref_sm100_loss");
   return o;
@@ -327,12 +329,12 @@ LossOut policy_forward(const Tensor& logits, const Tensor& labels, const Tensor&
   const Tensor adv = constant(advantage, labels.sizes().slice(0, advantage.dim()), "advantage", labels);
   const c10::cuda::CUDAGuard guard(logits.device());
   const int64_t B = logits.size(0), T = logits.size(1);
-  LossOut o{fp32({}, logits), fp32({}, logits), fp32({4 * l.rows + 4}, logits)};
+  LossOut o{fp32({}, logits), fp32({}, logits), fp32({LossState::size(l.rows)}, logits)};
   const LossState s(o.state);
   const size_t bytes = loss_sm100_workspace_bytes(B, T);
   const Tensor ws = workspace(bytes, logits);
-  logprob_forward(l, s.logprob, s.stats, ignore_index);
-  check(policy_sm100_loss(s.logprob, fptr(old), fptr(ref), fptr(adv), advantage.dim() == 2, iptr(l.labels), fptr(o.loss),
+  logprob_forward(l, s.logprob, s.rest, s.stats, ignore_index);
+  check(policy_sm100_loss(s.logprob, s.rest, fptr(old), fptr(ref), fptr(adv), advantage.dim() == 2, iptr(l.labels), fptr(o.loss),
                           fptr(o.second), s.coef, s.norm, B, T, (float)clip_low, (float)clip_high, (float)kl_coef,
                           ignore_index, ptr(ws), bytes, stream_of(logits)),
         "policy_sm100_loss");
@@ -342,7 +344,7 @@ LossOut policy_forward(const Tensor& logits, const Tensor& labels, const Tensor&
 // The gradient of a loss for the upstream gradient g of its scalar.
 Tensor loss_backward(const Tensor& logits, const Tensor& labels, const Tensor& state, const Tensor& g, bool normed,
                      int64_t ignore_index) {
-  TORCH_CHECK(state.numel() == 4 * labels.numel() + 4 && state.scalar_type() == at::kFloat && state.is_contiguous(),
+  TORCH_CHECK(state.numel() == LossState::size(labels.numel()) && state.scalar_type() == at::kFloat && state.is_contiguous(),
               "state must be the loss's forward's");
   if (g.defined())
     TORCH_CHECK(g.numel() == 1 && g.scalar_type() == at::kFloat && g.device() == logits.device(),

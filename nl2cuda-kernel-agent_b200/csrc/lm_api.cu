@@ -149,13 +149,14 @@ int ln_sm100_backward(const void* dy, int64_t dy_stride, const void* x, int64_t 
 }
 
 int lp_sm100_forward(const void* logits, int64_t batch_stride, int64_t t_stride,
-                     const int64_t* labels, float* logprob, float* stats, int64_t rows, int64_t T,
-                     int64_t V, int64_t ignore_index, int dtype, rbf_stream_t stream) {
+                     const int64_t* labels, float* logprob, float* rest, float* stats, int64_t rows,
+                     int64_t T, int64_t V, int64_t ignore_index, int dtype, rbf_stream_t stream) {
   int st = check_logits(batch_stride, t_stride, rows, T, V, dtype);
   if (st) return st;
   if ((st = need(logits, rows * V, elem_bytes(dtype), "logits"))) return st;
   if ((st = need(labels, rows, 8, "labels"))) return st;
   if ((st = need(logprob, rows, 4, "logprob"))) return st;
+  if (rest != nullptr && (st = need(rest, rows, 4, "rest"))) return st;
   if (stats != nullptr && (st = need(stats, rows, 8, "stats"))) return st;
   if ((st = check_device())) return st;
   LogitArgs a{};
@@ -169,6 +170,7 @@ int lp_sm100_forward(const void* logits, int64_t batch_stride, int64_t t_stride,
   a.ignore_index = ignore_index;
   a.dtype = dtype;
   a.logprob = logprob;
+  a.rest = rest;
   a.stats = stats;
   return cuda_status(launch_logprob_forward(a, as_stream(stream)), "log-probability launch");
 }
@@ -211,7 +213,7 @@ size_t loss_sm100_workspace_bytes(int64_t B, int64_t T) {
   return loss_workspace_bytes(B, T);
 }
 
-int pref_sm100_loss(const float* logprob, const float* ref_logprob, const int64_t* labels,
+int pref_sm100_loss(const float* logprob, const float* rest, const float* ref_logprob, const int64_t* labels,
                     float* loss, float* reward, float* coef, int64_t B, int64_t T, float beta,
                     float label_smoothing, int64_t ignore_index, void* workspace,
                     size_t workspace_bytes, rbf_stream_t stream) {
@@ -222,6 +224,7 @@ int pref_sm100_loss(const float* logprob, const float* ref_logprob, const int64_
   if (!(label_smoothing >= 0.f && label_smoothing <= 1.f))
     return refuse(RBF_ERR_INVALID_ARGUMENT, "label_smoothing must be in [0, 1]");
   if ((st = need(logprob, B * T, 4, "logprob"))) return st;
+  if (rest != nullptr && (st = need(rest, B * T, 4, "rest"))) return st;
   if ((st = need(ref_logprob, B * T, 4, "ref_logprob"))) return st;
   if ((st = need(labels, B * T, 8, "labels"))) return st;
   if ((st = need(loss, 1, 4, "loss"))) return st;
@@ -231,6 +234,7 @@ int pref_sm100_loss(const float* logprob, const float* ref_logprob, const int64_
   if ((st = check_device())) return st;
   LossArgs a{};
   a.logprob = logprob;
+  a.rest = rest;
   a.ref_logprob = ref_logprob;
   a.labels = labels;
   a.loss = loss;
@@ -245,7 +249,7 @@ int pref_sm100_loss(const float* logprob, const float* ref_logprob, const int64_
   return cuda_status(launch_loss(a, true, as_stream(stream)), "preference loss launch");
 }
 
-int policy_sm100_loss(const float* logprob, const float* old_logprob, const float* ref_logprob,
+int policy_sm100_loss(const float* logprob, const float* rest, const float* old_logprob, const float* ref_logprob,
                       const float* advantage, int per_token, const int64_t* labels, float* loss,
                       float* kl, float* coef, float* norm, int64_t B, int64_t T, float clip_low,
                       float clip_high, float kl_coef, int64_t ignore_index, void* workspace,
@@ -256,6 +260,7 @@ int policy_sm100_loss(const float* logprob, const float* old_logprob, const floa
     return refuse(RBF_ERR_INVALID_ARGUMENT, "clip_low and clip_high must be >= 0");
   if (!std::isfinite(kl_coef)) return refuse(RBF_ERR_INVALID_ARGUMENT, "kl_coef is not finite");
   if ((st = need(logprob, B * T, 4, "logprob"))) return st;
+  if (rest != nullptr && (st = need(rest, B * T, 4, "rest"))) return st;
   if ((st = need(old_logprob, B * T, 4, "old_logprob"))) return st;
   if ((st = need(ref_logprob, B * T, 4, "ref_logprob"))) return st;
   if ((st = need(advantage, per_token ? B * T : B, 4, "advantage"))) return st;
@@ -268,6 +273,7 @@ int policy_sm100_loss(const float* logprob, const float* old_logprob, const floa
   if ((st = check_device())) return st;
   LossArgs a{};
   a.logprob = logprob;
+  a.rest = rest;
   a.old_logprob = old_logprob;
   a.ref_logprob = ref_logprob;
   a.advantage = advantage;

@@ -37,6 +37,7 @@ struct LogitArgs {
   int64_t rows, T, V, ignore_index;
   int dtype;
   float* logprob;       // forward
+  float* rest;          // what fp32 drops of it, or NULL
   float* stats;         // [rows][2]: maximum, 1 / sum
   const float* coef;    // backward
   const float* scale0;
@@ -48,6 +49,7 @@ cudaError_t launch_logprob_backward(const LogitArgs& a, cudaStream_t stream);
 
 struct LossArgs {
   const float* logprob;
+  const float* rest;
   const float* old_logprob;
   const float* ref_logprob;
   const float* advantage;

@@ -126,9 +126,12 @@ __device__ __forceinline__ void accumulate_packs(MaxSum& v, const Pack<T, VEC> (
 
 template <typename T>
 __device__ __forceinline__ void write_row(const LogitArgs& a, int64_t r, int64_t label, bool scored, const T* x, MaxSum t) {
-  float lp = 0.f;
-  if (scored) lp = label >= 0 && label < a.V ? (to_f32(x[label]) - t.m) - logf(t.s) : NAN;
-  a.logprob[r] = lp;
+  // In 64 bits, and what fp32 drops of it kept for the losses: a reward is the difference of long sums of
+  // these, and the rounding of each (3e-7 at -10) is several times the error of s.
+  double lp = 0.0;
+  if (scored) lp = label >= 0 && label < a.V ? ((double)to_f32(x[label]) - (double)t.m) - log((double)t.s) : (double)NAN;
+  a.logprob[r] = (float)lp;
+  if (a.rest != nullptr) a.rest[r] = isfinite(lp) ? (float)(lp - (double)(float)lp) : 0.f;
   if (a.stats != nullptr) {
     a.stats[2 * r] = t.m;
     a.stats[2 * r + 1] = 1.f / t.s;
@@ -312,6 +315,10 @@ __device__ double block_sum(double v, double* smem) {
   return t;
 }
 
+__device__ __forceinline__ double logprob_at(const LossArgs& a, int64_t i) {
+  return a.rest != nullptr ? (double)a.logprob[i] + (double)a.rest[i] : (double)a.logprob[i];
+}
+
 template <bool PREF>
 __global__ void __launch_bounds__(kLossThreads) loss_kernel(const LossArgs a) {
   __shared__ double smem[32];
@@ -332,11 +339,11 @@ __global__ void __launch_bounds__(kLossThreads) loss_kernel(const LossArgs a) {
       const int64_t i = b * a.T + t;
       const bool scored = a.labels[i] != a.ignore_index;
       if (PREF) {
-        if (scored) s0 += (double)a.logprob[i] - (double)a.ref_logprob[i];
+        if (scored) s0 += logprob_at(a, i) - (double)a.ref_logprob[i];
       } else {
         float c = 0.f;
         if (scored) {
-          const double lp = a.logprob[i];
+          const double lp = logprob_at(a, i);
           const double adv = a.advantage[a.per_token ? i : b];
           const double ratio = exp(lp - (double)a.old_logprob[i]);
           // NaN passes through both (fmin / fmax would drop it).

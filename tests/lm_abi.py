@@ -12,12 +12,12 @@ SIGNATURES = {
     "ln_sm100_backward_workspace_bytes": (_SZ, [_I64, _I64]),
     "ln_sm100_backward": (_I, [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I, _I,
                                _P, _SZ, _P]),
-    "lp_sm100_forward": (_I, [_P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P]),
+    "lp_sm100_forward": (_I, [_P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P]),
     "lp_sm100_backward": (_I, [_P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
                                _I, _P]),
     "loss_sm100_workspace_bytes": (_SZ, [_I64, _I64]),
-    "pref_sm100_loss": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _F, _F, _I64, _P, _SZ, _P]),
-    "policy_sm100_loss": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I64, _I64, _F, _F, _F,
+    "pref_sm100_loss": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _F, _F, _I64, _P, _SZ, _P]),
+    "policy_sm100_loss": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I64, _I64, _F, _F, _F,
                                _I64, _P, _SZ, _P]),
     "ortho_sm100_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I]),
     "ortho_sm100": (_I, [_P, _I64, _I64, _P, _I64, _I64, _I64, ctypes.POINTER(_F), _I, _F, _I, _P,

@@ -64,7 +64,7 @@ def test_layernorm_refusals(lib):
 
 def test_logprob_refusals(lib):
     def fwd(x=A, sb=40, st=8, lab=A, lp=A, rows=10, T=5, V=8, dt=0):
-        return lib.lp_sm100_forward(x, sb, st, lab, lp, None, rows, T, V, -100, dt, None)
+        return lib.lp_sm100_forward(x, sb, st, lab, lp, None, None, rows, T, V, -100, dt, None)
     assert fwd(rows=-1) == INVALID
     assert fwd(T=4) == INVALID
     assert fwd(T=0) == INVALID
@@ -92,7 +92,7 @@ def test_loss_refusals(lib):
     assert size >= 3 * 8 * 4
 
     def pref(B=4, T=10, beta=0.1, s=0.0, lp=A, loss=A, ws=A, n=size):
-        return lib.pref_sm100_loss(lp, A, A, loss, A, A, B, T, beta, s, -100, ws, n, None)
+        return lib.pref_sm100_loss(lp, None, A, A, loss, A, A, B, T, beta, s, -100, ws, n, None)
     assert pref(B=3) == INVALID
     assert pref(B=-2) == INVALID
     assert pref(beta=math.inf) == INVALID
@@ -102,7 +102,7 @@ def test_loss_refusals(lib):
     assert pref(n=size - 1) == WORKSPACE
 
     def pol(lo=0.2, hi=0.2, k=0.0, adv=A, norm=A, ws=A, n=size):
-        return lib.policy_sm100_loss(A, A, A, adv, 0, A, A, A, A, norm, 4, 10, lo, hi, k, -100, ws,
+        return lib.policy_sm100_loss(A, None, A, A, adv, 0, A, A, A, A, norm, 4, 10, lo, hi, k, -100, ws,
                                      n, None)
     assert pol(lo=-0.1) == INVALID and pol(hi=math.nan) == INVALID
     assert pol(k=math.nan) == INVALID
