@@ -47,7 +47,7 @@ int check_ln(int64_t rows, int64_t D, int64_t stride, int dtype, int wdtype) {
 
 int check_logits(int64_t batch_stride, int64_t t_stride, int64_t rows, int64_t T, int64_t V, int dtype) {
   if (rows < 0 || T < 0 || V < 0) return refuse(RBF_ERR_INVALID_ARGUMENT, "negative size");
-  if (rows * 8 >= kMaxRows || V >= kMaxRows) return refuse(RBF_ERR_UNSUPPORTED, "rows >= 2^28 or V >= 2^31");
+  if (rows >= kMaxRows / 8 || V >= kMaxRows) return refuse(RBF_ERR_UNSUPPORTED, "rows >= 2^28 or V >= 2^31");
   if (rows > 0 && (T == 0 || rows % T != 0))
     return refuse(RBF_ERR_INVALID_ARGUMENT, "rows must be a multiple of T");
   if (rows > 0 && V == 0) return refuse(RBF_ERR_INVALID_ARGUMENT, "empty vocabulary");

@@ -400,6 +400,8 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
     }
   };
   stats(ring.row);
+  // Long rows: x and dy are read from shared memory again for dx, since the column sums take 64 registers.
+  constexpr bool AGAIN = NV * VEC * ROWS > 16;
   const float inv_d = 1.f / (float)D;
   T* dx = static_cast<T*>(a.y) + ring.row * D + first;
   const int64_t dx_hop = ring.step * D;
@@ -407,17 +409,22 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
   for (; ring.row < a.rows; ring.advance(), dx += dx_hop) {
     asm volatile("cp.async.wait_group %0;" ::"n"(R::STAGES - 2) : "memory");
     const int n = ring.left(ring.row, a.rows);
-    Pack<T, VEC> x[ROWS][NV], dy[ROWS][NV];
+    Pack<T, VEC> x[AGAIN ? 1 : ROWS][AGAIN ? 1 : NV], dy[AGAIN ? 1 : ROWS][AGAIN ? 1 : NV];
+    auto fetch = [&](int k, int i) {
+      x[AGAIN ? 0 : k][AGAIN ? 0 : i] = ring.read(n, k, i, 0);
+      dy[AGAIN ? 0 : k][AGAIN ? 0 : i] = ring.read(n, k, i, 1);
+    };
+    auto x_of = [&](int k, int i, int e) { return pair_of(x[AGAIN ? 0 : k][AGAIN ? 0 : i], e); };
+    auto dy_of = [&](int k, int i, int e) { return pair_of(dy[AGAIN ? 0 : k][AGAIN ? 0 : i], e); };
     float s[2 * ROWS];
     F2 shift[ROWS], rs[ROWS];
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
       rs[k] = twice(rstd[k]);
       shift[k] = twice(-mean[k]);
+      if (!AGAIN) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        x[k][i] = ring.read(n, k, i, 0);
-        dy[k][i] = ring.read(n, k, i, 1);
+        for (int i = 0; i < NV; ++i) fetch(k, i);
       }
     }
     ring.issue(a.rows);
@@ -429,17 +436,19 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
     for (int i = 0; i < NV; ++i) {
       if (!KEEP) weight(i);
 #pragma unroll
-      for (int k = 0; k < ROWS; ++k)
+      for (int k = 0; k < ROWS; ++k) {
+        if (AGAIN) fetch(k, i);
 #pragma unroll
         for (int e = 0; e < H; ++e) {
-          const F2 h = mul2(add2(pair_of(x[k][i], e), shift[k]), rs[k]);
-          const F2 d = pair_of(dy[k][i], e);  // 0 past D and past the last row
+          const F2 h = mul2(add2(x_of(k, i, e), shift[k]), rs[k]);
+          const F2 d = dy_of(k, i, e);  // 0 past D and past the last row
           const F2 gw = mul2(d, wv[KEEP ? i : 0][e]);
           t0[k] = add2(t0[k], gw);
           t1[k] = fma2(gw, h, t1[k]);
           dw[i][e] = fma2(d, h, dw[i][e]);
           db[i][e] = add2(db[i][e], d);
         }
+      }
     }
     if (a.y == nullptr) continue;
 #pragma unroll
@@ -457,10 +466,11 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
       for (int k = 0; k < ROWS; ++k) {
         const F2 m1 = twice(-s[2 * k] * inv_d), m2 = twice(-s[2 * k + 1] * inv_d);
         Pack<T, VEC> o;
+        if (AGAIN) fetch(k, i);
 #pragma unroll
         for (int e = 0; e < H; ++e) {
-          const F2 h = mul2(add2(pair_of(x[k][i], e), shift[k]), rs[k]);
-          const F2 gw = fma2(pair_of(dy[k][i], e), wv[KEEP ? i : 0][e], m1);
+          const F2 h = mul2(add2(x_of(k, i, e), shift[k]), rs[k]);
+          const F2 gw = fma2(dy_of(k, i, e), wv[KEEP ? i : 0][e], m1);
           set_pair(o, e, mul2(fma2(h, m2, gw), rs[k]));
         }
         if (k < n) store_pack<T, VEC>(out, o);

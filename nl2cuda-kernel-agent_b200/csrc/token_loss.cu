@@ -130,8 +130,9 @@ __device__ __forceinline__ void write_row(const LogitArgs& a, int64_t r, int64_t
   // these, and the rounding of each (3e-7 at -10) is several times the error of s.
   double lp = 0.0;
   if (scored) lp = label >= 0 && label < a.V ? ((double)to_f32(x[label]) - (double)t.m) - log((double)t.s) : (double)NAN;
-  a.logprob[r] = (float)lp;
-  if (a.rest != nullptr) a.rest[r] = isfinite(lp) ? (float)(lp - (double)(float)lp) : 0.f;
+  const float rounded = (float)lp;
+  a.logprob[r] = rounded;
+  if (a.rest != nullptr) a.rest[r] = isfinite(rounded) ? (float)(lp - (double)rounded) : 0.f;
   if (a.stats != nullptr) {
     a.stats[2 * r] = t.m;
     a.stats[2 * r + 1] = 1.f / t.s;
