@@ -26,6 +26,7 @@ namespace {
 constexpr int kLaneElems = 16;                   // values of a row per lane
 constexpr int kWarpElems = 32 * kLaneElems;
 constexpr int64_t kMaxRegD = 32 * kWarpElems;    // longest row held in the registers of one CTA
+constexpr int64_t kLongMin = 8 * kWarpElems;     // longest row of ln_backward_kernel, with 256 threads
 constexpr int kWideThreads = 1024;
 constexpr int kSumRows = 32;                     // partial rows that ln_sum adds side by side
 
@@ -514,8 +515,8 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
 }
 
 // ---- backward, any rows
-template <typename T, int VEC, int NV, int THREADS>
-__global__ void __launch_bounds__(THREADS) ln_backward_kernel(const LnArgs a, int W, int groups) {
+template <typename T, int VEC, int NV>
+__global__ void __launch_bounds__(256) ln_backward_kernel(const LnArgs a, int W, int groups) {
   extern __shared__ float sums[];  // groups > 1: [groups][D] column sums at the end
   __shared__ float2 red[32 * 2 * 8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -616,6 +617,87 @@ __global__ void __launch_bounds__(THREADS) ln_backward_kernel(const LnArgs a, in
       float t = 0.f;
       for (int k = 0; k < groups; ++k) t += sums[k * D + c];
       out[c] = t;
+    }
+  }
+}
+
+// ---- backward, long rows that the ring does not take
+// A CTA takes a row, 16 values a thread; the sums of a thread's own columns are in shared memory
+// (128 KB), at a quarter of the time that the row takes from HBM.  In registers, of which 1024 threads have
+// 64 each, they spilled: 4096 x 12288 fp32 in 136 us in place of 400, 4096 x 9001 bf16 in 137 in place of 1118.
+// From 4096 values on: 8192 x 8191 fp32 in 260 us, 291 with 512 threads and registers; 8192 x 4101 fp32 163, 230;
+// 8192 x 6001 bf16 197, 245; 8192 x 4500 bf16 151, 133.
+constexpr int kLongThreads = 1024;
+constexpr size_t kLongBytes = sizeof(float) * 2 * kLaneElems * kLongThreads;
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kLongThreads, 1) ln_long_backward_kernel(const LnArgs a) {
+  constexpr int NV = kLaneElems / VEC;
+  extern __shared__ float sums[];  // [dw, db][value of the thread][thread]
+  __shared__ float2 red[2 * 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* const dw = sums + threadIdx.x;
+  float* const db = dw + kLaneElems * kLongThreads;
+  int turn = 0;
+  const int D = (int)a.D;
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+#pragma unroll
+  for (int k = 0; k < kLaneElems; ++k) dw[k * kLongThreads] = db[k * kLongThreads] = 0.f;
+  const float inv_d = 1.f / (float)D;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    Row<T, VEC, NV> x, dy;
+    x.load(static_cast<const T*>(a.x) + r * a.x_stride, D, 32, warp, lane);
+    dy.load(static_cast<const T*>(a.dy) + r * a.dy_stride, D, 32, warp, lane);
+    const float mean = a.mean[r], rstd = a.rstd[r];
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = ((i * 32 + warp) * 32 + lane) * VEC;
+      if (c >= D) break;
+      float w[VEC];
+      load_param<VEC>(a.weight, c, a.wdtype, 1.f, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int k = (i * VEC + e) * kLongThreads;
+        const float h = (to_f32(x.p[i].v[e]) - mean) * rstd, d = to_f32(dy.p[i].v[e]);
+        const float gw = d * w[e];
+        s.x += gw;
+        s.y = fmaf(gw, h, s.y);
+        if (a.part != nullptr) {
+          dw[k] = fmaf(d, h, dw[k]);
+          db[k] += d;
+        }
+      }
+    }
+    if (a.y == nullptr) continue;
+    s = group_sum(s, 32, warp, 1, red, turn);
+    const float m1 = s.x * inv_d, m2 = s.y * inv_d;
+    T* dx = static_cast<T*>(a.y) + r * D;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = ((i * 32 + warp) * 32 + lane) * VEC;
+      if (c >= D) break;
+      float w[VEC];
+      load_param<VEC>(a.weight, c, a.wdtype, 1.f, w);
+      Pack<T, VEC> o;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float h = (to_f32(x.p[i].v[e]) - mean) * rstd;
+        o.v[e] = from_f32<T>(rstd * (to_f32(dy.p[i].v[e]) * w[e] - m1 - h * m2));
+      }
+      store_pack<T, VEC>(dx + c, o);
+    }
+  }
+  if (a.part == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = ((i * 32 + warp) * 32 + lane) * VEC;
+    if (c >= D) break;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      a.part[(int64_t)blockIdx.x * D + c + e] = dw[(i * VEC + e) * kLongThreads];
+      a.part[((int64_t)gridDim.x + blockIdx.x) * D + c + e] = db[(i * VEC + e) * kLongThreads];
     }
   }
 }
@@ -893,14 +975,16 @@ cudaError_t launch_ring_forward(const LnArgs& a, cudaStream_t stream) {
   return launch_ring(ln_ring_forward_kernel<T, 4, 2>, a, TW, 2, &parts, stream);
 }
 
-// One pack a thread and two rows: 48 us at that size; one row took 57 us, and two packs or four rows
-// do not fit the registers next to the column sums (70 us and more).
+// As few packs a thread as hold the row, since its column sums take 2 registers a value; two rows a block,
+// four where that leaves 16 values a thread.  8192 x 4096 bf16: 48 us, 57 with one row, 50 with four; fp32: 67 us,
+// 74 with two rows.  8192 x 8192 bf16: 108 us, 139 with one row.
 template <typename T>
 cudaError_t launch_ring_backward(const LnArgs& a, int* parts, cudaStream_t stream) {
   int nv = 1, TW;
   ring_shape<T>(a, &nv, &TW);
-  if (nv == 1) return launch_ring(ln_ring_backward_kernel<T, 1, 2>, a, TW, 2, parts, stream);
-  if (nv == 2) return launch_ring(ln_ring_backward_kernel<T, 2, 1>, a, TW, 1, parts, stream);
+  constexpr int R = sizeof(T) == 4 ? 4 : 2;
+  if (nv == 1) return launch_ring(ln_ring_backward_kernel<T, 1, R>, a, TW, R, parts, stream);
+  if (nv == 2) return launch_ring(ln_ring_backward_kernel<T, 2, 2>, a, TW, 2, parts, stream);
   return launch_ring(ln_ring_backward_kernel<T, 4, 1>, a, TW, 1, parts, stream);
 }
 
@@ -965,22 +1049,25 @@ cudaError_t launch_ln_backward(const LnArgs& a, cudaStream_t stream) {
   } else if (ring_fits(a, true)) {
     e = by_type(a.dtype, [&](auto t) { return launch_ring_backward<decltype(t)>(b, &parts, stream); });
     ++launches;
+  } else if (a.D > kLongMin) {
+    parts = (int)std::min<int64_t>(parts, kSmCount);
+    e = by_type(a.dtype, [&](auto t) {
+      using E = decltype(t);
+      constexpr int V = 16 / sizeof(E);
+      const int vec = pack_elems(a, true);
+      auto k = vec == V ? ln_long_backward_kernel<E, V> : vec == 2 ? ln_long_backward_kernel<E, 2> : ln_long_backward_kernel<E, 1>;
+      if (V == 8 && vec == 4) k = ln_long_backward_kernel<E, 4>;
+      const cudaError_t set = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLongBytes);
+      return set != cudaSuccess ? set : launch_kernel(k, dim3(parts), dim3(kLongThreads), kLongBytes, stream, b);
+    });
+    ++launches;
   } else {
     const Shape s = backward_shape(a, pack_elems(a, true));
     e = by_type(a.dtype, [&](auto t) {
       return by_backward_shape<decltype(t)>(s, [&](auto tt, auto vec, auto nv) {
         const size_t smem = s.groups > 1 && sums ? sizeof(float) * s.groups * a.D : 0;
-        auto go = [&](auto k) {
-          return launch_kernel(k, dim3(parts), dim3(s.threads), smem, stream, b, s.W, s.groups);
-        };
-        using E = decltype(tt);
-        constexpr int V = decltype(vec)::value, N = decltype(nv)::value;
-        if (s.threads <= 256) return go(ln_backward_kernel<E, V, N, 256>);
-        if constexpr (V * N == kLaneElems) {
-          if (s.threads == 512) return go(ln_backward_kernel<E, V, N, 512>);
-          return go(ln_backward_kernel<E, V, N, 1024>);
-        }
-        return cudaErrorInvalidConfiguration;  // unreachable: short rows take 256 threads
+        return launch_kernel(ln_backward_kernel<decltype(tt), decltype(vec)::value, decltype(nv)::value>, dim3(parts),
+                             dim3(s.threads), smem, stream, b, s.W, s.groups);
       });
     });
     ++launches;

@@ -120,6 +120,13 @@ def test_many_rows(rows, D, cuda_device):
     check(*inputs(rows, D, torch.float32, torch.float32, 77))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D", [(310, 9001), (200, 12290), (200, 12292), (330, 6004), (333, 16376)])
+def test_many_long_rows(rows, D, dtype, cuda_device):
+    """More long rows than CTAs, at every alignment."""
+    check(*inputs(rows, D, dtype, dtype, D))
+
+
 def test_strided_and_broadcast_operands(cuda_device):
     """Rows that lie apart, a transposed matrix, a misaligned slice, an expanded dy."""
     from cases.layernorm.op import layer_norm
