@@ -129,25 +129,37 @@ __global__ void __launch_bounds__(THREADS) ln_forward_kernel(const LnArgs a, int
 // an SM are on their way at any time, no registers wait for them, and no thread waits for another's
 // copy.  The rows of a block share each reduction and its barrier.  Arithmetic is on pairs: a value of
 // 16 bits has some 20 issue slots at the rate that HBM delivers them.
+//
+// SHIFT: rows that do not start on 16 bytes.  Of VEC rows one after another each starts at another place in
+// its first 16 bytes, but every VEC-th row at the same, so a CTA takes the rows of one such class: its packs
+// are aligned, and a thread's columns (all `shift` less than its place) stay the same.  What the first and the
+// last pack hold of other rows is set to 0 and not stored.
 constexpr int kRingThreads = 512;
 constexpr size_t kRingBytes = 196608;
 
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// The first `bytes` of 16, and zeros.
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 
 // OPS operands (x; or x and dy) of ROWS rows a block.  Pointers move from block to block: addresses made
 // anew from row and stride took more instructions than the arithmetic.
-template <typename T, int NV, int ROWS, int OPS>
+template <typename T, int NV, int ROWS, int OPS, bool SHIFT>
 struct Ring {
   static constexpr int VEC = 16 / sizeof(T);
   static constexpr int kPieces = ROWS * NV * OPS;  // 16-byte pieces of a thread and block
   static constexpr int kFit = (int)(kRingBytes / (kPieces * 16 * kRingThreads));
   static constexpr int STAGES = kFit > 8 ? 8 : kFit;
   static constexpr uint32_t kPiece = 16 * kRingThreads, kStage = kPieces * kPiece;
+  static constexpr int CLASSES = SHIFT ? VEC : 1;
   static_assert(STAGES >= 3, "ring");
   int g, in, D, pitch;      // pitch: elements between a thread's packs
-  unsigned columns;         // bit i: pack i lies inside the row
+  int cls, shift;           // of this CTA's rows, which are every CLASSES-th from `cls` on
+  unsigned columns, edge;   // bit i: pack i has elements of the row; and others
+  int64_t rows;             // of the class
   int64_t row, step;        // first row of this group's present block, rows from one block to the next
   uint32_t base;            // this thread's slots
   const T* next[OPS];       // this thread's first pack of the next block to copy
@@ -161,27 +173,39 @@ struct Ring {
     in = threadIdx.x - g * TW;
     D = (int)a.D;
     pitch = TW * VEC;
-    columns = 0;
+    cls = SHIFT ? blockIdx.x % CLASSES : 0;
+    shift = SHIFT ? (int)(cls * (a.D % VEC) % VEC) : 0;
+    columns = edge = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) columns |= (i * pitch + in * VEC < D ? 1u : 0u) << i;
-    step = (int64_t)gridDim.x * groups * ROWS;
-    row = next_row = ((int64_t)blockIdx.x * groups + g) * ROWS;
+    for (int i = 0; i < NV; ++i) {
+      columns |= (place(i) < shift + D ? 1u : 0u) << i;
+      if (SHIFT) edge |= (place(i) < shift || place(i) + VEC > shift + D ? 1u : 0u) << i;
+    }
+    rows = (a.rows - cls + CLASSES - 1) / CLASSES;
+    step = (int64_t)((gridDim.x - cls + CLASSES - 1) / CLASSES) * groups * ROWS;
+    row = next_row = ((int64_t)(blockIdx.x / CLASSES) * groups + g) * ROWS;
     base = ptx::smem_u32(smem) + threadIdx.x * 16;
 #pragma unroll
     for (int o = 0; o < OPS; ++o) {
-      stride[o] = st[o];
-      hop[o] = step * st[o];
-      next[o] = op[o] + row * st[o] + in * VEC;
+      stride[o] = CLASSES * st[o];
+      hop[o] = step * stride[o];
+      next[o] = op[o] + cls * st[o] + row * stride[o] - shift + in * VEC;
     }
     in_stage = out_stage = 0;
   }
+  // Where pack i of this thread begins, counted from the row's first pack; whether its element e is the row's.
+  __device__ __forceinline__ int place(int i) const { return i * pitch + in * VEC; }
+  __device__ __forceinline__ bool inside(int i, int e) const { return place(i) + e >= shift && place(i) + e < shift + D; }
+  // Row r of the class in the matrix, and this thread's first element of it in an output.
+  __device__ __forceinline__ int64_t index(int64_t r) const { return cls + r * CLASSES; }
+  __device__ __forceinline__ int64_t out(int64_t r) const { return index(r) * D - shift + in * VEC; }
   // How many of this group's ROWS rows from r on there are.
-  __device__ __forceinline__ int left(int64_t r, int64_t rows) const {
+  __device__ __forceinline__ int left(int64_t r) const {
     const int64_t n = rows - r;
     return n >= ROWS ? ROWS : n > 0 ? (int)n : 0;
   }
-  __device__ __forceinline__ void issue(int64_t rows) {
-    const int n = left(next_row, rows);
+  __device__ __forceinline__ void issue() {
+    const int n = left(next_row);
     const uint32_t at = base + in_stage * kStage;
 #pragma unroll
     for (int o = 0; o < OPS; ++o) {
@@ -191,7 +215,11 @@ struct Ring {
         if (k < n) {
 #pragma unroll
           for (int i = 0; i < NV; ++i)
-            if (columns >> i & 1u) copy_async16(at + ((k * NV + i) * OPS + o) * kPiece, p + i * pitch);
+            if (columns >> i & 1u) {
+              const uint32_t to = at + ((k * NV + i) * OPS + o) * kPiece;
+              if (SHIFT) copy_async16(to, p + i * pitch, min(16, (shift + D - place(i)) * (int)sizeof(T)));
+              else copy_async16(to, p + i * pitch);
+            }
         }
         p += stride[o];
       }
@@ -209,7 +237,37 @@ struct Ring {
       asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
                    : "r"(base + out_stage * kStage + ((k * NV + i) * OPS + o) * kPiece));
     *reinterpret_cast<uint4*>(&p) = u;
+    if (SHIFT && (edge >> i & 1u)) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (!inside(i, e)) p.v[e] = from_f32<T>(0.f);
+    }
     return p;
+  }
+  // Pack i of an output row, and of a parameter (as pairs).
+  __device__ __forceinline__ void store(T* p, int i, const Pack<T, VEC>& v) const {
+    if (SHIFT && (edge >> i & 1u)) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (inside(i, e)) p[e] = v.v[e];
+    } else {
+      store_pack<T, VEC>(p, v);
+    }
+  }
+  __device__ __forceinline__ void param(const void* w, int i, int dtype, float absent, F2 (&v)[VEC / 2]) const {
+    if constexpr (!SHIFT) {
+      load_param<VEC>(w, place(i), dtype, absent, v);
+    } else {
+      float f[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float one[1] = {0.f};
+        if (inside(i, e)) load_param<1>(w, place(i) + e - shift, dtype, absent, one);
+        f[e] = one[0];
+      }
+#pragma unroll
+      for (int e = 0; e < VEC / 2; ++e) v[e] = f2(f[2 * e], f[2 * e + 1]);
+    }
   }
   __device__ __forceinline__ void advance() {
     row += step;
@@ -259,27 +317,27 @@ __device__ __forceinline__ float total(F2 x) {
 }
 __device__ __forceinline__ F2 twice(float x) { return f2(x, x); }
 
-template <typename T, int NV, int ROWS>
+template <typename T, int NV, int ROWS, bool SHIFT>
 __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const LnArgs a, int TW) {
-  using R = Ring<T, NV, ROWS, 1>;
+  using R = Ring<T, NV, ROWS, 1, SHIFT>;
   constexpr int VEC = R::VEC, H = VEC / 2;
   extern __shared__ uint4 smem[];
   __shared__ float red[2][kRingThreads / 32][ROWS];
   const T* const op[1] = {static_cast<const T*>(a.x)};
   const int64_t stride[1] = {a.x_stride};
   R ring(smem, a, TW, op, stride);
-  const int W = TW / 32, first = ring.in * VEC;
+  const int W = TW / 32;
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
 #pragma unroll
-  for (int s = 0; s < R::STAGES - 1; ++s) ring.issue(a.rows);
+  for (int s = 0; s < R::STAGES - 1; ++s) ring.issue();
   // Weight and bias of a thread's columns: in registers where they suffice, else read again (from L1).
   constexpr bool KEEP = NV * VEC <= 8;
   F2 wv[KEEP ? NV : 1][H], bv[KEEP ? NV : 1][H];
   auto params = [&](int i) {
     if (ring.columns >> i & 1u) {
-      load_param<VEC>(a.weight, i * ring.pitch + first, a.wdtype, 1.f, wv[KEEP ? i : 0]);
-      load_param<VEC>(a.bias, i * ring.pitch + first, a.wdtype, 0.f, bv[KEEP ? i : 0]);
+      ring.param(a.weight, i, a.wdtype, 1.f, wv[KEEP ? i : 0]);
+      ring.param(a.bias, i, a.wdtype, 0.f, bv[KEEP ? i : 0]);
     }
   };
   if (KEEP) {
@@ -287,14 +345,14 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const 
     for (int i = 0; i < NV; ++i) params(i);
   }
   const float inv_d = 1.f / (float)ring.D;
-  T* y = static_cast<T*>(a.y) + ring.row * ring.D + first;
-  const int64_t y_hop = ring.step * ring.D;
+  T* y = static_cast<T*>(a.y) + ring.out(ring.row);
+  const int64_t y_row = (int64_t)R::CLASSES * ring.D, y_hop = ring.step * y_row;
   int turn = 0;
   // Values as they came (16 bits), or converted once where a thread holds few enough of them.
   constexpr bool WIDE = NV * ROWS * VEC <= 32;
-  for (; ring.row < a.rows; ring.advance(), y += y_hop) {
+  for (; ring.row < ring.rows; ring.advance(), y += y_hop) {
     asm volatile("cp.async.wait_group %0;" ::"n"(R::STAGES - 2) : "memory");
-    const int n = ring.left(ring.row, a.rows);
+    const int n = ring.left(ring.row);
     Pack<T, VEC> x[ROWS][NV];
     F2 xw[WIDE ? ROWS : 1][WIDE ? NV : 1][H] = {};
     float s[ROWS], q[ROWS];
@@ -313,7 +371,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const 
       }
       s[k] = total(t);
     }
-    ring.issue(a.rows);
+    ring.issue();
     ring_sum(s, W, ring.g, red, turn);
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
@@ -325,7 +383,12 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const 
         if (ring.columns >> i & 1u) {
 #pragma unroll
           for (int e = 0; e < H; ++e) {
-            const F2 d = add2(value(k, i, e), m);
+            F2 d = add2(value(k, i, e), m);
+            if (SHIFT && (ring.edge >> i & 1u)) {
+              float d0, d1;
+              unpack(d, d0, d1);
+              d = f2(ring.inside(i, 2 * e) ? d0 : 0.f, ring.inside(i, 2 * e + 1) ? d1 : 0.f);
+            }
             if (WIDE) xw[WIDE ? k : 0][WIDE ? i : 0][e] = d;
             t = fma2(d, d, t);
           }
@@ -337,8 +400,8 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const 
     for (int k = 0; k < ROWS; ++k) {
       q[k] = 1.f / sqrtf(q[k] * inv_d + a.eps);  // the reciprocal deviation
       if (ring.in == 0 && k < n && a.mean != nullptr) {
-        a.mean[ring.row + k] = s[k];
-        a.rstd[ring.row + k] = q[k];
+        a.mean[ring.index(ring.row + k)] = s[k];
+        a.rstd[ring.index(ring.row + k)] = q[k];
       }
     }
 #pragma unroll
@@ -355,32 +418,32 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const 
           const F2 d = WIDE ? value(k, i, e) : add2(value(k, i, e), m);
           set_pair(o, e, fma2(mul2(d, rs), wv[KEEP ? i : 0][e], bv[KEEP ? i : 0][e]));
         }
-        if (k < n) store_pack<T, VEC>(out, o);
-        out += ring.D;
+        if (k < n) ring.store(out, i, o);
+        out += y_row;
       }
     }
   }
 }
 
-template <typename T, int NV, int ROWS>
+template <typename T, int NV, int ROWS, bool SHIFT>
 __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const LnArgs a, int TW) {
-  using R = Ring<T, NV, ROWS, 2>;
+  using R = Ring<T, NV, ROWS, 2, SHIFT>;
   constexpr int VEC = R::VEC, H = VEC / 2;
   extern __shared__ uint4 smem[];
   __shared__ float red[2][kRingThreads / 32][2 * ROWS];
   const T* const op[2] = {static_cast<const T*>(a.x), static_cast<const T*>(a.dy)};
   const int64_t stride[2] = {a.x_stride, a.dy_stride};
   R ring(smem, a, TW, op, stride);
-  const int W = TW / 32, D = ring.D, first = ring.in * VEC;
+  const int W = TW / 32, D = ring.D;
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
 #pragma unroll
-  for (int s = 0; s < R::STAGES - 1; ++s) ring.issue(a.rows);
+  for (int s = 0; s < R::STAGES - 1; ++s) ring.issue();
   constexpr bool KEEP = NV * VEC <= 8;
   F2 wv[KEEP ? NV : 1][H], dw[NV][H], db[NV][H];
   auto weight = [&](int i) {
     if (ring.columns >> i & 1u) {
-      load_param<VEC>(a.weight, i * ring.pitch + first, a.wdtype, 1.f, wv[KEEP ? i : 0]);
+      ring.param(a.weight, i, a.wdtype, 1.f, wv[KEEP ? i : 0]);
     } else {
 #pragma unroll
       for (int e = 0; e < H; ++e) wv[KEEP ? i : 0][e] = twice(0.f);
@@ -396,20 +459,20 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
   auto stats = [&](int64_t r) {
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-      mean[k] = r + k < a.rows ? a.mean[r + k] : 0.f;
-      rstd[k] = r + k < a.rows ? a.rstd[r + k] : 0.f;
+      mean[k] = r + k < ring.rows ? a.mean[ring.index(r + k)] : 0.f;
+      rstd[k] = r + k < ring.rows ? a.rstd[ring.index(r + k)] : 0.f;
     }
   };
   stats(ring.row);
   // Long rows: x and dy are read from shared memory again for dx, since the column sums take 64 registers.
   constexpr bool AGAIN = NV * VEC * ROWS > 16;
   const float inv_d = 1.f / (float)D;
-  T* dx = static_cast<T*>(a.y) + ring.row * D + first;
-  const int64_t dx_hop = ring.step * D;
+  T* dx = static_cast<T*>(a.y) + ring.out(ring.row);
+  const int64_t dx_row = (int64_t)R::CLASSES * D, dx_hop = ring.step * dx_row;
   int turn = 0;
-  for (; ring.row < a.rows; ring.advance(), dx += dx_hop) {
+  for (; ring.row < ring.rows; ring.advance(), dx += dx_hop) {
     asm volatile("cp.async.wait_group %0;" ::"n"(R::STAGES - 2) : "memory");
-    const int n = ring.left(ring.row, a.rows);
+    const int n = ring.left(ring.row);
     Pack<T, VEC> x[AGAIN ? 1 : ROWS][AGAIN ? 1 : NV], dy[AGAIN ? 1 : ROWS][AGAIN ? 1 : NV];
     auto fetch = [&](int k, int i) {
       x[AGAIN ? 0 : k][AGAIN ? 0 : i] = ring.read(n, k, i, 0);
@@ -428,7 +491,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
         for (int i = 0; i < NV; ++i) fetch(k, i);
       }
     }
-    ring.issue(a.rows);
+    ring.issue();
     stats(ring.row + ring.step);
     F2 t0[ROWS], t1[ROWS];
 #pragma unroll
@@ -474,8 +537,8 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
           const F2 gw = fma2(dy_of(k, i, e), wv[KEEP ? i : 0][e], m1);
           set_pair(o, e, mul2(fma2(h, m2, gw), rs[k]));
         }
-        if (k < n) store_pack<T, VEC>(out, o);
-        out += D;
+        if (k < n) ring.store(out, i, o);
+        out += dx_row;
       }
     }
   }
@@ -489,12 +552,32 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
     auto& acc = which == 0 ? dw : db;
     float* out = a.part + ((int64_t)which * gridDim.x + blockIdx.x) * D;
     __syncthreads();
+    if (SHIFT) {
+      float* all = reinterpret_cast<float*>(smem);  // [groups][D]
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < H; ++e) {
+          float v[2];
+          unpack(acc[i][e], v[0], v[1]);
+#pragma unroll
+          for (int o = 0; o < 2; ++o)
+            if (ring.inside(i, 2 * e + o)) all[ring.g * D + ring.place(i) + 2 * e + o - ring.shift] = v[o];
+        }
+      __syncthreads();
+      for (int c = threadIdx.x; c < D; c += kRingThreads) {
+        float t = all[c];
+        for (int k = 1; k < groups; ++k) t += all[k * D + c];
+        out[c] = t;
+      }
+      continue;
+    }
     if (ring.g > 0) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         if (!(ring.columns >> i & 1u)) break;
 #pragma unroll
-        for (int e = 0; e < H; ++e) sums[((ring.g - 1) * D + i * ring.pitch + first) / 2 + e] = acc[i][e];
+        for (int e = 0; e < H; ++e) sums[((ring.g - 1) * D + ring.place(i)) / 2 + e] = acc[i][e];
       }
     }
     __syncthreads();
@@ -502,7 +585,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         if (!(ring.columns >> i & 1u)) break;
-        const int c = i * ring.pitch + first;
+        const int c = ring.place(i);
 #pragma unroll
         for (int e = 0; e < H; ++e) {
           F2 t = acc[i][e];
@@ -937,7 +1020,7 @@ int64_t reg_parts(int64_t rows) {
   return rows < most ? (rows > 0 ? rows : 1) : most;
 }
 
-// Rows of whole 16-byte packs, up to 32 KB each, go through the ring: the fewest packs a thread.
+// Rows of whole 16-byte packs, up to 32 KB each, go through the ring.
 // The forward below so many values goes a row at a time: its CTAs then have a block or two each.
 constexpr int64_t kRingForwardMin = 2 * 1024 * 1024;
 bool ring_fits(const LnArgs& a, bool backward) {
@@ -945,18 +1028,31 @@ bool ring_fits(const LnArgs& a, bool backward) {
   return pack_elems(a, backward) * eb == 16 && a.D * eb <= 32768;
 }
 
+// Other rows, where the matrices start on 16 bytes and their rows shift alike, up to 8 values a thread (their
+// parameters stay in registers, since loading them is a load a value).
+constexpr int64_t kShiftMinRows = 64;
+bool shift_fits(const LnArgs& a, bool backward) {
+  const int64_t vec = 16 / (int64_t)elem_bytes(a.dtype);
+  auto ok = [&](const void* p, int64_t stride) {
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (stride - a.D) % vec == 0);
+  };
+  return a.rows >= kShiftMinRows && a.D + vec - 1 <= 8 * kRingThreads && ok(a.x, a.x_stride) && ok(a.y, a.D) &&
+         (!backward || ok(a.dy, a.dy_stride));
+}
+
 // `nv` packs a thread or as many more as 512 threads need, and the threads of a row.
-template <typename T>
+template <typename T, bool SHIFT>
 void ring_shape(const LnArgs& a, int* nv, int* TW) {
   constexpr int VEC = 16 / sizeof(T);
-  while ((int64_t)*nv * VEC * kRingThreads < a.D) *nv *= 2;
+  const int64_t D = SHIFT ? a.D + VEC - 1 : a.D;
+  while ((int64_t)*nv * VEC * kRingThreads < D) *nv *= 2;
   *TW = 32;
-  while ((int64_t)*TW * *nv * VEC < a.D) *TW *= 2;
+  while ((int64_t)*TW * *nv * VEC < D) *TW *= 2;
 }
 
 template <typename K>
-cudaError_t launch_ring(K k, const LnArgs& a, int TW, int rows, int* parts, cudaStream_t stream) {
-  const int64_t blocks = ceil_div(a.rows, (int64_t)(kRingThreads / TW) * rows);
+cudaError_t launch_ring(K k, const LnArgs& a, int classes, int TW, int rows, int* parts, cudaStream_t stream) {
+  const int64_t blocks = classes * ceil_div(ceil_div(a.rows, classes), (int64_t)(kRingThreads / TW) * rows);
   *parts = (int)std::max<int64_t>(1, std::min<int64_t>(blocks, kSmCount));
   const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes);
   if (e != cudaSuccess) return e;
@@ -966,26 +1062,33 @@ cudaError_t launch_ring(K k, const LnArgs& a, int TW, int rows, int* parts, cuda
 // Four rows a block, since each block costs two reductions and their barriers: 8192 x 4096 bf16 in 33 us
 // with two packs a thread and four rows, 54 us with one row, 38 us with one pack (and 512 threads that
 // wait for each other) and four rows.
-template <typename T>
+template <typename T, bool SHIFT>
 cudaError_t launch_ring_forward(const LnArgs& a, cudaStream_t stream) {
-  int nv = a.D > 32 * (16 / (int64_t)sizeof(T)) ? 2 : 1, TW, parts;
-  ring_shape<T>(a, &nv, &TW);
-  if (nv == 1) return launch_ring(ln_ring_forward_kernel<T, 1, 4>, a, TW, 4, &parts, stream);
-  if (nv == 2) return launch_ring(ln_ring_forward_kernel<T, 2, 4>, a, TW, 4, &parts, stream);
-  return launch_ring(ln_ring_forward_kernel<T, 4, 2>, a, TW, 2, &parts, stream);
+  constexpr int VEC = 16 / sizeof(T), classes = SHIFT ? VEC : 1;
+  int nv = a.D > 32 * VEC && !(SHIFT && VEC == 8) ? 2 : 1, TW, parts;
+  ring_shape<T, SHIFT>(a, &nv, &TW);
+  if (nv == 1) return launch_ring(ln_ring_forward_kernel<T, 1, 4, SHIFT>, a, classes, TW, 4, &parts, stream);
+  if constexpr (!SHIFT || VEC == 4) {
+    if (nv == 2) return launch_ring(ln_ring_forward_kernel<T, 2, 4, SHIFT>, a, classes, TW, 4, &parts, stream);
+  }
+  if constexpr (!SHIFT) return launch_ring(ln_ring_forward_kernel<T, 4, 2, false>, a, classes, TW, 2, &parts, stream);
+  return cudaErrorInvalidConfiguration;  // shift_fits() lets no longer rows pass
 }
 
 // As few packs a thread as hold the row, since its column sums take 2 registers a value; two rows a block,
 // four where that leaves 16 values a thread.  8192 x 4096 bf16: 48 us, 57 with one row, 50 with four; fp32: 67 us,
 // 74 with two rows.  8192 x 8192 bf16: 108 us, 139 with one row.
-template <typename T>
+template <typename T, bool SHIFT>
 cudaError_t launch_ring_backward(const LnArgs& a, int* parts, cudaStream_t stream) {
+  constexpr int VEC = 16 / sizeof(T), classes = SHIFT ? VEC : 1, R = sizeof(T) == 4 ? 4 : 2;
   int nv = 1, TW;
-  ring_shape<T>(a, &nv, &TW);
-  constexpr int R = sizeof(T) == 4 ? 4 : 2;
-  if (nv == 1) return launch_ring(ln_ring_backward_kernel<T, 1, R>, a, TW, R, parts, stream);
-  if (nv == 2) return launch_ring(ln_ring_backward_kernel<T, 2, 2>, a, TW, 2, parts, stream);
-  return launch_ring(ln_ring_backward_kernel<T, 4, 1>, a, TW, 1, parts, stream);
+  ring_shape<T, SHIFT>(a, &nv, &TW);
+  if (nv == 1) return launch_ring(ln_ring_backward_kernel<T, 1, R, SHIFT>, a, classes, TW, R, parts, stream);
+  if constexpr (!SHIFT || VEC == 4) {
+    if (nv == 2) return launch_ring(ln_ring_backward_kernel<T, 2, 2, SHIFT>, a, classes, TW, 2, parts, stream);
+  }
+  if constexpr (!SHIFT) return launch_ring(ln_ring_backward_kernel<T, 4, 1, false>, a, classes, TW, 1, parts, stream);
+  return cudaErrorInvalidConfiguration;  // shift_fits() lets no longer rows pass
 }
 
 }  // namespace
@@ -1005,7 +1108,9 @@ cudaError_t launch_ln_forward(const LnArgs& a, cudaStream_t stream) {
       return launch_kernel(k, dim3(grid), dim3(kWideThreads), 0, stream, a);
     });
   } else if (ring_fits(a, false) && a.rows * a.D >= kRingForwardMin) {
-    e = by_type(a.dtype, [&](auto t) { return launch_ring_forward<decltype(t)>(a, stream); });
+    e = by_type(a.dtype, [&](auto t) { return launch_ring_forward<decltype(t), false>(a, stream); });
+  } else if (shift_fits(a, false) && a.rows * a.D >= kRingForwardMin) {
+    e = by_type(a.dtype, [&](auto t) { return launch_ring_forward<decltype(t), true>(a, stream); });
   } else {
     const Shape s = forward_shape(a);
     const unsigned grid = (unsigned)ceil_div(a.rows, s.groups);
@@ -1047,7 +1152,10 @@ cudaError_t launch_ln_backward(const LnArgs& a, cudaStream_t stream) {
       ++launches;
     }
   } else if (ring_fits(a, true)) {
-    e = by_type(a.dtype, [&](auto t) { return launch_ring_backward<decltype(t)>(b, &parts, stream); });
+    e = by_type(a.dtype, [&](auto t) { return launch_ring_backward<decltype(t), false>(b, &parts, stream); });
+    ++launches;
+  } else if (shift_fits(a, true)) {
+    e = by_type(a.dtype, [&](auto t) { return launch_ring_backward<decltype(t), true>(b, &parts, stream); });
     ++launches;
   } else if (a.D > kLongMin) {
     parts = (int)std::min<int64_t>(parts, kSmCount);

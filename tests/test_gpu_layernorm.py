@@ -127,6 +127,27 @@ def test_many_long_rows(rows, D, dtype, cuda_device):
     check(*inputs(rows, D, dtype, dtype, D))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D", [(64, 1), (65, 7), (71, 31), (64, 255), (4099, 1023), (2100, 1001), (1200, 2041), (1200, 2042),
+                                    (700, 4085), (700, 4089), (700, 4090), (530, 4094), (20000, 129), (530, 4095)])
+def test_unaligned_rows(rows, D, dtype, cuda_device):
+    """Rows that begin anywhere in 16 bytes, at the ends of what a CTA's threads hold."""
+    check(*inputs(rows, D, dtype, dtype, D))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_unaligned_rows_apart(dtype, cuda_device):
+    """Rows with gaps that shift like contiguous ones, or not; a first row off 16 bytes; nothing of the gaps
+    (NaN) reaches a result."""
+    x, w, b, dy = inputs(900, 2600 + 3, dtype, dtype, 3)
+    for gap, first in ((8, 0), (16, 0), (5, 0), (8, 8), (8, 3)):
+        big = torch.full((900, 2603 + gap), float("nan"), dtype=dtype, device=x.device)
+        wide = big.reshape(-1)[first:first + 899 * (2603 + gap) + 2603].as_strided((900, 2603), (2603 + gap, 1))
+        wide.copy_(x)
+        check(wide, w, b, dy)
+        check(x, w, None, wide)
+
+
 def test_strided_and_broadcast_operands(cuda_device):
     """Rows that lie apart, a transposed matrix, a misaligned slice, an expanded dy."""
     from cases.layernorm.op import layer_norm
