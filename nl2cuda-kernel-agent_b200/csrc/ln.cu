@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(THREADS) ln_forward_kernel(const LnArgs a, int
 }
 
 // ---- rows of whole 16-byte packs, and enough of them: one CTA per SM
-// `TW` threads (a group) take ROWS rows at a time, each thread NV packs of a row.  A thread copies
+// `TW` threads (a group, whole warps) take ROWS rows at a time, each thread NV packs of a row; threads that no
+// group has room for only wait for the end.  A thread copies
 // what it will read itself into shared memory (cp.async), a ring of blocks ahead: 160 to 190 KB
 // an SM are on their way at any time, no registers wait for them, and no thread waits for another's
 // copy.  The rows of a block share each reduction and its barrier.  Arithmetic is on pairs: a value of
@@ -133,7 +134,9 @@ __global__ void __launch_bounds__(THREADS) ln_forward_kernel(const LnArgs a, int
 // SHIFT: rows that do not start on 16 bytes.  Of VEC rows one after another each starts at another place in
 // its first 16 bytes, but every VEC-th row at the same, so a CTA takes the rows of one such class: its packs
 // are aligned, and a thread's columns (all `shift` less than its place) stay the same.  What the first and the
-// last pack hold of other rows is set to 0 and not stored.
+// last pack hold of other rows is set to 0 and not stored.  8192 x 1023 bf16, forward and backward: 20 and 26 us, 49 and
+// 41 with loads of single values; 4-byte and 8-byte packs were slower from 64 rows on as well (8192 x 4084 bf16: 56 and
+// 60 us, 68 and 75).
 constexpr int kRingThreads = 512;
 constexpr size_t kRingBytes = 196608;
 
@@ -184,6 +187,10 @@ struct Ring {
     rows = (a.rows - cls + CLASSES - 1) / CLASSES;
     step = (int64_t)((gridDim.x - cls + CLASSES - 1) / CLASSES) * groups * ROWS;
     row = next_row = ((int64_t)(blockIdx.x / CLASSES) * groups + g) * ROWS;
+    if (g >= groups) {
+      columns = 0;
+      row = next_row = rows;
+    }
     base = ptx::smem_u32(smem) + threadIdx.x * 16;
 #pragma unroll
     for (int o = 0; o < OPS; ++o) {
@@ -277,10 +284,12 @@ struct Ring {
 
 // Sums of N values (a power of two) over a group's W warps.  In a warp each step hands half of the
 // values to the other half of the lanes, so that N values take N + 5 - log2 N exchanges in place of
-// 5 N.  red: [2][warps of the CTA][N], used in turn, so that one barrier is enough.
+// 5 N.  slots: this group's 2^k >= W of [2][kRingSlots][N], used in turn, so that one barrier is enough; those
+// past W hold zeros.
+constexpr int kRingSlots = 2 * kRingThreads / 32;
 template <int N>
-__device__ __forceinline__ void ring_sum(float (&s)[N], int W, int g, float (*red)[kRingThreads / 32][N], int& turn) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ void ring_sum(float (&s)[N], int W, int wide, int g, float (*red)[kRingSlots][N], int& turn) {
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - g * W;  // of the group
   int v = 0;
 #pragma unroll
   for (int n = N / 2, o = 1; o < 32; n >>= 1, o <<= 1) {
@@ -297,17 +306,25 @@ __device__ __forceinline__ void ring_sum(float (&s)[N], int W, int g, float (*re
     }
   }
   // This lane holds the warp's sum of value v.
-  if (lane < N) red[turn][warp][v] = s[0];
+  if (lane < N) red[turn][g * wide + warp][v] = s[0];
   if (W == 1) __syncwarp();
   else named_sync(1 + g, W * 32);
-  const float* r = red[turn][g * W + (lane & (W - 1))];
+  const float* r = red[turn][g * wide + (lane & (wide - 1))];
 #pragma unroll
   for (int i = 0; i < N; ++i) s[i] = r[i];
-  for (int o = 1; o < W; o <<= 1) {
+  for (int o = 1; o < wide; o <<= 1) {
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
   }
   turn ^= 1;
+}
+
+// Zeros in the slots; the power of two that a group has of them.
+template <int N>
+__device__ __forceinline__ int ring_clear(int W, float (*red)[kRingSlots][N]) {
+  for (int i = threadIdx.x; i < 2 * kRingSlots * N; i += kRingThreads) (&red[0][0][0])[i] = 0.f;
+  __syncthreads();
+  return W == 1 ? 1 : 2 << (31 - __clz(W - 1));
 }
 
 __device__ __forceinline__ float total(F2 x) {
@@ -322,11 +339,11 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const 
   using R = Ring<T, NV, ROWS, 1, SHIFT>;
   constexpr int VEC = R::VEC, H = VEC / 2;
   extern __shared__ uint4 smem[];
-  __shared__ float red[2][kRingThreads / 32][ROWS];
+  __shared__ float red[2][kRingSlots][ROWS];
   const T* const op[1] = {static_cast<const T*>(a.x)};
   const int64_t stride[1] = {a.x_stride};
   R ring(smem, a, TW, op, stride);
-  const int W = TW / 32;
+  const int W = TW / 32, wide = ring_clear(W, red);
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
 #pragma unroll
@@ -372,7 +389,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const 
       s[k] = total(t);
     }
     ring.issue();
-    ring_sum(s, W, ring.g, red, turn);
+    ring_sum(s, W, wide, ring.g, red, turn);
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
       s[k] *= inv_d;  // the mean
@@ -395,7 +412,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_forward_kernel(const 
         }
       q[k] = total(t);
     }
-    ring_sum(q, W, ring.g, red, turn);
+    ring_sum(q, W, wide, ring.g, red, turn);
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
       q[k] = 1.f / sqrtf(q[k] * inv_d + a.eps);  // the reciprocal deviation
@@ -430,11 +447,11 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
   using R = Ring<T, NV, ROWS, 2, SHIFT>;
   constexpr int VEC = R::VEC, H = VEC / 2;
   extern __shared__ uint4 smem[];
-  __shared__ float red[2][kRingThreads / 32][2 * ROWS];
+  __shared__ float red[2][kRingSlots][2 * ROWS];
   const T* const op[2] = {static_cast<const T*>(a.x), static_cast<const T*>(a.dy)};
   const int64_t stride[2] = {a.x_stride, a.dy_stride};
   R ring(smem, a, TW, op, stride);
-  const int W = TW / 32, D = ring.D;
+  const int W = TW / 32, wide = ring_clear(W, red), D = ring.D;
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
 #pragma unroll
@@ -520,7 +537,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
       s[2 * k] = total(t0[k]);
       s[2 * k + 1] = total(t1[k]);
     }
-    ring_sum(s, W, ring.g, red, turn);
+    ring_sum(s, W, wide, ring.g, red, turn);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (!(ring.columns >> i & 1u)) break;
@@ -562,7 +579,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
           unpack(acc[i][e], v[0], v[1]);
 #pragma unroll
           for (int o = 0; o < 2; ++o)
-            if (ring.inside(i, 2 * e + o)) all[ring.g * D + ring.place(i) + 2 * e + o - ring.shift] = v[o];
+            if ((ring.columns >> i & 1u) && ring.inside(i, 2 * e + o)) all[ring.g * D + ring.place(i) + 2 * e + o - ring.shift] = v[o];
         }
       __syncthreads();
       for (int c = threadIdx.x; c < D; c += kRingThreads) {
@@ -1030,7 +1047,7 @@ bool ring_fits(const LnArgs& a, bool backward) {
 
 // Other rows, where the matrices start on 16 bytes and their rows shift alike, up to 8 values a thread (their
 // parameters stay in registers, since loading them is a load a value).
-constexpr int64_t kShiftMinRows = 64;
+constexpr int64_t kShiftMinRows = 64;  // eight classes of a few rows (no slower than the other path from there on)
 bool shift_fits(const LnArgs& a, bool backward) {
   const int64_t vec = 16 / (int64_t)elem_bytes(a.dtype);
   auto ok = [&](const void* p, int64_t stride) {
@@ -1046,8 +1063,7 @@ void ring_shape(const LnArgs& a, int* nv, int* TW) {
   constexpr int VEC = 16 / sizeof(T);
   const int64_t D = SHIFT ? a.D + VEC - 1 : a.D;
   while ((int64_t)*nv * VEC * kRingThreads < D) *nv *= 2;
-  *TW = 32;
-  while ((int64_t)*TW * *nv * VEC < D) *TW *= 2;
+  *TW = (int)(32 * ceil_div(D, (int64_t)32 * *nv * VEC));
 }
 
 template <typename K>
