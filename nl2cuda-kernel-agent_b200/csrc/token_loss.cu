@@ -14,6 +14,8 @@
 // log-probability at m = 15; and it overflows for logits masked with the type's lowest value.)
 // lp is formed from x_label - m and log s, both small where the label leads, so no digits are lost
 // against a large maximum.  The MUFU ex2 adds 2 ulp.
+#include <algorithm>
+
 #include "lm_common.cuh"
 #include "lm_kernels.cuh"
 
@@ -23,8 +25,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e);
-constexpr int kFwdThreads = 256, kFwdCtas = 6;  // threads of a CTA, CTAs an SM holds at least
-constexpr int kBwdThreads = 256, kBwdCtas = 4;
+constexpr int kFwdWarps = 48, kBwdWarps = 32;   // that an SM holds at least
 constexpr int kPacks = 4;                       // 16-byte loads in flight per thread
 constexpr int kMaxSplit = 8;     // CTAs (one cluster) of a forward row
 
@@ -142,10 +143,10 @@ __device__ __forceinline__ void write_row(const LogitArgs& a, int64_t r, int64_t
 // One row per CTA; or a cluster of `split` CTAs per row: with few rows there are more SMs than rows, and
 // a row of 128 K elements read by one SM alone takes longer than the rest of the pass.  The shares
 // meet in the first CTA's shared memory.
-template <typename T>
-__global__ void __launch_bounds__(kFwdThreads, kFwdCtas) logprob_forward_kernel(const LogitArgs a, int split) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, kFwdWarps * 32 / THREADS) logprob_forward_kernel(const LogitArgs a, int split) {
   constexpr int VEC = 16 / sizeof(T);
-  __shared__ MaxSum part[kMaxSplit][kFwdThreads / 32];
+  __shared__ MaxSum part[kMaxSplit][THREADS / 32];
   if (split > 1) ptx::cluster_sync();  // every CTA of the cluster runs before one writes to another
   ptx::griddep_wait();
   const int64_t r = blockIdx.x / split;
@@ -160,13 +161,13 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas) logprob_forward_kernel(
     const T* body = x + head;
     const int64_t begin = packs * share / split, end = packs * (share + 1) / split;
     int64_t i = begin + threadIdx.x;
-    for (; i + (kPacks - 1) * kFwdThreads < end; i += kPacks * kFwdThreads) {
+    for (; i + (kPacks - 1) * THREADS < end; i += kPacks * THREADS) {
       Pack<T, VEC> p[kPacks];
 #pragma unroll
-      for (int u = 0; u < kPacks; ++u) p[u] = load_stream<T, VEC>(body + (i + u * kFwdThreads) * VEC);
+      for (int u = 0; u < kPacks; ++u) p[u] = load_stream<T, VEC>(body + (i + u * THREADS) * VEC);
       accumulate_packs(v, p);
     }
-    for (; i < end; i += kFwdThreads) {
+    for (; i < end; i += THREADS) {
       const Pack<T, VEC> p[1] = {load_stream<T, VEC>(body + i * VEC)};
       accumulate_packs(v, p);
     }
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas) logprob_forward_kernel(
   if (split > 1) ptx::cluster_sync();
   else __syncthreads();
   if (share != 0 || threadIdx.x >= 32) return;
-  constexpr int W = kFwdThreads / 32;
+  constexpr int W = THREADS / 32;
   MaxSum t{-INFINITY, 0.f};
   for (int i = threadIdx.x; i < split * W; i += 32) t = merge(t, part[i / W][i % W]);
   t = warp_merge(t);
@@ -196,10 +197,10 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas) logprob_forward_kernel(
 // `slices` CTAs per row, each a share of its packs.  Registers for four CTAs an SM and no second set of
 // packs in flight: 98% of the copy rate at 16384 x 131072 bf16; a software pipeline over two packs in
 // the same registers was at 78%, one over single packs with six CTAs at 88%.
-template <typename T>
-__global__ void __launch_bounds__(kBwdThreads, kBwdCtas) logprob_backward_kernel(const LogitArgs a, int slices) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, kBwdWarps * 32 / THREADS) logprob_backward_kernel(const LogitArgs a, int slices) {
   constexpr int VEC = 16 / sizeof(T);
-  constexpr int STEP = kPacks * kBwdThreads;
+  constexpr int STEP = kPacks * THREADS;
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   // Last rows first: what the forward read last is still in L2.
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdCtas) logprob_backward_kernel
     Pack<T, VEC> zero;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) zero.v[e] = from_f32<T>(0.f);
-    for (; i < end; i += kBwdThreads) store_pack<T, VEC>(dx + head + i * VEC, zero);
+    for (; i < end; i += THREADS) store_pack<T, VEC>(dx + head + i * VEC, zero);
     if (slice == 0) {
       if (threadIdx.x < head) dx[threadIdx.x] = from_f32<T>(0.f);
       if (tail + threadIdx.x < a.V) dx[tail + threadIdx.x] = from_f32<T>(0.f);
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdCtas) logprob_backward_kernel
   auto fetch = [&]() {
 #pragma unroll
     for (int u = 0; u < kPacks; ++u) {
-      const int64_t k = i + u * kBwdThreads;
+      const int64_t k = i + u * THREADS;
       if (k >= end) break;
       const T* q = x + head + k * VEC;
       if (same) {
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdCtas) logprob_backward_kernel
   while (i < end) {
 #pragma unroll
     for (int u = 0; u < kPacks; ++u) {
-      const int64_t k = i + u * kBwdThreads;
+      const int64_t k = i + u * THREADS;
       if (k >= end) break;
       const int64_t j = head + k * VEC;
       Pack<T, VEC> o;
@@ -438,36 +439,43 @@ cudaError_t by_type(int dtype, F f) {
 
 cudaError_t launch_logprob_forward(const LogitArgs& a, cudaStream_t stream) {
   if (a.rows == 0) return cudaSuccess;
+  constexpr int kMost = 256;  // threads of a CTA
   // With few rows, enough CTAs for every SM to have two, as long as each keeps a few rounds of loads.
   int split = 1;
-  while (split < kMaxSplit && a.rows * split * 2 <= 2 * device_sm_count() &&
-         a.V / (split * 2) >= 2 * kFwdThreads * 8)
+  while (split < kMaxSplit && a.rows * split * 2 <= 2 * device_sm_count() && a.V / (split * 2) >= 2 * kMost * 8)
     split *= 2;
+  // Rows for all the CTAs of 128 threads that the SMs hold: these, since half as many threads wait for each
+  // other at a row's end.  16384 x 32768 bf16 132 us (256 threads: 148), 4096 x 5034 14 (20); but
+  // 1024 x 32768 15.5 (14.6) and 4 x 131071 fp32, in clusters, 10.5 (7.9).
+  const bool many = a.rows >= kFwdWarps / 4 * (int64_t)device_sm_count();
   cudaError_t e = by_type(a.dtype, [&](auto t) {
     using T = decltype(t);
-    const dim3 grid((unsigned)(a.rows * split)), block(kFwdThreads);
-    if (split > 1) return launch_kernel_cluster(logprob_forward_kernel<T>, grid, block, 0, split, stream, a, split);
-    return launch_kernel(logprob_forward_kernel<T>, grid, block, 0, stream, a, 1);
+    const dim3 grid((unsigned)(a.rows * split));
+    if (split > 1)
+      return launch_kernel_cluster(logprob_forward_kernel<T, kMost>, grid, dim3(kMost), 0, split, stream, a, split);
+    if (many) return launch_kernel(logprob_forward_kernel<T, 128>, grid, dim3(128), 0, stream, a, 1);
+    return launch_kernel(logprob_forward_kernel<T, kMost>, grid, dim3(kMost), 0, stream, a, 1);
   });
   if (e != cudaSuccess) return e;
   note_launches(1);
   return cudaGetLastError();
 }
 
-// CTAs per row of the backward: at least four steps each, and no more than give every SM 32 in all.
-int64_t logprob_backward_slices(int64_t rows, int64_t V, int dtype) {
-  const int64_t steps = ceil_div(V, (int64_t)kPacks * kBwdThreads * (16 / (int64_t)elem_bytes(dtype)));
-  const int64_t want = ceil_div(32 * (int64_t)device_sm_count(), rows > 0 ? rows : 1);
-  const int64_t most = steps / 4 > 1 ? steps / 4 : 1;
-  return want < 1 ? 1 : want < most ? want : most;
-}
-
 cudaError_t launch_logprob_backward(const LogitArgs& a, cudaStream_t stream) {
   if (a.rows == 0 || a.V == 0) return cudaSuccess;
-  const int64_t slices = logprob_backward_slices(a.rows, a.V, a.dtype);
+  // Long rows take CTAs of 256 threads: 16384 x 32768 bf16 289 us (128 threads: 296), 2000 x 50001 fp32 115
+  // (121).  Rows of up to 32 KB and small calls take 128: 8192 x 1001 bf16 17 us (256: 28), 4096 x 5034 15 (20),
+  // 128 x 50257 8.8 (11.4).
+  const int64_t row = a.V * (int64_t)elem_bytes(a.dtype);
+  const int threads = row <= 32768 || row * a.rows <= (int64_t(64) << 20) ? 128 : 256;
+  // CTAs per row: at least four steps each, and no more than give every SM 32 in all.
+  const int64_t steps = ceil_div(row, (int64_t)kPacks * threads * 16);
+  const int64_t want = ceil_div(32 * (int64_t)device_sm_count(), a.rows);
+  const int64_t slices = std::min(want, std::max<int64_t>(1, steps / 4));
   cudaError_t e = by_type(a.dtype, [&](auto t) {
-    return launch_kernel(logprob_backward_kernel<decltype(t)>, dim3((unsigned)(a.rows * slices)),
-                         dim3(kBwdThreads), 0, stream, a, (int)slices);
+    using T = decltype(t);
+    auto k = threads == 128 ? logprob_backward_kernel<T, 128> : logprob_backward_kernel<T, 256>;
+    return launch_kernel(k, dim3((unsigned)(a.rows * slices)), dim3(threads), 0, stream, a, (int)slices);
   });
   if (e != cudaSuccess) return e;
   note_launches(1);
