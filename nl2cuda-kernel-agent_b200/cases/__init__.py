@@ -1,1 +1,3 @@
-"""Algorithm cases.  Only ``rbf`` (the Gaussian RBF kernel matrix) is built here."""
+"""Algorithm cases: the pairwise matrices (``rbf``, ``cosine_sim``) and the operators of a
+language-model fine-tuning step (``layernorm``, ``token_logprob``, ``preference_loss``,
+``policy_loss``, ``orthogonalize``)."""

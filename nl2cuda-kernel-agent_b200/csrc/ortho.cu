@@ -18,9 +18,9 @@
 // rounding to 8 or 11 bits in the first steps is a few percent of the result.)  fp16 has the range
 // for it because the spectrum is bounded: |X_0|_2 <= |X_0|_F <= 1, and |X_{k+1}|_2 <= the maximum of
 // |a s + b s^3 + c s^5| over [0, bound_k], a bound on every entry of X; those of A and B follow.
-// The scales 2^k put each matrix's bound just below 2^15; scale_table() works them out per matrix
-// on the device, so zero, tiny and diverging updates need no host round trip.  Powers of two, so
-// scaling adds no error.
+// The scales 2^k put each matrix's bound just below 2^15; scale_table() works them out, on the host for
+// |X_0|_F = 1 and on the device for a matrix that is no larger than eps, so that none needs a host round
+// trip.  Powers of two, so scaling adds no error.
 //
 // The tensor core truncates each addition to its fp32 accumulator, so a long sum of one sign comes out
 // low by half a unit per MMA: 1.8e-5 of the result at a depth of 2601.  So an accumulator takes a
@@ -600,6 +600,7 @@ struct PrepArgs {
   __half* t_lo;
   int64_t ld_g, ld_t, g_matrix, t_matrix;
   int* status;             // [0] status word, [1] arrivals of the products' CTAs
+  Scale usual[kMaxOps];    // the factors for |X_0|_F = 1
 };
 
 // Sums of squares in 64 bits: an update of any magnitude has a norm.  A warp takes pieces of
@@ -655,7 +656,7 @@ __global__ void __launch_bounds__(kNormThreads) ortho_norm_kernel(const PrepArgs
 
 // 2^k that brings values of at most `bound` below 2^15 (bounds past 2^+-100 keep the last scale:
 // what is smaller does not count next to the rest, what is larger has diverged).
-__device__ double pow2_scale(double bound) {
+__host__ __device__ inline double pow2_scale(double bound) {
   int e = 0;
   if (bound > 0.0 && isfinite(bound)) e = ilogb(bound) + 1;
   e = e < -100 ? -100 : e > 100 ? 100 : e;
@@ -664,7 +665,7 @@ __device__ double pow2_scale(double bound) {
 
 // max |f| over [0, top] of f = s^k (c0 + c1 u + c2 u^2): at the ends, or where f' = 0, a quadratic in u.
 // With u = s (k = 0 or 1) or u = s^2 (k = 1, `odd`: the polynomial of a step).
-__device__ double max_on(double top, int k, bool odd, double c0, double c1, double c2) {
+__host__ __device__ inline double max_on(double top, int k, bool odd, double c0, double c1, double c2) {
   auto f = [&](double s) {
     const double u = odd ? s * s : s;
     return fabs((k == 1 ? s : 1.0) * (c0 + u * (c1 + u * c2)));
@@ -689,11 +690,11 @@ __device__ double max_on(double top, int k, bool odd, double c0, double c1, doub
 
 constexpr double kSlack = 1.0 + 1e-3;  // on the bounds, for rounding along the way
 
-__device__ double first_scale(double rho) { return pow2_scale(rho * kSlack); }
+__host__ __device__ inline double first_scale(double rho) { return pow2_scale(rho * kSlack); }
 
 // The factors of every product for one matrix; rho is |X_0|_F.  x bounds |X|_2; A, T, P and Q are
 // polynomials in the eigenvalues of X X^T, whose bounds follow; sx ... sq are the matrices' scales.
-__device__ void scale_table(double rho, const PrepArgs& a, Scale* out) {
+__host__ __device__ inline void scale_table(double rho, const PrepArgs& a, Scale* out) {
   double x = rho * kSlack, u = 0.0, q = 0.0, next = 0.0;
   double sx = first_scale(rho), sa = 1.0, st = 1.0, sp = 1.0, sq = 1.0;
   int step = 0;
@@ -759,11 +760,12 @@ __device__ void scale_table(double rho, const PrepArgs& a, Scale* out) {
 constexpr int kTile = 64;
 constexpr int kTilePitch = kTile + 1;
 
-// X_0 in both orders, a 64 x 64 tile of G per CTA; the first CTA of a matrix writes its scales.
+// X_0 in both orders, a 64 x 64 tile of G per CTA; the first CTA of a matrix writes its factors.
+static_assert(kMaxOps <= 256, "a thread copies one");
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) ortho_split_kernel(const PrepArgs a) {
   __shared__ uint32_t tile[kTile * kTilePitch];  // hi in the low half, lo in the high half
-  __shared__ double s_factor;
+  __shared__ double s_factor, s_rho;
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   const int64_t z = blockIdx.z;
@@ -794,13 +796,22 @@ __global__ void __launch_bounds__(256) ortho_split_kernel(const PrepArgs a) {
     t = warp_sum(t);
     if (threadIdx.x == 0) {
       const double norm = sqrt(t), den = norm + (double)a.eps;
-      const bool first = blockIdx.x == 0 && blockIdx.y == 0;
+      // |X_0|_F is 1 unless the update is no larger than eps; only then are the factors worked out here (6 us
+      // for 15 products).
       const double rho = den > 0.0 ? norm / den : 0.0;
-      s_factor = first_scale(rho) / den;
-      if (first) scale_table(rho, a, a.scale + z * a.ops);
+      s_rho = rho > 0.5 ? 1.0 : rho;
+      s_factor = first_scale(s_rho) / den;
     }
   }
   __syncthreads();
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
+    Scale* out = a.scale + z * a.ops;
+    if (s_rho == 1.0) {
+      if (threadIdx.x < a.ops) out[threadIdx.x] = a.usual[threadIdx.x];
+    } else if (threadIdx.x == 0) {
+      scale_table(s_rho, a, out);
+    }
+  }
   const double factor = s_factor;
   // In fp32 where the factor has its full precision there (one more rounding, the same for all).
   const bool wide = !(fabs(factor) > 1e-30 && fabs(factor) < 1e30);
@@ -1073,6 +1084,7 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
   for (int k = 0; k < o.steps; ++k)
     for (int e = 0; e < 3; ++e) p.coef[k][e] = o.coefficients[3 * k + e];
   for (int i = 0; i < it.ops; ++i) p.kind[i] = it.op[i].kind;
+  scale_table(1.0, p, p.usual);
   p.part = ws_at<double>(o.workspace, L.part);
   p.scale = ws_at<Scale>(o.workspace, L.scale);
   const Split& g = it.mat[tall ? mXT0 : mX];
