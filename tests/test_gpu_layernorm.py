@@ -51,14 +51,13 @@ def bounds(x, w, b, dy, want, dtype, wdtype):
     g = dyd * wd
     gm = g.abs().mean(1, keepdim=True)
     gh = (g * h).abs().mean(1, keepdim=True)
-    em = e.mean(1, keepdim=True)
     hm = (h * h).mean(1, keepdim=True).sqrt()
     eg = 30 * U32 * (g.abs() + gm)
     eh = e * gh + h.abs() * ((g.abs() * e).mean(1, keepdim=True) + 30 * U32 * (gh + gm * hm))
     n = x.size(0)
     return {
         "y": e * wd.abs() + 3 * U32 * (h * wd).abs() + 2 * U32 * bd.abs() + rounded(y, dtype),
-        "dx": rstd * (eg + eh + em * gm * 0) + 30 * U32 * dx.abs() + rounded(dx, dtype),
+        "dx": rstd * (eg + eh) + 30 * U32 * dx.abs() + rounded(dx, dtype),
         "dw": (dyd.abs() * e).sum(0) + (n + 32) * U32 * (dyd * h).abs().sum(0) + rounded(dw, wdtype),
         "db": (n + 32) * U32 * dyd.abs().sum(0) + rounded(db, wdtype),
     }

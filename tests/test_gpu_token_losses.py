@@ -48,7 +48,7 @@ def lp_error(x, labels):
 def grad_bound(want, p, c, spread, dtype, V):
     """c p: the exponent's rounding (|x - m| <= spread), the approximation, 1 / s and products; and
     at the label c - c p.  Then one rounding."""
-    return U32 * (2 * spread + V / 256 + 100) * c.abs() * p + 2 * U32 * c.abs() * (p > 0) * 0 \
+    return U32 * (2 * spread + V / 256 + 100) * c.abs() * p \
         + 2 * U32 * want.abs() + rounded(want, dtype)
 
 
@@ -79,6 +79,13 @@ def test_logprob_and_gradient(B, T, V, dtype, cuda_device):
     assert not leaf.grad[labels == IGNORE].any()
     with torch.no_grad():
         assert torch.equal(token_logprob(leaf, labels, IGNORE), lp.detach())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,V", [(9, 250, 517), (2, 1000, 33), (5, 420, 9001)])
+def test_many_rows(B, T, V, dtype, cuda_device):
+    """Rows for every CTA that the SMs hold, and for several of each."""
+    test_logprob_and_gradient(B, T, V, dtype, cuda_device)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -257,6 +264,19 @@ def test_policy_loss(B, T, V, per_token, dtype, cuda_device):
                   + 4 * U32 * (5 * a * m).sum() / n)
     extra = 2 * e * (8 * k + 5 * a) / n + 6 * U32 * (2 * m * (8 * k + 5 * a) / n)
     check_logits_gradient(leaf, x64, lp64, lp64.grad, extra, dtype)
+
+
+def test_logprob_past_fp32(cuda_device):
+    """A log-probability that overflows fp32 is -inf, and so is its answer's reward (not NaN)."""
+    from cases.preference_loss.op import preference_loss
+    from cases.token_logprob.op import token_logprob
+    x = torch.zeros(2, 1, 4, device="cuda")
+    x[0, 0, 0], x[0, 0, 1] = -3.4e38, 3e38
+    labels = torch.zeros(2, 1, dtype=torch.long, device="cuda")
+    assert float(token_logprob(x, labels)[0]) == -math.inf
+    loss, reward = preference_loss(x, labels, torch.zeros(2, 1, device="cuda"))
+    assert float(reward[0]) == -math.inf and float(loss) == math.inf
+    assert abs(float(reward[1]) + 0.1 * math.log(4)) < 1e-7
 
 
 def test_nothing_scored(cuda_device):

@@ -66,6 +66,7 @@ def test_logprob_refusals(lib):
     def fwd(x=A, sb=40, st=8, lab=A, lp=A, rows=10, T=5, V=8, dt=0):
         return lib.lp_sm100_forward(x, sb, st, lab, lp, None, None, rows, T, V, -100, dt, None)
     assert fwd(rows=-1) == INVALID
+    assert fwd(rows=1 << 61, T=1) == UNSUPPORTED  # 8 times that passes 64 bits
     assert fwd(T=4) == INVALID
     assert fwd(T=0) == INVALID
     assert fwd(V=0) == INVALID
