@@ -725,8 +725,8 @@ __global__ void __launch_bounds__(256) ln_backward_kernel(const LnArgs a, int W,
 // A CTA takes a row, 16 values a thread; the sums of a thread's own columns are in shared memory
 // (128 KB), at a quarter of the time that the row takes from HBM.  In registers, of which 1024 threads have
 // 64 each, they spilled: 4096 x 12288 fp32 in 136 us in place of 400, 4096 x 9001 bf16 in 137 in place of 1118.
-// From 4096 values on: 8192 x 8191 fp32 in 260 us, 291 with 512 threads and registers; 8192 x 4101 fp32 163, 230;
-// 8192 x 6001 bf16 197, 245; 8192 x 4500 bf16 151, 133.
+// From 4096 values on, against 512 threads and registers: 8192 x 8191 fp32 in 260 us (291), 8192 x 4101 fp32 163 (230),
+// 8192 x 6001 bf16 197 (245), 8192 x 4500 bf16 151 (133).
 constexpr int kLongThreads = 1024;
 constexpr size_t kLongBytes = sizeof(float) * 2 * kLaneElems * kLongThreads;
 
@@ -1045,15 +1045,16 @@ bool ring_fits(const LnArgs& a, bool backward) {
   return pack_elems(a, backward) * eb == 16 && a.D * eb <= 32768;
 }
 
-// Other rows, where the matrices start on 16 bytes and their rows shift alike, up to 8 values a thread (their
-// parameters stay in registers, since loading them is a load a value).
+// Other rows, where the matrices start on 16 bytes and their rows shift alike: up to four packs a thread in the
+// forward, 4096 x 9001 bf16 in 96 us (212 with loads of single values); up to two in the backward, 8192 x 8175 bf16
+// in 173 us (ln_long_backward_kernel: 247), while with four 4096 x 9001 takes 266 (138).
 constexpr int64_t kShiftMinRows = 64;  // eight classes of a few rows (no slower than the other path from there on)
 bool shift_fits(const LnArgs& a, bool backward) {
   const int64_t vec = 16 / (int64_t)elem_bytes(a.dtype);
   auto ok = [&](const void* p, int64_t stride) {
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (stride - a.D) % vec == 0);
   };
-  return a.rows >= kShiftMinRows && a.D + vec - 1 <= 8 * kRingThreads && ok(a.x, a.x_stride) && ok(a.y, a.D) &&
+  return a.rows >= kShiftMinRows && a.D + vec - 1 <= (backward ? 2 : 4) * vec * kRingThreads && ok(a.x, a.x_stride) && ok(a.y, a.D) &&
          (!backward || ok(a.dy, a.dy_stride));
 }
 
@@ -1084,11 +1085,8 @@ cudaError_t launch_ring_forward(const LnArgs& a, cudaStream_t stream) {
   int nv = a.D > 32 * VEC && !(SHIFT && VEC == 8) ? 2 : 1, TW, parts;
   ring_shape<T, SHIFT>(a, &nv, &TW);
   if (nv == 1) return launch_ring(ln_ring_forward_kernel<T, 1, 4, SHIFT>, a, classes, TW, 4, &parts, stream);
-  if constexpr (!SHIFT || VEC == 4) {
-    if (nv == 2) return launch_ring(ln_ring_forward_kernel<T, 2, 4, SHIFT>, a, classes, TW, 4, &parts, stream);
-  }
-  if constexpr (!SHIFT) return launch_ring(ln_ring_forward_kernel<T, 4, 2, false>, a, classes, TW, 2, &parts, stream);
-  return cudaErrorInvalidConfiguration;  // shift_fits() lets no longer rows pass
+  if (nv == 2) return launch_ring(ln_ring_forward_kernel<T, 2, 4, SHIFT>, a, classes, TW, 4, &parts, stream);
+  return launch_ring(ln_ring_forward_kernel<T, 4, 2, SHIFT>, a, classes, TW, 2, &parts, stream);
 }
 
 // As few packs a thread as hold the row, since its column sums take 2 registers a value; two rows a block,
@@ -1100,9 +1098,7 @@ cudaError_t launch_ring_backward(const LnArgs& a, int* parts, cudaStream_t strea
   int nv = 1, TW;
   ring_shape<T, SHIFT>(a, &nv, &TW);
   if (nv == 1) return launch_ring(ln_ring_backward_kernel<T, 1, R, SHIFT>, a, classes, TW, R, parts, stream);
-  if constexpr (!SHIFT || VEC == 4) {
-    if (nv == 2) return launch_ring(ln_ring_backward_kernel<T, 2, 2, SHIFT>, a, classes, TW, 2, parts, stream);
-  }
+  if (nv == 2) return launch_ring(ln_ring_backward_kernel<T, 2, 2, SHIFT>, a, classes, TW, 2, parts, stream);
   if constexpr (!SHIFT) return launch_ring(ln_ring_backward_kernel<T, 4, 1, false>, a, classes, TW, 1, parts, stream);
   return cudaErrorInvalidConfiguration;  // shift_fits() lets no longer rows pass
 }

@@ -128,7 +128,8 @@ def test_many_long_rows(rows, D, dtype, cuda_device):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,D", [(64, 1), (65, 7), (71, 31), (64, 255), (4099, 1023), (2100, 1001), (1200, 2041), (1200, 2042),
-                                    (700, 4085), (700, 4089), (700, 4090), (530, 4094), (20000, 129), (530, 4095)])
+                                    (700, 4085), (700, 4089), (700, 4090), (530, 4094), (20000, 129), (530, 4095), (520, 8185), (520, 8189), (260, 16377),
+                                    (260, 16378)])
 def test_unaligned_rows(rows, D, dtype, cuda_device):
     """Rows that begin anywhere in 16 bytes, at the ends of what a CTA's threads hold."""
     check(*inputs(rows, D, dtype, dtype, D))
