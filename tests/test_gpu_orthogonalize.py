@@ -103,6 +103,13 @@ def test_against_64_bits(shape, dtype, cuda_device):
     check(update(shape, dtype, shape[0] + shape[1]))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(4100, 8190), (8190, 4097)])
+def test_widest_tiles(shape, dtype, cuda_device):
+    """Large enough for tiles of 256 x 256, of sizes that fill none."""
+    check(update(shape, dtype, 5))
+
+
 @pytest.mark.parametrize("shape", [(3, 40, 70), (2, 3, 130, 65), (5, 256, 256), (20, 7, 129),
                                    (2, 700, 900), (7, 384, 128)])
 def test_batches(shape, cuda_device):
@@ -250,7 +257,7 @@ def test_verify_all_passes(cuda_device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape", [(40, 400), (129, 1300), (1500, 300), (3, 70, 500)])
+@pytest.mark.parametrize("shape", [(40, 400), (129, 1300), (1500, 300), (3, 70, 500), (20, 200, 1500), (8000, 300)])
 @pytest.mark.parametrize("steps", [1, 2, 3, 4, 8])
 def test_groups_of_steps(shape, steps, dtype, cuda_device):
     """Long rows: 16-bit types take several steps through X at once, of every group size, with
