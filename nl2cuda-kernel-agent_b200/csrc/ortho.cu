@@ -562,8 +562,9 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
       if (lane == 0) {
         __threadfence_block();
         if (atomicAdd(stored, 1u) == (unsigned)(p + 1) * kEpiWarps - 1) {
-          __threadfence();
-          asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(it.arrived) : "memory");
+          // The fence takes in the other warps' stores and gives them out with the count.
+          asm volatile("fence.acq_rel.gpu;" ::: "memory");
+          asm volatile("red.relaxed.gpu.global.add.u32 [%0], 1;" ::"l"(it.arrived) : "memory");
         }
       }
     }
