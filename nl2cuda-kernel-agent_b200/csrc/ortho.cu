@@ -33,7 +33,7 @@
 // Kernel: one launch runs the whole iteration (cooperative, one CTA per SM).  A product's tiles are
 // shared out over the CTA pairs; each CTA counts itself in when its part is stored, and the loads of
 // the next product wait until all have.  A launch for each product took 11 us from one to the next on a
-// batch of four of 256 x 256; this takes 8.  Warp 0 loads operand slices by TMA (64 deep, 128-byte
+// batch of four of 256 x 256; this takes 7.5.  Warp 0 loads operand slices by TMA (64 deep, 128-byte
 // swizzle, hi and lo of both operands) into a ring of stages; warp 1 issues 3 x 4 MMAs per stage into one
 // of the TMEM accumulators; warps 4..11 read the others, apply the epilogue and store.  All
 // on CTA pairs (cta_group::2), tiles of 256 x 256, 128 or 64: a CTA of the pair loads its 128 rows of P
@@ -856,7 +856,7 @@ __global__ void __launch_bounds__(256) ortho_split_kernel(const PrepArgs a) {
 // Steps that a group may hold.  Carrying A over (two products of r^3 in place of going through X: r^2 c + 2
 // r^2 c) saves (1.5 c / r - 1.5) r^3 a step, at one product more.  Up to three steps, which leaves the
 // error where it was: an error of A grows by a^2 a step; four steps and more let it show (8 times, for an
-// update with a few strong directions).  4096 x 8192 bf16: 5.3 -> 3.9 ms.
+// update with a few strong directions).
 int group_size(const float* coef, int step, int steps) {
   const int left = steps - step, groups = (left + 2) / 3;
   const int n = (left + groups - 1) / groups;
@@ -1009,15 +1009,15 @@ cudaError_t launch_iteration(IterArgs& it, cudaStream_t stream) {
 // Estimated time of the products with tiles of width bn, in cycles.  A slice of 64 costs a pair the larger
 // of its 12 MMAs (6 bn cycles) and its operands' way into shared memory (64 bytes a cycle and CTA: 1024, 768
 // and 640 for bn = 256, 128 and 64; 850 for 128 with every SM at it).  A product ends with what nothing
-// hides, the epilogue of a tile and the wait for the other CTAs: 6000 + 130 bn.  Measured for 64, 128
-// and 256: four of 256 x 256: 134, 207 and 374 us; 2048 x 4096: 960, 835 and 1110; 4096 x 8192 (not
-// grouped): 7.1, 5.6 and 5.3 ms.
+// hides, the epilogue of a tile and the wait for the other CTAs: 3700 + 130 bn.  Measured for 64, 128
+// and 256: four of 256 x 256: 128, 204 and 361 us; 2048 x 4096 bf16: 921, 799 and 1089, grouped 734, 671 and 1049;
+// 4096 x 8192: 6.9, 5.4 and 5.0 ms, grouped 5.3, 4.2 and 4.0.
 int64_t estimate(const IterArgs& it, const Op* op, int ops, int bn) {
   const int64_t pairs = device_sm_count() / 2, slice = bn == 256 ? 1536 : bn == 128 ? 850 : 640;
   int64_t cost = 0;
   for (int i = 0; i < ops; ++i) {
     const Split &p = it.mat[op[i].p], &q = it.mat[op[i].q];
-    cost += ceil_div(tiles_of(p.rows, q.rows, bn, op[i].out_kind) * it.batch, pairs) * ceil_div(p.cols, BK) * slice + 6000 + 130 * bn;
+    cost += ceil_div(tiles_of(p.rows, q.rows, bn, op[i].out_kind) * it.batch, pairs) * ceil_div(p.cols, BK) * slice + 3700 + 130 * bn;
   }
   return cost;
 }
