@@ -26,7 +26,8 @@ enum { LM_F32 = 0, LM_BF16 = 1, LM_F16 = 2 };
 /* ---- layer norm --------------------------------------------------------------------------
  *   y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(var + eps)      over rows of length D
  * x [rows, D] (type dtype), weight and bias [D] (type wdtype; NULL: 1 and 0), y [rows, D]
- * (type dtype).  mean and rstd [rows] fp32 are written for the backward; both NULL: not kept.
+ * (type dtype), which must not overlap x.  mean and rstd [rows] fp32 are written for the backward; both
+ * NULL: not kept.
  * var is the mean of (x - mean)^2 (two passes over the row on chip, no cancellation). */
 RBF_API int ln_sm100_forward(const void* x, int64_t x_stride, const void* weight,
                              const void* bias, void* y, float* mean, float* rstd, int64_t rows,
@@ -39,7 +40,8 @@ RBF_API size_t ln_sm100_backward_workspace_bytes(int64_t rows, int64_t D);
  *   dx = rstd * (g - mean(g) - xh * mean(g * xh)),  dweight = sum_rows dy * xh,
  *   dbias = sum_rows dy
  * dx [rows, D] contiguous (type dtype); dweight and dbias [D] (type wdtype).  Any of the three
- * may be NULL: not computed.  The sums run in a fixed order: equal calls give equal bits. */
+ * may be NULL: not computed.  dx must overlap neither x nor dy.  The sums run in a fixed order: equal
+ * calls give equal bits. */
 RBF_API int ln_sm100_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
                               const void* weight, const float* mean, const float* rstd, void* dx,
                               void* dweight, void* dbias, int64_t rows, int64_t D, int dtype,
@@ -61,7 +63,7 @@ RBF_API int lp_sm100_forward(const void* logits, int64_t batch_stride, int64_t t
 
 /* dlogits[r, j] = c_r * ((j == label_r) - exp(x[j] - max_r) * inv_r),
  * c_r = coef[r] * scale
- * dlogits [rows, V] contiguous (type dtype); rows that are not scored are zeroed.  scale: the
+ * dlogits [rows, V] contiguous (type dtype), which must not overlap the logits; rows that are not scored are zeroed.  scale: the
  * product of the device scalars scale0 and scale1 (either may be NULL: 1). */
 RBF_API int lp_sm100_backward(const void* logits, int64_t batch_stride, int64_t t_stride,
                               const int64_t* labels, const float* stats, const float* coef,
@@ -82,9 +84,9 @@ RBF_API size_t loss_sm100_workspace_bytes(int64_t B, int64_t T);
  *   loss = mean_p [ -(1 - s) log sigmoid(z_p) - s log sigmoid(-z_p) ],   s = label_smoothing
  * reward [B], loss [1]; coef [B, T] receives d loss / d logprob for lp_sm100_backward. */
 RBF_API int pref_sm100_loss(const float* logprob, const float* rest, const float* ref_logprob,
-                            const int64_t* labels, float* loss, float* reward, float* coef, int64_t B, int64_t T,
-                            float beta, float label_smoothing, int64_t ignore_index,
-                            void* workspace, size_t workspace_bytes, rbf_stream_t stream);
+                            const int64_t* labels, float* loss, float* reward, float* coef,
+                            int64_t B, int64_t T, float beta, float label_smoothing,
+                            int64_t ignore_index, void* workspace, size_t workspace_bytes, rbf_stream_t stream);
 
 /* Clipped policy loss, a mean over all scored positions (count of them; 1 if there are none):
  *   ratio = exp(logprob - old_logprob),  d = ref_logprob - logprob,  kl = exp(d) - d - 1

@@ -148,6 +148,17 @@ def test_unaligned_rows_apart(dtype, cuda_device):
         check(x, w, None, wide)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D", [(5, 512), (100, 512), (2100, 1024), (70, 6144), (70, 12288)])
+def test_misaligned_parameters(rows, D, dtype, cuda_device):
+    """Weight and bias that begin off 16 bytes, under rows that do not."""
+    x, w, b, dy = inputs(rows, D, dtype, torch.float32, D)
+    for pdtype in {dtype, torch.float32}:
+        both = torch.zeros(2 * D + 3, dtype=pdtype, device=x.device)
+        both[1:D + 1], both[D + 2:2 * D + 2] = w, b
+        check(x, both[1:D + 1], both[D + 2:2 * D + 2], dy)
+
+
 def test_strided_and_broadcast_operands(cuda_device):
     """Rows that lie apart, a transposed matrix, a misaligned slice, an expanded dy."""
     from cases.layernorm.op import layer_norm

@@ -159,6 +159,14 @@ def test_magnitudes(scale, cuda_device):
         assert float((got - want).norm()) <= 1e-5 * float(want.norm())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("share", [0.1, 0.5, 0.99, 1.01, 3.0])
+def test_norm_near_eps(share, dtype, cuda_device):
+    """eps of a share of the update's norm: the first X is well below 1."""
+    g = update((130, 300), dtype, 8)
+    check(g, eps=share * float(g.double().norm()))
+
+
 def test_zero_and_nan(cuda_device):
     from cases.orthogonalize.op import orthogonalize
     g = update((3, 50, 60), torch.float32, 6)
