@@ -722,44 +722,41 @@ __global__ void __launch_bounds__(256) ln_backward_kernel(const LnArgs a, int W,
 }
 
 // ---- backward, long rows that the ring does not take
-// A CTA takes a row, 16 values a thread; the sums of a thread's own columns are in shared memory
-// (128 KB), at a quarter of the time that the row takes from HBM.  In registers, of which 1024 threads have
+// A CTA takes a row, 16 values a thread; the sums of a thread's own columns are in shared memory (64 or
+// 128 KB), at a quarter of the time that the row takes from HBM.  In registers, of which 1024 threads have
 // 64 each, they spilled: 4096 x 12288 fp32 in 136 us in place of 400, 4096 x 9001 bf16 in 137 in place of 1118.
-// From 4096 values on, against 512 threads and registers: 8192 x 8191 fp32 in 260 us (291), 8192 x 4101 fp32 163 (230),
-// 8192 x 6001 bf16 197 (245), 8192 x 4500 bf16 151 (133).
-constexpr int kLongThreads = 1024;
-constexpr size_t kLongBytes = sizeof(float) * 2 * kLaneElems * kLongThreads;
-
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kLongThreads, 1) ln_long_backward_kernel(const LnArgs a) {
-  constexpr int NV = kLaneElems / VEC;
+// Rows of up to 8192 values take two CTAs of 512 threads an SM, one of which loads while the other waits for its sums:
+// 8192 x 4101 fp32 in 117 us, 164 with one of 1024 (230 with 512 threads and registers).
+template <typename T, int VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) ln_long_backward_kernel(const LnArgs a) {
+  constexpr int NV = kLaneElems / VEC, W = THREADS / 32;
   extern __shared__ float sums[];  // [dw, db][value of the thread][thread]
   __shared__ float2 red[2 * 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float* const dw = sums + threadIdx.x;
-  float* const db = dw + kLaneElems * kLongThreads;
+  float* const db = dw + kLaneElems * THREADS;
   int turn = 0;
   const int D = (int)a.D;
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
 #pragma unroll
-  for (int k = 0; k < kLaneElems; ++k) dw[k * kLongThreads] = db[k * kLongThreads] = 0.f;
+  for (int k = 0; k < kLaneElems; ++k) dw[k * THREADS] = db[k * THREADS] = 0.f;
   const float inv_d = 1.f / (float)D;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     Row<T, VEC, NV> x, dy;
-    x.load(static_cast<const T*>(a.x) + r * a.x_stride, D, 32, warp, lane);
-    dy.load(static_cast<const T*>(a.dy) + r * a.dy_stride, D, 32, warp, lane);
+    x.load(static_cast<const T*>(a.x) + r * a.x_stride, D, W, warp, lane);
+    dy.load(static_cast<const T*>(a.dy) + r * a.dy_stride, D, W, warp, lane);
     const float mean = a.mean[r], rstd = a.rstd[r];
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = ((i * 32 + warp) * 32 + lane) * VEC;
+      const int c = ((i * W + warp) * 32 + lane) * VEC;
       if (c >= D) break;
       float w[VEC];
       load_param<VEC>(a.weight, c, a.wdtype, 1.f, w);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const int k = (i * VEC + e) * kLongThreads;
+        const int k = (i * VEC + e) * THREADS;
         const float h = (to_f32(x.p[i].v[e]) - mean) * rstd, d = to_f32(dy.p[i].v[e]);
         const float gw = d * w[e];
         s.x += gw;
@@ -771,12 +768,12 @@ __global__ void __launch_bounds__(kLongThreads, 1) ln_long_backward_kernel(const
       }
     }
     if (a.y == nullptr) continue;
-    s = group_sum(s, 32, warp, 1, red, turn);
+    s = group_sum(s, W, warp, 1, red, turn);
     const float m1 = s.x * inv_d, m2 = s.y * inv_d;
     T* dx = static_cast<T*>(a.y) + r * D;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = ((i * 32 + warp) * 32 + lane) * VEC;
+      const int c = ((i * W + warp) * 32 + lane) * VEC;
       if (c >= D) break;
       float w[VEC];
       load_param<VEC>(a.weight, c, a.wdtype, 1.f, w);
@@ -792,12 +789,12 @@ __global__ void __launch_bounds__(kLongThreads, 1) ln_long_backward_kernel(const
   if (a.part == nullptr) return;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = ((i * 32 + warp) * 32 + lane) * VEC;
+    const int c = ((i * W + warp) * 32 + lane) * VEC;
     if (c >= D) break;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      a.part[(int64_t)blockIdx.x * D + c + e] = dw[(i * VEC + e) * kLongThreads];
-      a.part[((int64_t)gridDim.x + blockIdx.x) * D + c + e] = db[(i * VEC + e) * kLongThreads];
+      a.part[(int64_t)blockIdx.x * D + c + e] = dw[(i * VEC + e) * THREADS];
+      a.part[((int64_t)gridDim.x + blockIdx.x) * D + c + e] = db[(i * VEC + e) * THREADS];
     }
   }
 }
@@ -1024,6 +1021,13 @@ cudaError_t by_forward_shape(const Shape& s, F f) {
   return by_forward_count<T, 1, 4>(s, f);
 }
 
+template <typename T, int THREADS>
+auto long_backward(int vec) {
+  constexpr int V = 16 / sizeof(T);
+  if (V == 8 && vec == 4) return ln_long_backward_kernel<T, 4, THREADS>;
+  return vec == V ? ln_long_backward_kernel<T, V, THREADS> : vec == 2 ? ln_long_backward_kernel<T, 2, THREADS> : ln_long_backward_kernel<T, 1, THREADS>;
+}
+
 template <typename F>
 cudaError_t by_type(int dtype, F f) {
   if (dtype == LM_F32) return f(float{});
@@ -1170,15 +1174,14 @@ cudaError_t launch_ln_backward(const LnArgs& a, cudaStream_t stream) {
     e = by_type(a.dtype, [&](auto t) { return launch_ring_backward<decltype(t), true>(b, &parts, stream); });
     ++launches;
   } else if (a.D > kLongMin) {
-    parts = (int)std::min<int64_t>(parts, kSmCount);
+    const bool half = a.D <= 512 * kLaneElems;
+    parts = (int)std::min<int64_t>(parts, (half ? 2 : 1) * kSmCount);
     e = by_type(a.dtype, [&](auto t) {
-      using E = decltype(t);
-      constexpr int V = 16 / sizeof(E);
-      const int vec = pack_elems(a, true);
-      auto k = vec == V ? ln_long_backward_kernel<E, V> : vec == 2 ? ln_long_backward_kernel<E, 2> : ln_long_backward_kernel<E, 1>;
-      if (V == 8 && vec == 4) k = ln_long_backward_kernel<E, 4>;
-      const cudaError_t set = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLongBytes);
-      return set != cudaSuccess ? set : launch_kernel(k, dim3(parts), dim3(kLongThreads), kLongBytes, stream, b);
+      const int threads = half ? 512 : 1024;
+      auto k = half ? long_backward<decltype(t), 512>(pack_elems(a, true)) : long_backward<decltype(t), 1024>(pack_elems(a, true));
+      const int smem = (int)sizeof(float) * 2 * kLaneElems * threads;
+      const cudaError_t set = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      return set != cudaSuccess ? set : launch_kernel(k, dim3(parts), dim3(threads), smem, stream, b);
     });
     ++launches;
   } else {
