@@ -481,7 +481,8 @@ __global__ void __launch_bounds__(kRingThreads, 1) ln_ring_backward_kernel(const
     }
   };
   stats(ring.row);
-  // Long rows: x and dy are read from shared memory again for dx, since the column sums take 64 registers.
+  // x and dy are read from shared memory again for dx where they and the column sums take more registers than
+  // there are.
   constexpr bool AGAIN = NV * VEC * ROWS > 16;
   const float inv_d = 1.f / (float)D;
   T* dx = static_cast<T*>(a.y) + ring.out(ring.row);
@@ -724,7 +725,7 @@ __global__ void __launch_bounds__(256) ln_backward_kernel(const LnArgs a, int W,
 // ---- backward, long rows that the ring does not take
 // A CTA takes a row, 16 values a thread; the sums of a thread's own columns are in shared memory (64 or
 // 128 KB), at a quarter of the time that the row takes from HBM.  In registers, of which 1024 threads have
-// 64 each, they spilled: 4096 x 12288 fp32 in 136 us in place of 400, 4096 x 9001 bf16 in 137 in place of 1118.
+// 64 each, they spilled: 4096 x 12288 fp32 in 132 us in place of 400, 4096 x 9001 bf16 in 137 in place of 1118.
 // Rows of up to 8192 values take two CTAs of 512 threads an SM, one of which loads while the other waits for its sums:
 // 8192 x 4101 fp32 in 117 us, 164 with one of 1024 (230 with 512 threads and registers).
 template <typename T, int VEC, int THREADS>
@@ -791,10 +792,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) ln_long_backward_kern
   for (int i = 0; i < NV; ++i) {
     const int c = ((i * W + warp) * 32 + lane) * VEC;
     if (c >= D) break;
+    constexpr int N = VEC < 4 ? VEC : 4;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      a.part[(int64_t)blockIdx.x * D + c + e] = dw[(i * VEC + e) * THREADS];
-      a.part[((int64_t)gridDim.x + blockIdx.x) * D + c + e] = db[(i * VEC + e) * THREADS];
+    for (int e = 0; e < VEC; e += N) {
+      Pack<float, N> v, u;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        v.v[k] = dw[(i * VEC + e + k) * THREADS];
+        u.v[k] = db[(i * VEC + e + k) * THREADS];
+      }
+      store_pack<float, N>(a.part + (int64_t)blockIdx.x * D + c + e, v);
+      store_pack<float, N>(a.part + ((int64_t)gridDim.x + blockIdx.x) * D + c + e, u);
     }
   }
 }
@@ -1041,17 +1049,19 @@ int64_t reg_parts(int64_t rows) {
   return rows < most ? (rows > 0 ? rows : 1) : most;
 }
 
-// Rows of whole 16-byte packs, up to 32 KB each, go through the ring.
+// Rows of whole 16-byte packs go through the ring: up to 32 KB each in the forward, 16 KB in the backward, whose column
+// sums leave no registers for four packs a thread (4096 x 8192 fp32: 101 us, ln_long_backward_kernel 81;
+// 4096 x 16384 bf16: 155, 138).
 // The forward below so many values goes a row at a time: its CTAs then have a block or two each.
 constexpr int64_t kRingForwardMin = 2 * 1024 * 1024;
 bool ring_fits(const LnArgs& a, bool backward) {
   const int64_t eb = (int64_t)elem_bytes(a.dtype);
-  return pack_elems(a, backward) * eb == 16 && a.D * eb <= 32768;
+  return pack_elems(a, backward) * eb == 16 && a.D * eb <= (backward ? 16384 : 32768);
 }
 
 // Other rows, where the matrices start on 16 bytes and their rows shift alike: up to four packs a thread in the
 // forward, 4096 x 9001 bf16 in 96 us (212 with loads of single values); up to two in the backward, 8192 x 8175 bf16
-// in 173 us (ln_long_backward_kernel: 247), while with four 4096 x 9001 takes 266 (138).
+// in 173 us (ln_long_backward_kernel with one CTA an SM: 247), while with four 4096 x 9001 takes 266 (138).
 constexpr int64_t kShiftMinRows = 64;  // eight classes of a few rows (no slower than the other path from there on)
 bool shift_fits(const LnArgs& a, bool backward) {
   const int64_t vec = 16 / (int64_t)elem_bytes(a.dtype);
@@ -1102,9 +1112,7 @@ cudaError_t launch_ring_backward(const LnArgs& a, int* parts, cudaStream_t strea
   int nv = 1, TW;
   ring_shape<T, SHIFT>(a, &nv, &TW);
   if (nv == 1) return launch_ring(ln_ring_backward_kernel<T, 1, R, SHIFT>, a, classes, TW, R, parts, stream);
-  if (nv == 2) return launch_ring(ln_ring_backward_kernel<T, 2, 2, SHIFT>, a, classes, TW, 2, parts, stream);
-  if constexpr (!SHIFT) return launch_ring(ln_ring_backward_kernel<T, 4, 1, false>, a, classes, TW, 1, parts, stream);
-  return cudaErrorInvalidConfiguration;  // shift_fits() lets no longer rows pass
+  return launch_ring(ln_ring_backward_kernel<T, 2, 2, SHIFT>, a, classes, TW, 2, parts, stream);
 }
 
 }  // namespace
