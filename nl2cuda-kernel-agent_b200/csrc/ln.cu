@@ -1061,13 +1061,15 @@ bool ring_fits(const LnArgs& a, bool backward) {
 
 // Other rows, where the matrices start on 16 bytes and their rows shift alike: up to four packs a thread in the
 // forward, 4096 x 9001 bf16 in 96 us (212 with loads of single values); up to two in the backward, 8192 x 8175 bf16
-// in 173 us (ln_long_backward_kernel with one CTA an SM: 247), while with four 4096 x 9001 takes 266 (138).
+// in 171 us (ln_long_backward_kernel: 212), while with four 4096 x 9001 takes 266 (137).  With two packs of which
+// many lie past the row it is the slower one: 8192 x 4500 bf16 138 us (97), 8192 x 6001 149 (155).
 constexpr int64_t kShiftMinRows = 64;  // eight classes of a few rows (no slower than the other path from there on)
 bool shift_fits(const LnArgs& a, bool backward) {
   const int64_t vec = 16 / (int64_t)elem_bytes(a.dtype);
   auto ok = [&](const void* p, int64_t stride) {
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (stride - a.D) % vec == 0);
   };
+  if (backward && a.D > kLongMin && a.D < kLongMin * 3 / 2) return false;
   return a.rows >= kShiftMinRows && a.D + vec - 1 <= (backward ? 2 : 4) * vec * kRingThreads && ok(a.x, a.x_stride) && ok(a.y, a.D) &&
          (!backward || ok(a.dy, a.dy_stride));
 }
