@@ -8,8 +8,8 @@
 // some 10 flops each.  Every row is read once and held on chip; the variance is a second pass over
 // registers, not over memory, and has no cancellation.
 //
-// In the backward a thread keeps the sums of its columns' dy * xh and dy in registers over all
-// its rows; each CTA writes one row of partial sums at its end and a second, short kernel adds
+// In the backward a thread keeps the sums of its columns' dy * xh and dy in registers (long rows: in
+// shared memory) over all its rows; each CTA writes one row of partial sums at its end and a second, short kernel adds
 // those in a fixed order.  No atomics: equal calls give equal bits.
 //
 // Statistics, sums and partial sums are fp32; every output is rounded once.
