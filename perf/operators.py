@@ -8,7 +8,6 @@ calls.  ``work(case)`` is the traffic and arithmetic that a pass cannot do witho
 ``exact(case, seed)`` the outputs from the definitions in 64 bits.
 """
 import functools
-import importlib
 import math
 import os
 import sys
@@ -172,16 +171,17 @@ def prepare(case, seed):
 # -------------------------------------------------------------------------------- the passes
 
 @functools.cache
-def _call(op):
-    """The package's public call of an operator."""
+def _ops():
+    """The package's public calls."""
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     sys.path.insert(0, os.path.join(root, "nl2cuda-kernel-agent_b200"))
-    case, name = {"layernorm": ("layernorm", "layer_norm"),
-                  "logprob": ("token_logprob", "token_logprob"),
-                  "preference": ("preference_loss", "preference_loss"),
-                  "policy": ("policy_loss", "policy_loss"),
-                  "orthogonalize": ("orthogonalize", "orthogonalize")}[op]
-    return getattr(importlib.import_module(f"cases.{case}.op"), name)
+    from cases.layernorm.op import layer_norm
+    from cases.orthogonalize.op import orthogonalize
+    from cases.policy_loss.op import policy_loss
+    from cases.preference_loss.op import preference_loss
+    from cases.token_logprob.op import token_logprob
+    return {"layernorm": layer_norm, "orthogonalize": orthogonalize, "policy": policy_loss,
+            "preference": preference_loss, "logprob": token_logprob}
 
 
 def run(s):
@@ -189,7 +189,7 @@ def run(s):
 
 
 def _run_own(s):
-    f = _call(s["op"])
+    f = _ops()[s["op"]]
     if s["op"] == "layernorm":
         if not s["train"]:
             with torch.no_grad():
