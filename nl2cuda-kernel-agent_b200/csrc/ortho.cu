@@ -292,6 +292,15 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
             }
           }
         }
+        // The leader's commits arrive here too: none may be on its way when this CTA's shared memory goes, so
+        // every stage is awaited once more.
+        for (int s = 0; s < P::STAGES && ok; ++s) {
+          ok = ptx::mbar_wait_bounded(&empty[stage], phase ^ 1, it.status, it.timeout_ns);
+          if (++stage == P::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
         // Error path: let every load issued land before the CTA exits (the leader's barriers count
         // both CTAs' bytes, and the final cluster barrier holds the peer until then).
         if (!ok)
@@ -349,9 +358,8 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
             }
           }
         }
-        if (elected) ptx::mma_commit_pair(drain);  // every MMA issued so far finishes before TMEM is freed
+        if (elected) ptx::mma_commit_pair(drain);
         __syncwarp();
-        ptx::mbar_wait_bounded(drain, 0, it.status, it.timeout_ns);
       }
     }
   } else {
@@ -571,6 +579,9 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
   }
   ptx::tc_fence_before();
   __syncthreads();
+  // Every MMA issued finishes before TMEM is freed, and the leader's last commit, which arrives in both CTAs,
+  // has arrived here before this CTA may leave.
+  if (warp == 1) ptx::mbar_wait_bounded(drain, 0, it.status, it.timeout_ns);
   ptx::cluster_sync();  // neither CTA leaves before both are done with each other's memory
   if (warp == 1) {
     ptx::tc_fence_after();
