@@ -256,6 +256,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (++stage == NS) { stage = 0; phase ^= 1; }
         }
       }
+      // Pair variant: the leader's commits arrive here too, and none may be on its way when this
+      // CTA's shared memory goes: every stage is awaited once more.
+      for (int s = 0; PAIR && ok && s < NS; ++s) {
+        ok = ptx::mbar_wait_bounded(&empty[stage], phase ^ 1, a.status, a.timeout_ns);
+        if (++stage == NS) { stage = 0; phase ^= 1; }
+      }
+      if (PAIR && ok) ok = ptx::mbar_wait_bounded(a_empty, a_phase ^ 1, a.status, a.timeout_ns);
       // Let every load issued land before the CTA exits (in the pair variant the leader's
       // barriers count both CTAs' bytes, and the final cluster barrier holds the peer until then).
       if (!ok) {
@@ -405,7 +412,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       // Teardown: every MMA issued so far must finish before TMEM is freed.
       commit(drain);
-      ptx::mbar_wait_bounded(drain, 0, a.status, a.timeout_ns);
+      if (!PAIR) ptx::mbar_wait_bounded(drain, 0, a.status, a.timeout_ns);
     }
   } else {
     // ------------------------------------------------------------ epilogue
@@ -536,7 +543,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   // Pair variant: the leader's MMAs read the peer's shared memory and write its TMEM, and the
   // peer arrives on the leader's barriers; neither CTA leaves (or frees TMEM) before both are done.
-  if (PAIR) ptx::cluster_sync();
+  // The leader's last commit arrives in both CTAs, so both wait for it.
+  if (PAIR) {
+    if (warp == 1) ptx::mbar_wait_bounded(drain, 0, a.status, a.timeout_ns);
+    ptx::cluster_sync();
+  }
 #ifdef RBF_TRACE
   if (threadIdx.x == 0 && blockIdx.x < 1024) g_fwd_span[blockIdx.x][1] = ptx::globaltimer();
 #endif
