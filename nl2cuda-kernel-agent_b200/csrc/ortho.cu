@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
             if (!ok) break;
             ptx::mbar_arrive(begun);
           }
-          ptx::fence_proxy_async();
+          ptx::fence_proxy_async_global();
           for (int t = unit; t < total && ok; t += units) {
             const int z = t / tiles;
             int tm, tn;
@@ -566,6 +566,8 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
       if (!ok) break;
       // This warp's part of the product is in memory, and the CTA's once all warps have said so (a
       // count, not a barrier: a warp that gives up on a wait leaves the others to give up on theirs).
+      // TMA reads it in other CTAs: every thread's stores pass the proxy fence before the count.
+      ptx::fence_proxy_async_global();
       __syncwarp();
       if (lane == 0) {
         __threadfence_block();

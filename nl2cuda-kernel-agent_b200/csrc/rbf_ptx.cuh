@@ -181,10 +181,10 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// Order generic-proxy accesses of any memory before later async-proxy ones, and after earlier ones:
+// Order generic-proxy accesses of global memory before later async-proxy ones, and after earlier ones:
 // global data that plain stores wrote is read by TMA behind a synchronisation with such a fence on
-// both sides of it.
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
+// both sides of it, the writers' after their stores.  (Without .global it waits for shared memory too.)
+__device__ __forceinline__ void fence_proxy_async_global() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
 
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");

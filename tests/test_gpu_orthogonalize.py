@@ -276,3 +276,23 @@ def test_groups_of_steps(shape, steps, dtype, cuda_device):
     check(g, steps, [schedule[k % 4] for k in range(steps)])
     # a^2 = 225 is past what a group may carry: these two steps (15 times, then back) stand alone.
     check(g, steps, ([(15.0, 0.0, 0.0), (1 / 15, 0.0, 0.0)] + [(1.875, -1.25, 0.375)] * steps)[:steps])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (8, 64), (3, 40, 70), (4, 256, 256), (300, 1100), (2100, 1001)])
+def test_equal_calls_give_equal_bits(shape, dtype, cuda_device, monkeypatch):
+    """Calls back to back, every other one with another update (and so other contents in the workspace that
+    the next one gets): each product reads what this call's products wrote, and CTA pairs that end at
+    once leave no arrival behind for the next call."""
+    from cases.orthogonalize.op import orthogonalize
+    g, other = update(shape, dtype, sum(shape)), update(shape, dtype, 1 + sum(shape), scale=30.0)
+    want = orthogonalize(g)
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(60):
+        orthogonalize(other)
+        outs.append(orthogonalize(g))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for out in outs)
+    monkeypatch.setenv("RBF_CHECK_STATUS", "1")
+    assert torch.equal(orthogonalize(g), want)
