@@ -63,17 +63,15 @@ bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 Tensor given(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
-// The gradients of a backward pass that is not itself differentiable: differentiating them raises.
-variable_list once(variable_list out, const variable_list& upstream, const char* name) {
+// A gradient that is not itself differentiable.  Where any of the operands that it depends on requires a
+// gradient, differentiating it raises: without a graph it would count as a constant.
+Tensor once(const Tensor& grad, at::ArrayRef<Tensor> depends_on, const char* name) {
   bool again = false;
-  if (at::GradMode::is_enabled())
-    for (const auto& g : upstream) again = again || wants_grad(g);
-  if (!again) return out;
-  for (auto& t : out)
-    if (t.defined()) t = t.detach().requires_grad_(true);
-  auto error = std::make_shared<torch::autograd::DelayedError>(
-      std::string(name) + " cannot be differentiated twice", (int64_t)out.size());
-  return (*error)(std::move(out));
+  if (grad.defined() && at::GradMode::is_enabled())
+    for (const auto& t : depends_on) again = again || wants_grad(t);
+  if (!again) return grad;
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " cannot be differentiated twice", 1);
+  return (*error)({grad.detach().requires_grad_(true)})[0];
 }
 
 // --------------------------------------------------------------------------------- layer norm
@@ -170,8 +168,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const std::array<bool, 3> need = {ctx->needs_input_grad(0), has_w && ctx->needs_input_grad(1),
                                       has_b && ctx->needs_input_grad(has_w ? 2 : 1)};
     auto out = ln_backward(g[0], saved[0], saved[1], saved[2], need, (at::ScalarType)ctx->saved_data["wtype"].toInt());
-    out.emplace_back();
-    return once(std::move(out), g, "layer_norm");
+    const Tensor &x = saved[0], &w = saved[1], &dy = g[0];
+    return {once(out[0], {dy, x, w}, "layer_norm"), once(out[1], {dy, x}, "layer_norm"), once(out[2], {dy}, "layer_norm"), Tensor()};
   }
 };
 
@@ -260,8 +258,8 @@ struct TokenLogprob : torch::autograd::Function<TokenLogprob> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
-    return once({token_logprob_backward(s[0], s[1], s[2], g[0], ctx->saved_data["ignore"].toInt()), Tensor(), Tensor()},
-                g, "token_logprob");
+    const Tensor dx = token_logprob_backward(s[0], s[1], s[2], g[0], ctx->saved_data["ignore"].toInt());
+    return {once(dx, {g[0], s[0]}, "token_logprob"), Tensor(), Tensor()};
   }
 };
 
@@ -366,8 +364,9 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
     variable_list out(6);
-    out[0] = loss_backward(s[0], s[1], s[2], g[0], false, ctx->saved_data["ignore"].toInt());
-    return once(std::move(out), g, "preference_loss");
+    const Tensor dx = loss_backward(s[0], s[1], s[2], g[0], false, ctx->saved_data["ignore"].toInt());
+    out[0] = once(dx, {g[0], s[0]}, "preference_loss");
+    return out;
   }
 };
 
@@ -384,8 +383,9 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
     variable_list out(9);
-    out[0] = loss_backward(s[0], s[1], s[2], g[0], true, ctx->saved_data["ignore"].toInt());
-    return once(std::move(out), g, "policy_loss");
+    const Tensor dx = loss_backward(s[0], s[1], s[2], g[0], true, ctx->saved_data["ignore"].toInt());
+    out[0] = once(dx, {g[0], s[0]}, "policy_loss");
+    return out;
   }
 };
 
