@@ -36,7 +36,11 @@ rbf_stream_t stream_of(const Tensor& t) {
   return reinterpret_cast<rbf_stream_t>(at::cuda::getCurrentCUDAStream(t.device().index()).stream());
 }
 
-void check_cuda(const Tensor& t, const char* name) { TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor"); }
+// Every operand passes here.  There is no forward-mode derivative: a tangent would be dropped, which reads as 0.
+void check_cuda(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), name, " carries a forward-mode tangent: there is no forward-mode derivative");
+}
 
 void check_with(const Tensor& t, const char* name, const Tensor& first, const char* first_name) {
   check_cuda(t, name);

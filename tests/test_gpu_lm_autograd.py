@@ -1,7 +1,8 @@
 """What the language-model operators do not differentiate is refused, never left out: gradients of
-gradients."""
+gradients and forward-mode tangents."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +88,31 @@ def test_first_gradients_stay_plain(name, leaf, cuda_device):
     assert torch.equal(g, h)
     call(s).sum().backward()
     assert torch.equal(s[leaf].grad, g) and not s[leaf].grad.requires_grad
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "token_logprob", "preference_loss", "policy_loss", "orthogonalize"])
+def test_forward_mode_is_refused(name, cuda_device):
+    call, names = calls()[name]
+    for k in names:
+        s = operands()
+        with fwad.dual_level():
+            s[k] = fwad.make_dual(s[k], torch.ones_like(s[k]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(s)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call(s)
+    s = operands()
+    with fwad.dual_level():  # a level alone changes nothing
+        got = call(s)
+    assert torch.equal(got, call(s))
+
+
+@pytest.mark.parametrize("name,leaf", [DIFFERENTIABLE[0], DIFFERENTIABLE[1]])
+def test_tangent_of_an_upstream_gradient_is_refused(name, leaf, cuda_device):
+    call, s = calls()[name][0], operands()
+    s[leaf].requires_grad_(True)
+    y = call(s)
+    with fwad.dual_level():
+        up = fwad.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, s[leaf], up)
