@@ -37,9 +37,11 @@ rbf_stream_t stream_of(const Tensor& t) {
 }
 
 // Every operand passes here.  There is no forward-mode derivative: a tangent would be dropped, which reads as 0.
+// The kernels read an operand's bytes, which in a lazily negated view (the imaginary part of a conjugate) have the other sign.
 void check_cuda(const Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
   TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), name, " carries a forward-mode tangent: there is no forward-mode derivative");
+  TORCH_CHECK(!t.is_neg(), name, " is a lazily negated view: take its resolve_neg()");
 }
 
 void check_with(const Tensor& t, const char* name, const Tensor& first, const char* first_name) {

@@ -1,5 +1,5 @@
 """What the language-model operators do not differentiate is refused, never left out: gradients of
-gradients and forward-mode tangents."""
+gradients, forward-mode tangents, and views that are negated lazily."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
@@ -116,3 +116,16 @@ def test_tangent_of_an_upstream_gradient_is_refused(name, leaf, cuda_device):
         up = fwad.make_dual(torch.ones_like(y), torch.ones_like(y))
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(y, s[leaf], up)
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "token_logprob", "preference_loss", "policy_loss", "orthogonalize"])
+def test_lazily_negated_views(name, cuda_device):
+    """The bytes of such a view have the other sign: refused; resolved, it is taken."""
+    call, names = calls()[name]
+    for k in names:
+        s = operands()
+        s[k] = torch._neg_view(s[k])
+        with pytest.raises(RuntimeError, match="negated"):
+            call(s)
+        s[k] = s[k].resolve_neg()
+        call(s)
