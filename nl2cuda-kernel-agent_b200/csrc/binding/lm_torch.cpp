@@ -348,6 +348,7 @@ LossOut policy_forward(const Tensor& logits, const Tensor& labels, const Tensor&
 // The gradient of a loss for the upstream gradient g of its scalar.
 Tensor loss_backward(const Tensor& logits, const Tensor& labels, const Tensor& state, const Tensor& g, bool normed,
                      int64_t ignore_index) {
+  check_with(state, "state", logits, "logits");
   TORCH_CHECK(state.numel() == LossState::size(labels.numel()) && state.scalar_type() == at::kFloat && state.is_contiguous(),
               "state must be the loss's forward's");
   if (g.defined())

@@ -451,3 +451,21 @@ def test_other_streams(cuda_device):
     torch.cuda.synchronize()
     for o in outs:
         assert all(torch.equal(p, q) for p, q in zip(o, want))
+
+
+def test_state_of_another_device_is_refused(cuda_device):
+    """The backwards without autograd take the forward's state; its address has to be the GPU's."""
+    from cases.policy_loss import native as policy
+    from cases.preference_loss import native as preference
+    from cases.token_logprob import native as logprob
+    x = torch.randn(2, 3, 40, device="cuda")
+    labels, zero = torch.zeros(2, 3, dtype=torch.int64, device="cuda"), torch.zeros(2, 3, device="cuda")
+    state = preference.preference_forward(x, labels, zero, 0.1, 0.0, -100)[2]
+    with pytest.raises(RuntimeError, match="state must be a CUDA tensor"):
+        preference.preference_backward(x, labels, state.cpu(), None, -100)
+    state = policy.policy_forward(x, labels, zero, zero, torch.ones(2, device="cuda"), 0.2, 0.2, 0.0, -100)[2]
+    with pytest.raises(RuntimeError, match="state must be a CUDA tensor"):
+        policy.policy_backward(x, labels, state.cpu(), None, -100)
+    stats = logprob.logprob_forward(x, labels, -100)[1]
+    with pytest.raises(RuntimeError, match="stats must be a CUDA tensor"):
+        logprob.logprob_backward(x, labels, stats.cpu(), zero, -100)
