@@ -1,7 +1,7 @@
 """PyTorch definition of layer norm: the correctness standard of the Case.
 
-``reference_forward`` takes the mean and the variance apart, in elementary operations; its
-backward is torch autograd.
+``reference_forward`` takes the mean and the variance apart, in elementary operations and in at least
+fp32, and rounds once; its backward is torch autograd.
 """
 import torch
 
@@ -10,10 +10,12 @@ from cases.layernorm import config
 
 def reference_forward(inputs, params):
     """inputs = {"x": [..., D], "weight": [D], "bias": [D]}, params = {"eps"} -> y."""
-    x = inputs["x"]
+    dtype = inputs["x"].dtype
+    x, weight, bias = (t if t.dtype == torch.float64 else t.float()
+                       for t in (inputs["x"], inputs["weight"], inputs["bias"]))
     c = x - x.mean(dim=-1, keepdim=True)
     var = c.pow(2).mean(dim=-1, keepdim=True)
-    return c / torch.sqrt(var + params["eps"]) * inputs["weight"] + inputs["bias"]
+    return (c / torch.sqrt(var + params["eps"]) * weight + bias).to(dtype)
 
 
 def make_inputs(seed, dtype, device, requires_grad=False):

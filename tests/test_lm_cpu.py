@@ -189,3 +189,22 @@ def test_loss_definitions():
             total += 0.1 * (math.exp(d) - d - 1) - min(r * a, min(max(r, 0.8), 1.2) * a)
             n += 1
     assert abs(float(loss) - total / n) < 1e-9 and float(kl) > 0
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_layernorm_reference_rounds_once(dtype, monkeypatch):
+    """An exact implementation, 64 bits and one rounding, passes the gate in every type that the case offers."""
+    import dataclasses
+
+    from cases.layernorm import CASE, config
+    from framework.verify import verify_all
+    monkeypatch.setattr(config, "ROWS", 512)
+    monkeypatch.setattr(config, "D", 256)
+
+    def exact(inputs, params):
+        x, w, b = (inputs[k].double() for k in ("x", "weight", "bias"))
+        y = torch.nn.functional.layer_norm(x, x.shape[-1:], w, b, params["eps"])
+        return y.to(inputs["x"].dtype)
+
+    ok, report = verify_all(dataclasses.replace(CASE, dtype=dtype), exact, device="cpu")
+    assert ok, report
