@@ -298,3 +298,49 @@ def test_offsets_past_32_bits(cuda_device):
     # The other rows add zeros, in another grouping of the sums: a few fp32 roundings, then one.
     for p, q in ((dw, dws), (db, dbs)):
         assert float((p.float() - q.float()).abs().max()) <= 2.0 ** -7 * float(q.abs().max())
+
+
+# What adds up a column: a CTA's rows one after another (144 CTAs or more where there are that many rows, blocks
+# of up to 4 rows), its groups (16 at most), and the CTAs' partial sums, 32 of them side by side: ten after one
+# another, then 32.
+def column_chain(rows):
+    return -(-rows // 144) + 4 + 16 + 10 + 32
+
+
+def check_columns(rows, D, dtype, dy, seed):
+    """dweight and dbias in fp32 within the roundings of their chain of additions."""
+    from cases.layernorm import native
+    x, w, b, _ = inputs(rows, D, dtype, torch.float32, seed)
+    want = formulas(x, w, b, dy, EPS)
+    h = (x.double() - x.double().mean(1, keepdim=True)) * want[4]
+    e = 40 * U32 * (x.double().abs().amax(1, keepdim=True) * want[4] + h.abs())  # of h, as in `bounds`
+    size = dy.double().abs()
+    chain = column_chain(rows) * U32
+    _, stats = native.ln_forward(x, w, b, EPS)
+    _, dw, db = native.ln_backward(dy, x, w, stats)
+    assert_within("dw", dw, want[2], (size * e).sum(0) + chain * (size * h.abs()).sum(0) + rounded(want[2], torch.float32))
+    assert_within("db", db, want[3], chain * size.sum(0) + rounded(want[3], torch.float32))
+
+
+COLUMNS = [(40000, 136), (20000, 129), (4099, 1023), (2100, 1024), (1200, 2041), (530, 4096), (700, 4089), (520, 8189), (310, 9001),
+           (330, 6004), (200, 12290), (90, 20000), (60, 100), (33, 1001)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D", COLUMNS)
+def test_column_sums_within_their_chain(rows, D, dtype, cuda_device):
+    dy = inputs(rows, D, dtype, dtype, rows + D)[3]
+    check_columns(rows, D, dtype, dy, rows + D + 1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D", COLUMNS)
+def test_every_row_is_in_the_column_sums(rows, D, dtype, cuda_device):
+    """dy is 0 but for a few rows: the first and the last ones (every class of alignment, a CTA's last block) and
+    some between, so that the bound is a few roundings of those and a row left out shows at its full size."""
+    full = inputs(rows, D, dtype, dtype, rows * D)[3]
+    gen = torch.Generator().manual_seed(rows)
+    for some in (list(range(9)), list(range(rows - 9, rows)), torch.randint(0, rows, (8,), generator=gen).tolist()):
+        dy = torch.zeros_like(full)
+        dy[some] = full[some]
+        check_columns(rows, D, dtype, dy, rows + 3)
