@@ -831,8 +831,9 @@ __global__ void __launch_bounds__(32 * kSumRows) ln_sum_kernel(const LnArgs a, i
 }
 
 // ---- rows longer than kMaxRegD: one CTA per row, which reads it once per pass (from L2) ----------
-// HAS_W, HAS_B: the parameter is given.  An absent one has no load in the code at all: with a test
-// for NULL around the load, a row with weight but no bias faulted (an access to address 0).
+// HAS_W, HAS_B: the parameter is given.  An absent one has neither a load nor a test for NULL in the loops
+// over the row.  (The test alone is safe too, as in the other kernels, while the load behind it is a plain one: a
+// read-only load, __ldg, had been lifted above the test and read address 0.)
 
 __device__ __forceinline__ float2 block_sum2(float2 v, float2* red) {
   v.x = warp_sum(v.x);

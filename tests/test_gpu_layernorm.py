@@ -344,3 +344,12 @@ def test_every_row_is_in_the_column_sums(rows, D, dtype, cuda_device):
         dy = torch.zeros_like(full)
         dy[some] = full[some]
         check_columns(rows, D, dtype, dy, rows + 3)
+
+
+@pytest.mark.parametrize("has_w,has_b", [(True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("rows,D", [(2100, 1024), (2100, 1001), (530, 4096), (70, 6004), (70, 12288), (33, 1001), (300, 8188)])
+def test_without_parameters_on_every_path(rows, D, has_w, has_b, cuda_device):
+    """Rings of whole packs and of shifted rows, rows taken one at a time, long rows."""
+    for dtype in (torch.bfloat16, torch.float32):
+        x, w, b, dy = inputs(rows, D, dtype, torch.float32, D)
+        check(x, w if has_w else None, b if has_b else None, dy)
