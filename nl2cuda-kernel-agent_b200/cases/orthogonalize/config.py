@@ -9,14 +9,3 @@ STEPS = 5
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 EPS = 1e-7
 DTYPE = os.environ.get("ORTHO_DTYPE", "float32")
-
-
-def flops(m, n, steps=STEPS):
-    """Algorithmic FLOP: a step's X X^T and A^2 (symmetric: half of each) and B X."""
-    r, c = min(m, n), max(m, n)
-    return steps * (3 * r * r * c + r ** 3)
-
-
-def hbm_bytes(m, n, elem=4):
-    """Bytes that cannot be avoided: the update read, the result written."""
-    return 2 * m * n * elem

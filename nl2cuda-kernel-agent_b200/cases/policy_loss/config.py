@@ -9,9 +9,3 @@ CLIP_LOW = 0.2
 CLIP_HIGH = 0.2
 KL_COEF = 0.05
 DTYPE = os.environ.get("POLICY_DTYPE", "float32")
-
-
-def hbm_bytes(scored, rows, v, elem=4):
-    """Algorithmic HBM bytes of one forward + backward: both read the scored rows, the backward
-    writes every row's gradient."""
-    return elem * v * (2 * scored + rows)

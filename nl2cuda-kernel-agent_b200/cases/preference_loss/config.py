@@ -8,9 +8,3 @@ IGNORE_INDEX = -100
 BETA = 0.1
 LABEL_SMOOTHING = 0.0
 DTYPE = os.environ.get("PREF_DTYPE", "float32")
-
-
-def hbm_bytes(scored, rows, v, elem=4):
-    """Algorithmic HBM bytes of one forward + backward: both read the scored rows, the backward
-    writes every row's gradient."""
-    return elem * v * (2 * scored + rows)

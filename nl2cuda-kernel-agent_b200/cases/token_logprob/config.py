@@ -6,9 +6,3 @@ T = int(os.environ.get("LP_T", "64"))     # positions of each
 V = int(os.environ.get("LP_V", "8192"))   # vocabulary
 IGNORE_INDEX = -100
 DTYPE = os.environ.get("LP_DTYPE", "float32")
-
-
-def hbm_bytes(scored, rows, v, elem=4):
-    """Algorithmic HBM bytes of one forward + backward: both read the scored rows, the backward
-    writes every row's gradient."""
-    return elem * v * (2 * scored + rows)

@@ -1063,7 +1063,9 @@ bool ring_fits(const LnArgs& a, bool backward) {
 // Other rows, where the matrices start on 16 bytes and their rows shift alike: up to four packs a thread in the
 // forward, 4096 x 9001 bf16 in 96 us (212 with loads of single values); up to two in the backward, 8192 x 8175 bf16
 // in 171 us (ln_long_backward_kernel: 212), while with four 4096 x 9001 takes 266 (137).  With two packs of which
-// many lie past the row it is the slower one: 8192 x 4500 bf16 138 us (97), 8192 x 6001 149 (155).
+// many lie past the row it is the slower one: 8192 rows of 4500 bf16 values 138 us (97), 5001 143 (133), 5700 142 (109),
+// 6100 148 (113).  Odd lengths near the upper end are about even: 8192 x 5801 145 (149), 8192 x 6001 149 (158), 1000 x 6001
+// 31.4 (30.7).
 constexpr int64_t kShiftMinRows = 64;  // eight classes of a few rows (no slower than the other path from there on)
 bool shift_fits(const LnArgs& a, bool backward) {
   const int64_t vec = 16 / (int64_t)elem_bytes(a.dtype);

@@ -781,7 +781,7 @@ __global__ void __launch_bounds__(256) ortho_split_kernel(const PrepArgs a) {
   ptx::griddep_launch_dependents();
   const int64_t z = blockIdx.z;
   const int64_t i0 = (int64_t)blockIdx.y * kTile, j0 = (int64_t)blockIdx.x * kTile;
-  // 8 columns of two rows a thread; the loads do not wait for the norm.
+  // 8 columns of two rows a thread, on their way while the norm's partial sums are added.
   const int cx = (threadIdx.x & 7) * 8, ry = threadIdx.x >> 3;
   Pack<T, 8> p[2];
 #pragma unroll

@@ -33,6 +33,9 @@ struct MaxSum {
   float m, s;
 };
 
+// For a term of the gradient: three roundings (the difference, log2 e, the product) leave it off by 1.3e-7 |x - m|
+// of itself at most, 1.3e-6 of a term that is e^-10 of the row's largest.  A single term, unlike the sum below, gains
+// nothing from more.
 __device__ __forceinline__ float exp_diff(float x, float m) { return exp2_approx((x - m) * kLog2e); }
 
 // For the sum: with what log2 e loses in fp32 (1.3e-8 of it), which makes every term of a given size
