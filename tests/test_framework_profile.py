@@ -47,6 +47,23 @@ def test_ncu_section_captures_name_one_kernel_each():
         assert f"-k regex:{k}" in c and " -c 3 " in c
 
 
+def test_ncu_commands_refuse_what_does_not_run_under_it(capsys):
+    with pytest.raises(ValueError, match="LaunchFailed"):
+        profile.ncu_commands("orthogonalize", None)
+    with pytest.raises(SystemExit) as e:
+        profile.main(["--case", "orthogonalize", "--ncu-commands"])
+    out = capsys.readouterr()
+    assert e.value.code != 0 and "ncu " not in out.out and "LaunchFailed" in out.err
+    for case in ("layernorm", "token_logprob", "preference_loss", "policy_loss"):
+        assert not any("ortho" in c for c in profile.ncu_commands(case, None))
+
+
+def test_smoke_launches_nothing_that_does_not_run_under_ncu():
+    """The smoke run is listed under ncu as a whole."""
+    import __graft_entry__ as entry
+    assert not set(entry.SMOKE_OPERATORS) & set(profile.NOT_CAPTURED)
+
+
 def test_cli_summaries(capsys):
     assert profile.main(["--launches", os.path.join(FIX, "ncu_launches_sample.csv")]) == 0
     assert "kern_b" in capsys.readouterr().out
