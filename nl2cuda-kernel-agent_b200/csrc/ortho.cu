@@ -26,9 +26,11 @@
 // low by half a unit per MMA: 1.8e-5 of the result at a depth of 2601.  So an accumulator takes a
 // run of slices only, and the epilogue warps add these partial sums in registers, rounded to nearest.
 // The products with lo, two thirds of the MMAs but 2^-11 of the sum, go to an accumulator of their own
-// where there is room for one.  2601 x 1001 fp32, runs 128, 192 and 256 deep: error 2.9e-6, 4.0e-6 and
-// 5.1e-6 (the fp32 library products': 3.3e-6) in 472, 410 and 364 us; 192 is taken.  fp16 and bf16
-// results, whose own rounding is far larger, take 1024 and 2048.
+// where there is room for one.  fp32 results: products of up to 3 slices add up every slice, those of up to 24
+// every second, longer ones every third.  Errors (and the fp32 library products'), with runs of three throughout and
+// with these: 2601 x 1001 4.1e-6 and 2.8e-6 (3.3e-6) in 383 and 418 us, 365 x 1135 3.7e-6 and 2.7e-6 (2.3e-6) in
+// 245 and 275, 120 x 834 3.2e-6 and 1.9e-6 (1.5e-6) in 142 and 158, 130 x 4000 2.9e-6 and 1.8e-6 (1.3e-6) in 247
+// and 261.  fp16 and bf16 results, whose own rounding is far larger, take 1024 and 2048 values.
 //
 // Kernel: one launch runs the whole iteration (cooperative, one CTA per SM).  A product's tiles are
 // shared out over the CTA pairs; each CTA counts itself in when its part is stored, and the loads of
@@ -91,6 +93,7 @@ struct Split {
 struct Op {
   uint8_t kind, p, q, d, t, add;  // matrices: the operands, where D and its transpose go, what is added
   uint8_t out_kind;
+  uint8_t run;                    // slices that share a TMEM accumulator
   int tiles;                      // of one matrix of the batch
 };
 
@@ -104,7 +107,6 @@ struct IterArgs {
   Split mat[kMatrices];
   Op op[kMaxOps];
   int ops, batch;
-  int run;                        // slices that share a TMEM accumulator
   int out_dtype;
   void* out;                      // of the last product: out[column * ld_out + row]
   int64_t ld_out, out_matrix;
@@ -319,14 +321,14 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
         for (int p = 0; p < products && ok; ++p) {
           const Op op = it.op[p];
           const int num_kc = (int)((it.mat[op.p].cols + BK - 1) / BK), total = op.tiles * it.batch;
-          // A unit of work is one run of it.run stages of a tile: each has an accumulator of its own.
-          const int runs = (num_kc + it.run - 1) / it.run;
+          // A unit of work is one run of op.run stages of a tile: each has an accumulator of its own.
+          const int runs = (num_kc + op.run - 1) / op.run;
           for (int t = unit; t < total && ok; t += units) {
             for (int run = 0; run < runs && ok; ++run) {
               if (!ptx::mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1, it.status, it.timeout_ns)) { ok = false; break; }
               ptx::tc_fence_after();
               const uint32_t d = tmem + (uint32_t)acc * P::ACC;
-              const int depth = min(it.run, num_kc - run * it.run);
+              const int depth = min((int)op.run, num_kc - run * op.run);
               for (int kc = 0; kc < depth; ++kc) {
                 if (!ptx::mbar_wait_bounded(&full[stage], phase, it.status, it.timeout_ns)) { ok = false; break; }
                 ptx::tc_fence_after();
@@ -377,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
       const int num_kc = (int)((it.mat[op.p].cols + BK - 1) / BK);
       const int tiles_m = (int)((M + kTileRows - 1) / kTileRows), tiles_n = (int)((N + BN - 1) / BN);
       const int total = op.tiles * it.batch;
-      const int runs = (num_kc + it.run - 1) / it.run;
+      const int runs = (num_kc + op.run - 1) / op.run;
       const bool sym = op.out_kind == kSymmetric;
       const bool adds = op.add != kNone;
       const Split d = it.mat[op.d], dt = it.mat[op.t], add = it.mat[adds ? op.add : mA];
@@ -885,7 +887,7 @@ int group_size(const float* coef, int step, int steps) {
 int list_ops(bool tall, bool whole, bool grouped, const float* coef, int steps, Op* op) {
   int n = 0, xt = mXT0;
   auto put = [&](int kind, int p, int q, int d, int t, int out_kind, int add = kNone) {
-    op[n++] = Op{(uint8_t)kind, (uint8_t)p, (uint8_t)q, (uint8_t)d, (uint8_t)t, (uint8_t)add, (uint8_t)out_kind, 0};
+    op[n++] = Op{(uint8_t)kind, (uint8_t)p, (uint8_t)q, (uint8_t)d, (uint8_t)t, (uint8_t)add, (uint8_t)out_kind, 0, 0};
   };
   for (int step = 0; step < steps;) {
     const int size = grouped ? group_size(coef, step, steps) : 1;
@@ -1035,6 +1037,12 @@ int64_t estimate(const IterArgs& it, const Op* op, int ops, int bn) {
   return cost;
 }
 
+// Slices that share an accumulator, of a product of `slices`: see the truncation above.
+int run_of(int dtype, int64_t slices) {
+  if (dtype != LM_F32) return dtype == LM_F16 ? 16 : 32;
+  return slices <= 3 ? 1 : slices <= 24 ? 2 : 3;
+}
+
 // The products and the tile width with the least estimated time.
 int plan(IterArgs& it, bool tall, bool whole, bool may_group, const float* coef, int steps) {
   Op op[kMaxOps];
@@ -1128,7 +1136,7 @@ cudaError_t launch_orthogonalize(const OrthoArgs& o, const WaitConfig& wc, cudaS
   cudaError_t e = o.dtype == LM_F32 ? by_pack(float{}) : o.dtype == LM_BF16 ? by_pack(__nv_bfloat16{}) : by_pack(__half{});
   if (e != cudaSuccess) return e;
 
-  it.run = o.dtype == LM_F32 ? 3 : o.dtype == LM_F16 ? 16 : 32;
+  for (int i = 0; i < it.ops; ++i) it.op[i].run = (uint8_t)run_of(o.dtype, ceil_div(it.mat[it.op[i].p].cols, BK));
   it.out = o.out;
   it.ld_out = o.cols;
   it.out_matrix = o.rows * o.cols;
