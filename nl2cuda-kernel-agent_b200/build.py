@@ -7,6 +7,8 @@ __graft_entry__.build(), by framework/loader.py (rebuild when a source is newer 
 and directly:  python nl2cuda-kernel-agent_b200/build.py [--verbose] [--ptxas-info]
 """
 import argparse
+import contextlib
+import fcntl
 import glob
 import os
 import subprocess
@@ -77,6 +79,16 @@ def build_binding(verbose=False):
     subprocess.run(cmd, check=True)
     os.replace(out + ".tmp", out)
     return out
+
+
+@contextlib.contextmanager
+def exclusive():
+    """One process at a time: ranks that start together find the same file stale, and would write the
+    same objects and the same temporary file."""
+    os.makedirs(BUILD, exist_ok=True)
+    with open(os.path.join(BUILD, ".lock"), "w") as f:
+        fcntl.flock(f, fcntl.LOCK_EX)  # released with the file
+        yield
 
 
 def headers():

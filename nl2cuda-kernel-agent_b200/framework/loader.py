@@ -59,8 +59,10 @@ def load_kernel(name, sources=None, base_dir=None, extra_cuda_cflags=None, extra
             if shutil.which(_build.NVCC) is None and not os.path.exists(path):
                 raise RuntimeError(f"{path} is missing and nvcc is not available to build it")
             if shutil.which(_build.NVCC) is not None:
-                _build.build(verbose=verbose, name=name, srcs=srcs,
-                             extra_cuda_cflags=extra_cuda_cflags)
+                with _build.exclusive():
+                    if _build.stale(name, srcs):  # another process may have built it meanwhile
+                        _build.build(verbose=verbose, name=name, srcs=srcs,
+                                     extra_cuda_cflags=extra_cuda_cflags)
         lib = ctypes.CDLL(path)
         _loaded[name] = lib
         return lib
@@ -76,7 +78,9 @@ def load_torch_binding():
         path = _build.binding_path()
         if _build.binding_stale():
             if shutil.which(os.environ.get("CXX", "g++")) is not None:
-                _build.build_binding()
+                with _build.exclusive():
+                    if _build.binding_stale():
+                        _build.build_binding()
             elif not os.path.exists(path):
                 raise RuntimeError(f"{path} is missing and there is no C++ compiler to build it")
         import torch  # noqa: F401  (the module's symbols come from torch's libraries)
