@@ -353,3 +353,20 @@ def test_without_parameters_on_every_path(rows, D, has_w, has_b, cuda_device):
     for dtype in (torch.bfloat16, torch.float32):
         x, w, b, dy = inputs(rows, D, dtype, torch.float32, D)
         check(x, w if has_w else None, b if has_b else None, dy)
+
+
+@pytest.mark.parametrize("rows,D", [(2100, 1024), (2100, 1001), (530, 4096), (70, 12288)])
+def test_nan_stays_in_its_row_of_a_block(rows, D, cuda_device):
+    """Rows share blocks, reductions and 16-byte packs with their neighbours, but no values."""
+    from cases.layernorm import native
+    x, w, b, dy = inputs(rows, D, torch.bfloat16, torch.bfloat16, 11)
+    y, stats = native.ln_forward(x, w, b, EPS)
+    dx = native.ln_backward(dy, x, w, stats, (True, False, False))[0]
+    bad = [1, 6, rows // 2, rows - 1]
+    x[bad, 0], x[bad, D - 1] = float("nan"), float("inf")
+    yb, sb = native.ln_forward(x, w, b, EPS)
+    dxb = native.ln_backward(dy, x, w, sb, (True, False, False))[0]
+    fine = torch.ones(rows, dtype=torch.bool, device="cuda")
+    fine[bad] = False
+    assert torch.isnan(yb[bad]).all() and torch.isnan(dxb[bad]).all()
+    assert torch.equal(yb[fine], y[fine]) and torch.equal(dxb[fine], dx[fine])
