@@ -6,6 +6,7 @@
 // ordinary call take 5 to 50 us: the same binding through ctypes and Python autograd functions
 // cost 150 to 230 us of host time for a forward and a backward.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -439,7 +440,9 @@ Tensor orthogonalize(const Tensor& update, const std::vector<float>& coefficient
                     ptr(ws), bytes, stream_of(update)),
         "ortho_sm100");
   const char* env = std::getenv("RBF_CHECK_STATUS");
-  if (env != nullptr && *env != '\0' && std::string(env) != "0" && out.numel() > 0) {
+  // Not while the stream is captured: there is nothing to read yet, and waiting would end the capture.
+  if (env != nullptr && *env != '\0' && std::string(env) != "0" && out.numel() > 0 &&
+      c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) {
     int status = 0;
     check(rbf_sm100_read_status(ptr(ws), stream_of(update), &status), "rbf_sm100_read_status");
     TORCH_CHECK(status == 0, "orthogonalize: device status ", status, " (a bounded device-side wait timed out)");

@@ -323,3 +323,18 @@ def test_fp32_is_as_exact_as_fp32_products(shape, cuda_device):
 
     got = error(orthogonalize(g))
     assert got <= 1.5 * error(plain), (got, error(plain))
+
+
+def test_status_is_not_read_inside_a_capture(cuda_device, monkeypatch):
+    from cases.orthogonalize.op import orthogonalize
+    monkeypatch.setenv("RBF_CHECK_STATUS", "1")
+    g = update((100, 300), torch.bfloat16, 4)
+    want = orthogonalize(g)
+    static = torch.zeros_like(g)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = orthogonalize(static)
+    static.copy_(g)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
