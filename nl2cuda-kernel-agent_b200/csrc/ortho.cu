@@ -35,7 +35,7 @@
 // Kernel: one launch runs the whole iteration (cooperative, one CTA per SM).  A product's tiles are
 // shared out over the CTA pairs; each CTA counts itself in when its part is stored, and the loads of
 // the next product wait until all have.  A launch for each product took 11 us from one to the next on a
-// batch of four of 256 x 256; this takes 7.5.  Warp 0 loads operand slices by TMA (64 deep, 128-byte
+// batch of four of 256 x 256; this takes 7.2.  Warp 0 loads operand slices by TMA (64 deep, 128-byte
 // swizzle, hi and lo of both operands) into a ring of stages; warp 1 issues 3 x 4 MMAs per stage into one
 // of the TMEM accumulators; warps 4..11 read the others, apply the epilogue and store.  All
 // on CTA pairs (cta_group::2), tiles of 256 x 256, 128 or 64: a CTA of the pair loads its 128 rows of P
